@@ -44,6 +44,7 @@ extern "C" {
 #define MN_STATUS_DEGENERATE_RANGE 2 /* ThreTopK global max == min */
 #define MN_STATUS_TOO_MANY_EDGES 4
 #define MN_STATUS_TC_TIMEOUT 256     /* a bounded tensor-core wait gave up */
+#define MN_STATUS_BAD_LENGTHS 512    /* packed sequences: offsets or lengths out of range */
 
 /* GEMM epilogues (mn_gemm_f16) */
 #define MN_EPI_BIAS 0       /* fp16(acc + bias) */
@@ -312,6 +313,79 @@ int mn_attention(int batch, int nq, int nk, int heads, int head_dim, int dtype,
                  const void* k, const void* v, int64_t kv_sb, int64_t kv_sn,
                  int64_t kv_sh, int window, float scale, void* out,
                  int out_dtype, int* status, void* stream);
+
+/* Attention over packed sequences of different lengths, with grouped heads,
+ * an optional causal mask and an optional learned bias by distance buckets.
+ *
+ * Sequence b owns the query rows cu_q[b] .. cu_q[b + 1] and the key rows
+ * cu_k[b] .. cu_k[b + 1], of which the first len_k[b] are in use (all of them
+ * when len_k is NULL).  With nq and nk of them, query i stands at position
+ * i + nk - nq among the keys: the last query meets the last key.  causal
+ * hides keys behind that position.  Head h reads key head h / (heads /
+ * kv_heads).  For query i, key j, head h:
+ *   x_ij = scale q_i . k_j + table[bucket(j - (i + nk - nq)), h]
+ *   out_i = sum_j softmax_j(x_ij) v_j        (0 where no key is seen)
+ * Query rows of no sequence (from cu_q[nseq] on) come out as 0.
+ *
+ * bucket(r): with two_sided, n = |r| and keys ahead (r > 0) take the second
+ * half of the buckets; otherwise n = max(-r, 0).  The bucket of n is the
+ * number of borders <= n.  borders is a host array, read during the call,
+ * ascending, of one side's bucket count - 1 entries.
+ *
+ * q [tq, heads, head_dim], k and v [tk, kv_heads, head_dim] with element
+ * strides (_st per row, _sh per head) and contiguous channels, fp16 or bf16;
+ * head_dim a multiple of 8 up to 128; pointers 16-byte aligned and strides
+ * multiples of 8.  out, dq, dk, dv: contiguous, of the same type.  bias_table
+ * [buckets, heads] contiguous, of bias_dtype; dbias fp32, the same shape.
+ * lse [kv_heads, tq, heads / kv_heads] fp32: log2 of each row's sum of
+ * exponentials (+inf where no key is seen); NULL when no backward follows. */
+typedef struct mn_packed_args {
+  const void *q, *k, *v;
+  const int32_t *cu_q, *cu_k, *len_k;
+  const void* bias_table;
+  const int32_t* borders;
+  void* out;
+  float* lse;
+  /* backward only */
+  const void* dout;
+  void *dq, *dk, *dv;
+  float* dbias;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, do_st, do_sh;
+  int32_t nseq, tq, tk, heads, kv_heads, head_dim, dtype, causal;
+  int32_t bias_dtype, buckets, two_sided, num_borders;
+  float scale;
+  int32_t reserved;
+} mn_packed_args;
+
+size_t mn_packed_attention_workspace_bytes(const mn_packed_args* args);
+int mn_packed_attention(const mn_packed_args* args, void* workspace,
+                        size_t workspace_bytes, int* status, void* stream);
+
+/* Gradients of mn_packed_attention: reads its out and lse and dout, writes
+ * dq, dk, dv (rows of no sequence and unused key rows get 0) and, with a
+ * bias_table, dbias.  Every sum has a fixed order. */
+size_t mn_packed_attention_backward_workspace_bytes(const mn_packed_args* args);
+int mn_packed_attention_backward(const mn_packed_args* args, void* workspace,
+                                 size_t workspace_bytes, int* status,
+                                 void* stream);
+
+/* bias[h, i, j] = table[bucket(j - (i + query_start)), h] for queries x keys
+ * positions, and the table's gradient: dtable[u, h] = the sum of dbias[h, i,
+ * j] over the positions of bucket u, in a fixed order and fp32.  table
+ * [buckets, heads], bias and dbias [heads, queries, keys], all contiguous and
+ * of one dtype; dtable fp32 [buckets, heads].  Buckets as above. */
+int mn_relative_bias(int heads, int queries, int keys, int query_start,
+                     int buckets, int two_sided, int num_borders,
+                     const int32_t* borders, int dtype, const void* table,
+                     void* bias, void* stream);
+size_t mn_relative_bias_backward_workspace_bytes(int heads, int queries,
+                                                 int keys, int buckets);
+int mn_relative_bias_backward(int heads, int queries, int keys,
+                              int query_start, int buckets, int two_sided,
+                              int num_borders, const int32_t* borders,
+                              int dtype, const void* dbias, float* dtable,
+                              void* workspace, size_t workspace_bytes,
+                              void* stream);
 
 /* LayerNorm(x + y) written in fp32 (y 16-bit of type half_dtype, optional):
  * the latent encoder's final norm over every carrier row, which fp16 / bf16

@@ -33,5 +33,6 @@ from .attention import (  # noqa: F401
     local_attention_packed,
     unbiased_local_attention,
 )
+from .packed import RelativeBuckets, packed_attention, relative_position_bias  # noqa: F401
 
 __version__ = "0.1.0"

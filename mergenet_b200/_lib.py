@@ -20,6 +20,7 @@ MN_ERR_ARG, MN_ERR_UNSUPPORTED, MN_ERR_WORKSPACE, MN_ERR_LAUNCH = -1, -2, -3, -4
 MN_INFEASIBLE_BUDGET = 1
 MN_STATUS_INFEASIBLE_BUDGET, MN_STATUS_DEGENERATE_RANGE, MN_STATUS_TOO_MANY_EDGES = 1, 2, 4
 MN_STATUS_TC_TIMEOUT = 256
+MN_STATUS_BAD_LENGTHS = 512
 MN_EPI_BIAS = 0
 MN_EPI_BIAS_GELU = 1
 
@@ -42,6 +43,20 @@ class RouteDims(ctypes.Structure):
 
 
 _P = c_void_p
+
+
+class PackedArgs(ctypes.Structure):
+    """mn_packed_args, in the header's order."""
+    _fields_ = (
+        [(n, c_void_p) for n in ("q", "k", "v", "cu_q", "cu_k", "len_k", "bias_table", "borders", "out", "lse", "dout",
+                                 "dq", "dk", "dv", "dbias")]
+        + [(n, c_int64) for n in ("q_st", "q_sh", "k_st", "k_sh", "v_st", "v_sh", "do_st", "do_sh")]
+        + [(n, c_int) for n in ("nseq", "tq", "tk", "heads", "kv_heads", "head_dim", "dtype", "causal", "bias_dtype",
+                                "buckets", "two_sided", "num_borders")]
+        + [("scale", c_float), ("reserved", c_int)]
+    )
+
+
 _SIGNATURES = {
     "mn_version": (c_int, []),
     "mn_neighbor_table_width": (c_int, [c_int, c_int, c_double, POINTER(c_int)]),
@@ -80,6 +95,14 @@ _SIGNATURES = {
                                    c_int, c_int, c_int, c_float, _P, c_int, _P, _P]),
     "mn_attention": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, _P, c_int64, c_int64, c_int64, _P, _P,
                              c_int64, c_int64, c_int64, c_int, c_float, _P, c_int, _P, _P]),
+    "mn_packed_attention_workspace_bytes": (c_size_t, [POINTER(PackedArgs)]),
+    "mn_packed_attention": (c_int, [POINTER(PackedArgs), _P, c_size_t, _P, _P]),
+    "mn_packed_attention_backward_workspace_bytes": (c_size_t, [POINTER(PackedArgs)]),
+    "mn_packed_attention_backward": (c_int, [POINTER(PackedArgs), _P, c_size_t, _P, _P]),
+    "mn_relative_bias": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, c_int, _P, _P, _P]),
+    "mn_relative_bias_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "mn_relative_bias_backward": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, c_int, _P, _P, _P,
+                                          c_size_t, _P]),
     "mn_add_layernorm": (c_int, [c_int64, c_int, _P, _P, _P, _P, c_float, _P, _P, _P, c_int, _P]),
     "mn_add_layernorm_f32": (c_int, [c_int64, c_int, _P, _P, _P, _P, c_float, _P, c_int, _P]),
     "mn_embed_layernorm": (c_int, [c_int, c_int, c_int, _P, _P, _P, _P, _P, c_float, _P, _P, c_int, _P]),

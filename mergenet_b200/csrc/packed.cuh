@@ -1,0 +1,84 @@
+// What the kernels of the packed attention share: the sequences' offsets and
+// the bucket of a distance.
+#pragma once
+
+#include "common.cuh"
+
+namespace mn {
+
+constexpr int kMaxBorders = 127;
+
+// Ascending distances at which the next bucket begins (passed by value).
+struct Borders {
+  int n;
+  int two_sided;
+  int side;  // buckets to a side
+  int at[kMaxBorders];
+};
+
+// Bucket of r = key position - query position: the number of borders at or
+// below the distance; keys ahead take the second side.
+__device__ __forceinline__ int bucket_of(const Borders& b, int r) {
+  const int n = b.two_sided ? abs(r) : max(-r, 0);
+  int u = 0;
+  for (int i = 0; i < b.n; ++i) u += b.at[i] <= n ? 1 : 0;
+  return u + (b.two_sided && r > 0 ? b.side : 0);
+}
+
+// false when the arguments describe no valid buckets
+inline bool make_borders(Borders* b, int buckets, int two_sided, int num_borders, const int32_t* at) {
+  b->two_sided = two_sided ? 1 : 0;
+  b->side = two_sided ? buckets / 2 : buckets;
+  b->n = num_borders;
+  if (buckets < 1 || (two_sided && buckets % 2) || num_borders != b->side - 1 || num_borders > kMaxBorders ||
+      (num_borders > 0 && !at))
+    return false;
+  for (int i = 0; i < num_borders; ++i) {
+    if (at[i] < 1 || (i > 0 && at[i] < at[i - 1])) return false;
+    b->at[i] = at[i];
+  }
+  return true;
+}
+
+// One sequence: query rows [q0, q0 + nq), key rows [k0, k0 + nk) of a slot of
+// `slot` rows.  Offsets are clamped to the tensors, so that whatever they hold
+// no access leaves them.
+struct Seq {
+  int q0, nq, k0, nk, slot;
+};
+
+__device__ __forceinline__ Seq load_seq(const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, int b, int tq,
+                                        int tk) {
+  Seq s;
+  s.q0 = min(max(cu_q[b], 0), tq);
+  s.nq = min(max(cu_q[b + 1], s.q0), tq) - s.q0;
+  s.k0 = min(max(cu_k[b], 0), tk);
+  s.slot = min(max(cu_k[b + 1], s.k0), tk) - s.k0;
+  s.nk = len_k ? min(max(len_k[b], 0), s.slot) : s.slot;
+  return s;
+}
+
+// Index of the sequence that holds `row` by the ends cu[1..n], or n.
+__device__ __forceinline__ int seq_of_row(const int32_t* cu, int n, int row) {
+  int lo = 0, hi = n;  // first b with cu[b + 1] > row
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid + 1] > row) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// Data condition of the offsets, looked at by one thread block.
+__device__ __forceinline__ bool bad_lengths(const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, int n, int tq,
+                                            int tk, int first, int step) {
+  bool bad = false;
+  for (int b = first; b < n; b += step) {
+    const int q0 = cu_q[b], q1 = cu_q[b + 1], k0 = cu_k[b], k1 = cu_k[b + 1];
+    bad |= q0 < 0 || q1 < q0 || q1 > tq || k0 < 0 || k1 < k0 || k1 > tk || (b == 0 && (q0 != 0 || k0 != 0));
+    if (len_k) bad |= len_k[b] < 0 || len_k[b] > k1 - k0;
+  }
+  return bad;
+}
+
+}  // namespace mn
