@@ -24,7 +24,7 @@ BUILD = ROOT / "_build"
 LIB = PKG / "libmergenet_b200.so"
 
 SOURCES = ["tables.cpp", "route.cu", "dropin.cu", "attention.cu", "attention_tc.cu", "attention_ws.cu", "norm.cu", "gemm_tc.cu", "carrier_train.cu",
-           "packed_attention.cu", "relative_bias.cu"]
+           "packed_forward.cu", "packed_backward.cu", "relative_bias.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
               "-Xptxas", "-warn-spills"]

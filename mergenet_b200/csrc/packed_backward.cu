@@ -1,13 +1,12 @@
-// Attention over packed sequences of different lengths (mn_packed_attention)
-// and its gradients: one warp per query row and head (forward, dq) or per key
-// row and key head (dk, dv), the channels over the lanes, an online softmax.
-#include "packed.cuh"
+// Gradients of the packed attention (mn_packed_attention_backward): one warp
+// per query row and head (dq) or per key row and key head (dk, dv), the
+// channels over the lanes.
+#include "packed_tc.cuh"
 
 namespace mn {
 namespace pk {
 
 constexpr int kThreads = 128;
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 __device__ __forceinline__ void load_row(const T* p, int d, int lane, float (&x)[4]) {
@@ -22,39 +21,6 @@ __device__ __forceinline__ void store_row(T* p, int d, int lane, const float (&x
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (lane + 32 * i < d) p[lane + 32 * i] = from_f32<T>(x[i] * f);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) forward_kernel(mn_packed_args a, Borders bo, int* err) {
-  const int lane = threadIdx.x & 31;
-  if (blockIdx.x == 0 && err && bad_lengths(a.cu_q, a.cu_k, a.len_k, a.nseq, a.tq, a.tk, threadIdx.x, kThreads))
-    atomicOr(err, MN_STATUS_BAD_LENGTHS);
-  const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (w >= (int64_t)a.tq * a.heads) return;
-  const int t = (int)(w / a.heads), h = (int)(w % a.heads), g = a.heads / a.kv_heads, hk = h / g, d = a.head_dim;
-  const int b = seq_of_row(a.cu_q, a.nseq, t);
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  if (b < a.nseq) {
-    const Seq s = load_seq(a.cu_q, a.cu_k, a.len_k, b, a.tq, a.tk);
-    const int pos = t - s.q0 + s.nk - s.nq;
-    const int end = a.causal ? min(s.nk, pos + 1) : s.nk;
-    float q[4], k[4], v[4];
-    load_row(static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh, d, lane, q);
-    for (int j = 0; j < end; ++j) {
-      load_row(static_cast<const T*>(a.k) + (int64_t)(s.k0 + j) * a.k_st + hk * a.k_sh, d, lane, k);
-      load_row(static_cast<const T*>(a.v) + (int64_t)(s.k0 + j) * a.v_st + hk * a.v_sh, d, lane, v);
-      float x = dot4(q, k) * a.scale;
-      if (a.bias_table) x += load_any(a.bias_table, a.bias_dtype, bucket_of(bo, j - pos) * a.heads + h);
-      x *= kLog2e;
-      const float mn = fmaxf(m, x), c = m == -INFINITY ? 0.f : exp2f(m - mn), p = exp2f(x - mn);
-      l = l * c + p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * c + p * v[i];
-      m = mn;
-    }
-  }
-  store_row(static_cast<T*>(a.out) + ((int64_t)t * a.heads + h) * d, d, lane, acc, l > 0.f ? 1.f / l : 0.f);
-  if (a.lse && lane == 0) a.lse[((int64_t)hk * a.tq + t) * g + h % g] = l > 0.f ? m + log2f(l) : INFINITY;
 }
 
 // dq, each row's delta, and each row's sums of ds by bucket (part)
@@ -152,47 +118,12 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(mn_packed_args a, Borders
   store_row(static_cast<T*>(a.dv) + ((int64_t)row * a.kv_heads + hk) * d, d, lane, dv, 1.f);
 }
 
-static int check(const mn_packed_args* a, Borders* bo, bool backward) {
-  if (!a || a->nseq < 1 || a->tq < 0 || a->tk < 0 || a->heads < 1 || a->kv_heads < 1) return MN_ERR_ARG;
-  if (a->heads % a->kv_heads || a->head_dim < 1 || !(a->scale > 0.f) || !(a->scale < INFINITY)) return MN_ERR_ARG;
-  if (!a->cu_q || !a->cu_k || (a->tq > 0 && (!a->q || !a->out)) || (a->tk > 0 && (!a->k || !a->v))) return MN_ERR_ARG;
-  if (backward && a->tq > 0 && (!a->dout || !a->lse || !a->dq)) return MN_ERR_ARG;
-  if (backward && a->tk > 0 && (!a->dk || !a->dv)) return MN_ERR_ARG;
-  if (a->dtype != MN_F16 && a->dtype != MN_BF16) return MN_ERR_UNSUPPORTED;
-  const int g = a->heads / a->kv_heads;
-  if (a->head_dim > 128 || a->head_dim % 8 || g > 128) return MN_ERR_UNSUPPORTED;
-  if ((int64_t)a->tq * g >= (1 << 30) || (int64_t)a->tk * g >= (1 << 30)) return MN_ERR_UNSUPPORTED;
-  bo->n = 0;
-  if (a->bias_table) {
-    if (a->bias_dtype < 0 || a->bias_dtype > 2 || (backward && !a->dbias)) return MN_ERR_ARG;
-    if (!make_borders(bo, a->buckets, a->two_sided, a->num_borders, a->borders)) return MN_ERR_ARG;
-    const int last = bo->n ? bo->at[bo->n - 1] : 1;
-    if (a->buckets > 64 || ((a->two_sided ? 2 : 1) * (int64_t)last + 1) * g > 8192) return MN_ERR_UNSUPPORTED;
-  }
-  return MN_OK;
-}
-
 static unsigned blocks(int64_t warps) { return (unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)); }
 
 }  // namespace pk
 }  // namespace mn
 
 using namespace mn;
-
-extern "C" size_t mn_packed_attention_workspace_bytes(const mn_packed_args*) { return 0; }
-
-extern "C" int mn_packed_attention(const mn_packed_args* args, void*, size_t, int* status, void* stream) {
-  Borders bo;
-  const int rc = pk::check(args, &bo, false);
-  if (rc != MN_OK) return rc;
-  if (args->tq == 0) return MN_OK;
-  cudaGetLastError();
-  const unsigned n = pk::blocks((int64_t)args->tq * args->heads);
-  auto st = static_cast<cudaStream_t>(stream);
-  if (args->dtype == MN_F16) pk::forward_kernel<__half><<<n, pk::kThreads, 0, st>>>(*args, bo, status);
-  else pk::forward_kernel<__nv_bfloat16><<<n, pk::kThreads, 0, st>>>(*args, bo, status);
-  return cudaGetLastError() == cudaSuccess ? MN_OK : MN_ERR_LAUNCH;
-}
 
 extern "C" size_t mn_packed_attention_backward_workspace_bytes(const mn_packed_args* a) {
   if (!a || a->tq < 1 || a->heads < 1) return 0;

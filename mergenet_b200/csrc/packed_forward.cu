@@ -1,0 +1,600 @@
+// Attention over packed sequences (mn_packed_attention), on the tensor cores.
+//
+//   x = scale Q K^T + bias,  out = softmax(x) V  within each sequence
+//
+// A tile is 128 rows of (token, head of the group), token-major: the heads
+// that share a key head sit in one tile, so grouped heads read their keys and
+// values once and one token's form is a tile of its heads.  Per block of 128
+// keys:
+//
+//   * a load warp brings K and V (a ring of stages) by TMA;
+//   * an MMA warp issues S = Q K^T into tensor memory and, once the softmax
+//     warps have written the probabilities there as 16-bit values, O += P V
+//     with P read from tensor memory;
+//   * four softmax warps a tile, one row a thread, keep the row's running
+//     maximum and sum.  O is rescaled in place only when a row's maximum has
+//     grown by more than 2^8 since its last scale, so rarely.
+//
+// Up to 64 channels one CTA works on one tile and two CTAs share an SM: P has
+// its own columns, so S(j + 1) is computed while the softmax works on S(j).
+// Up to 128 channels one CTA works on two tiles that share K and V (a single
+// tile would ask the L2 for 64 bytes a cycle and SM); P overlays S, and the
+// tensor core alternates between the tiles.
+//
+// With few rows and many keys (SPLIT) the keys are divided over grid.y, and
+// within a CTA of two tile slots the blocks alternate between the slots; the
+// parts are joined by a second kernel in a fixed order.
+#include <algorithm>
+
+#include "packed_tc.cuh"
+
+namespace mn {
+namespace pk {
+
+constexpr float kRescaleLog2 = 8.0f;  // growth of a row's maximum before O is rescaled
+
+template <int DT, bool BIAS>
+struct Fwd {
+  static constexpr int NQ = DT == 64 ? 1 : 2;         // tile slots of a CTA
+  static constexpr int kHalves = DT / 64;
+  static constexpr int kStages = DT == 64 ? 4 : (BIAS ? 4 : 5);
+  // Four softmax warps a slot, then the MMA and the load warp.  A softmax thread
+  // holds a row of 128 scores: with two slots it takes registers from a third
+  // group of four warps, whose other two are idle; the shares stay within what
+  // the CTA was launched with.
+  static constexpr bool kExchange = NQ == 2;
+  static constexpr int kThreads = NQ == 1 ? 192 : 384;
+  static constexpr int kLaunchRegs = kExchange ? 168 : 0, kMore = 208, kLess = 80;
+  static_assert(NQ * kMore + kLess <= 3 * 168, "register exchange");
+  static constexpr uint32_t kTile = kHalves * kHalfBytes;
+  static constexpr uint32_t kQ = 0, kRing = NQ * kTile, kBars = kRing + kStages * kTile;
+  // barriers: Q landed; ring stages full, empty; per slot S ready, S read, P ready, P V done; drain
+  static constexpr int bQ = 0, bFull = 1, bEmpty = bFull + kStages, bS = bEmpty + kStages, bSFree = bS + NQ,
+                       bP = bSFree + NQ, bPV = bP + NQ, bDrain = bPV + NQ, kNumBars = bDrain + 1;
+  static constexpr uint32_t kMisc = kBars + ((kNumBars * 8 + 15) / 16) * 16;  // TMEM base, sequence index
+  static constexpr uint32_t kLut = kMisc + 16;
+  static constexpr uint32_t bytes(uint32_t lut_floats) { return kLut + lut_floats * 4 + 1024; }
+  // TMEM columns
+  static constexpr uint32_t kCols = DT == 64 ? 256 : 512;
+  static constexpr uint32_t cS = 0, cP = DT == 64 ? 128 : 0, cO = DT == 64 ? 192 : 256;
+};
+
+struct FwdParams {
+  mn_packed_args a;
+  int group, ntok;          // heads to a key head, tokens to a tile
+  int span, reach;          // bias: distances held, offset of distance 0
+  int two_sided;
+  int splits;               // grid.y
+  float* part_o;            // [part][kv_heads][tq * group][head_dim]
+  float* part_lse;          // [part][kv_heads][tq * group]
+  int* err;
+};
+
+#ifndef MN_PK_POLY_PAIRS
+#define MN_PK_POLY_PAIRS 4  // of every 16 probability pairs, this many take the FMA-pipe exp2
+#endif
+
+template <typename ET, int DT, bool BIAS, bool SPLIT>
+__global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
+    forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdParams p,
+                   const __grid_constant__ Borders bo) {
+  using F = Fwd<DT, BIAS>;
+  constexpr int NQ = F::NQ, ST = F::kStages, HV = F::kHalves;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + F::kBars);
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(base + F::kMisc);
+  float* lut = reinterpret_cast<float*>(base + F::kLut);
+  const mn_packed_args& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hk = blockIdx.x % a.kv_heads, slot_id = blockIdx.x / a.kv_heads;
+  const int tile_tokens = SPLIT ? p.ntok : NQ * p.ntok;  // SPLIT: both slots work on one tile
+  const int G = p.group;
+
+  if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), F::kCols);
+  if (warp == 1) {
+    const int b = seq_of_slot(a.cu_q, a.nseq, tile_tokens, a.tq, slot_id);
+    if (lane == 0) misc[1] = (uint32_t)b;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && p.err &&
+        bad_lengths(a.cu_q, a.cu_k, a.len_k, a.nseq, a.tq, a.tk, lane, 32))
+      atomicOr(p.err, MN_STATUS_BAD_LENGTHS);
+  }
+  if (warp == 2 && lane == 0) {
+    for (int i = 0; i < F::kNumBars; ++i)
+      tc::mbar_init(bars + i, (i >= F::bSFree && i < F::bPV) ? 4 : 1);
+    tc::fence_mbar_init();
+  }
+  if (warp == 3 && lane == 0) {
+    tma::prefetch_map(&tm_q);
+    tma::prefetch_map(&tm_k);
+    tma::prefetch_map(&tm_v);
+  }
+  if (BIAS)
+    for (int i = tid; i < G * p.span; i += F::kThreads) {
+      const int g = i / p.span, r = i % p.span - p.reach;
+      lut[i] = load_any(a.bias_table, a.bias_dtype, (int64_t)bucket_of(bo, r) * a.heads + hk * G + g) * kLog2e;
+    }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = misc[0];
+  const int b = (int)misc[1];
+  const Seq s = load_seq_or_tail(a, b);
+  const int tiles = (s.nq + tile_tokens - 1) / tile_tokens;
+  const int local = slot_id - slot_of_seq(a.cu_q, b, tile_tokens, a.tq);
+  const bool present = local >= 0 && local < tiles;
+  // the last tiles see the most keys under a causal mask: they go first
+  const int t0 = present ? (a.causal ? tiles - 1 - local : local) * tile_tokens : 0;
+  const int shift = s.nk - s.nq;  // position of query 0
+
+  // key blocks of slot i: [0, end[i]) in whole, [j0, j1) of this split
+  int end[NQ], tok[NQ];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    tok[i] = SPLIT ? t0 : t0 + i * p.ntok;
+    const int last = min(s.nq, tok[i] + p.ntok) - 1;  // last token of the tile
+    const int keys = a.causal ? min(s.nk, last + shift + 1) : s.nk;
+    end[i] = present && last >= tok[i] && keys > 0 ? (keys + 127) >> 7 : 0;
+  }
+  const int nblk = max(end[0], end[NQ - 1]);
+  const int j0 = SPLIT ? (int)((int64_t)nblk * blockIdx.y / p.splits) : 0;
+  const int j1 = SPLIT ? (int)((int64_t)nblk * (blockIdx.y + 1) / p.splits) : nblk;
+  // slot i takes block j?  its first block, and the one after j
+  auto takes = [&](int i, int j) { return SPLIT ? (NQ == 1 || ((j - j0) & 1) == i) : j < end[i]; };
+  auto first_of = [&](int i) { return SPLIT ? j0 + (NQ == 1 ? 0 : i) : j0; };
+  constexpr int kStep = SPLIT ? NQ : 1;
+  auto end_of = [&](int i) { return SPLIT ? j1 : end[i]; };
+  auto last_user = [&](int j) {  // the highest slot that takes block j
+    return SPLIT ? (NQ == 1 ? 0 : (j - j0) & 1) : (NQ > 1 && j < end[NQ - 1] ? NQ - 1 : 0);
+  };
+  constexpr int ab_bf16 = std::is_same<ET, __nv_bfloat16>::value ? 1 : 0;
+  bool ok = true;
+
+  if (warp >= 4 * NQ) {
+    if (F::kExchange) regs_give<F::kLess>();
+    if (warp == 4 * NQ + 1) {
+      // ---------------------------------------------------------------- loads
+      if (lane == 0 && j1 > j0) {
+        int nq_tiles = 0;
+        for (int i = 0; i < (SPLIT ? 1 : NQ); ++i) nq_tiles += end[i] > 0 || i == 0;
+        tma::expect_tx(bars + F::bQ, (uint32_t)nq_tiles * HV * 128u * (uint32_t)(G * p.ntok));
+        for (int i = 0; i < nq_tiles; ++i)
+          for (int h = 0; h < HV; ++h)
+            tma::load_4d(tc::smem_u32(base + F::kQ + i * F::kTile + h * kHalfBytes), &tm_q, h * 64, 0, hk, s.q0 + tok[i],
+                         bars + F::bQ);
+        int n = 0;
+        for (int j = j0; j < j1 && ok; ++j) {
+          for (int kv = 0; kv < 2; ++kv, ++n) {
+            const int st = n % ST;
+            if (n >= ST && !(ok = tc::mbar_wait(bars + F::bEmpty + st, ((n / ST) - 1) & 1, p.err))) break;
+            tma::expect_tx(bars + F::bFull + st, F::kTile);
+            for (int h = 0; h < HV; ++h)
+              load_3d(tc::smem_u32(base + F::kRing + st * F::kTile + h * kHalfBytes), kv ? &tm_v : &tm_k, h * 64, hk,
+                      s.k0 + j * 128, bars + F::bFull + st);
+          }
+        }
+        if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+        // every copy issued has landed before the CTA may release its shared memory
+        tc::mbar_wait(bars + F::bQ, 0, nullptr);
+        for (int m = max(0, n - ST); m < n; ++m) tc::mbar_wait(bars + F::bFull + m % ST, (m / ST) & 1, nullptr);
+      }
+      __syncwarp();
+    } else if (warp == 4 * NQ) {
+      // ----------------------------------------------------------------- MMAs
+      constexpr uint32_t idesc_o = tc::idesc_f16(ab_bf16, 1, 128, DT);
+      int done[NQ];  // blocks of the slot whose S has been issued
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) done[i] = 0;
+      auto cols_of = [&](int j) { return min(128, (s.nk - j * 128 + 31) & ~31); };  // keys of block j, in 32s
+      auto full = [&](int n) { return tc::mbar_wait(bars + F::bFull + n % ST, (n / ST) & 1, p.err); };
+      auto issue_s = [&](int i, int j) -> bool {
+        const int n = 2 * (j - j0);
+        if (!full(n)) return false;
+        if (lane == 0) {
+          tc::fence_after_sync();
+          const uint64_t dq = tc::sw128_desc(tc::smem_u32(base + F::kQ + (SPLIT ? 0 : i) * F::kTile), 16);
+          const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + F::kRing + (n % ST) * F::kTile), 16);
+          const uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, cols_of(j));
+#pragma unroll
+          for (int kk = 0; kk < DT / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3);
+            tc::mma_f16_ss(tmem + F::cS + i * 128, dq + off, dk + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          tc::mma_commit(bars + F::bS + i);
+          if (i == last_user(j)) tc::mma_commit(bars + F::bEmpty + n % ST);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_pv = [&](int i, int j, int c) -> bool {  // c: the slot's block count before this one
+        const int n = 2 * (j - j0) + 1;
+        if (!tc::mbar_wait(bars + F::bP + i, c & 1, p.err) || !full(n)) return false;
+        const int cols = cols_of(j);
+        uint8_t* v = base + F::kRing + (n % ST) * F::kTile;
+        if (s.nk - j * 128 < cols && (SPLIT || i == 0 || j >= end[0])) zero_rows(v, s.nk - j * 128, cols, HV);
+        if (lane == 0) {
+          tc::fence_after_sync();
+          const uint64_t dv = tc::sw128_desc(tc::smem_u32(v), kHalfBytes);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            if (kk * 16 < cols)
+              tc::mma_f16_ts(tmem + F::cO + i * DT, tmem + F::cP + i * 128 + kk * 8, dv + 128 * kk, idesc_o,
+                             (c > 0 || kk > 0) ? 1u : 0u);
+          if (i == last_user(j)) tc::mma_commit(bars + F::bEmpty + n % ST);
+        }
+        __syncwarp();
+        return true;
+      };
+      if (j1 > j0) {
+        ok = tc::mbar_wait(bars + F::bQ, 0, p.err);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          if (ok && first_of(i) < end_of(i)) ok = issue_s(i, first_of(i));
+        for (int j = j0; j < j1 && ok; ++j) {
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            if (!ok || !takes(i, j)) continue;
+            const int c = done[i]++;
+            const bool more = j + kStep < end_of(i);
+            if (DT == 64) {
+              // P has its own columns: S(j + 1) as soon as S(j) has been read
+              if (more) ok = tc::mbar_wait(bars + F::bSFree + i, c & 1, p.err) && issue_s(i, j + kStep);
+              if (ok) ok = issue_pv(i, j, c);
+              if (ok && lane == 0) tc::mma_commit(bars + F::bPV + i);
+            } else {
+              // P overlays S: the MMAs of a CTA run in the order of issue, so
+              // S(j + 1) overwrites P(j) only after P V(j) has read it
+              ok = issue_pv(i, j, c);
+              if (ok && more) ok = issue_s(i, j + kStep);
+              if (ok && !more && lane == 0) tc::mma_commit(bars + F::bPV + i);
+            }
+          }
+        }
+        if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+        if (lane == 0) {  // every MMA issued has completed before the CTA may release its memory
+          tc::mma_commit(bars + F::bDrain);
+          tc::mbar_wait(bars + F::bDrain, 0, nullptr);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------- softmax
+    if (F::kExchange) regs_take<F::kMore>();
+    const int i = warp >> 2, wq = warp & 3;
+    const int r = wq * 32 + lane;
+    const uint32_t lane_sel = (uint32_t)(wq * 32) << 16;
+    const uint32_t t_s = tmem + F::cS + i * 128 + lane_sel, t_p = tmem + F::cP + i * 128 + lane_sel,
+                   t_o = tmem + F::cO + i * DT + lane_sel;
+    const float sl2 = a.scale * kLog2e;  // scores enter the softmax in log2 units
+    const int my = tok[i] + r / G, g = r % G;
+    const bool mine = present && r < G * p.ntok && my < s.nq;  // a row of the sequence
+    const int pos = my + shift;
+    const int klim = a.causal && mine ? min(s.nk, pos + 1) : s.nk;  // keys this row sees
+    const bool live = __any_sync(MN_FULL_MASK, mine);
+    // rows ascend in position: the warp's first row sees the fewest keys, the last of its own the most
+    const int kmin = __reduce_min_sync(MN_FULL_MASK, klim), kmax = __reduce_max_sync(MN_FULL_MASK, mine ? klim : 0);
+    const int pmin = __reduce_min_sync(MN_FULL_MASK, mine ? pos : 0x7fffffff);
+    const int pmax = __reduce_max_sync(MN_FULL_MASK, mine ? pos : -0x7fffffff);
+    const float* row_lut = lut + (BIAS ? (mine ? g : 0) * p.span : 0);
+    float m_run = -INFINITY, l_run = 0.f;
+    int c = 0;
+    for (int j = first_of(i); j < end_of(i) && ok; j += kStep, ++c) {
+      ok = tc::mbar_wait(bars + F::bS + i, c & 1, p.err);
+      if (!ok) break;
+      tc::fence_after_sync();
+      const int k0 = j * 128;
+      const int nch = (min(128, s.nk - k0) + 31) >> 5;          // chunks of 32 columns that S and P hold
+      const int wch = min(nch, max(0, (kmax - k0 + 31) >> 5));  // of those, seen by some row of the warp
+      float x[128];
+      if (live) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (u < wch) tc::tmem_ld32_nowait(t_s + u * 32, x + u * 32);
+        tc::tmem_ld_wait<128>(x);
+      }
+      if (DT == 64) {
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tma::arrive(bars + F::bSFree + i);
+      }
+      // P V(j - 1) has read P(j - 1); a warp without rows waits too, or its
+      // arrival for P(j) could complete the phase of P(j - 1)
+      if (DT == 64 && c > 0 && !(ok = tc::mbar_wait(bars + F::bPV + i, (c - 1) & 1, p.err))) break;
+      float corr = 1.f;
+      if (live) {
+        const bool masked = kmin < k0 + nch * 32;
+        float add = 0.f;  // bias of a block whose distances all lie beyond the table's reach
+        float f = sl2;
+        if (BIAS) {
+          const int lo = k0 - pmax, hi = k0 + 127 - pmin;  // distances of the warp's rows
+          if (hi <= -p.reach) {
+            add = row_lut[0];
+          } else if (lo >= p.span - 1 - p.reach) {
+            add = row_lut[p.span - 1];
+          } else {
+            const int at = k0 - pos + p.reach;
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              if (e / 32 < wch) x[e] = fmaf(x[e], sl2, row_lut[min(max(at + e, 0), p.span - 1)]);
+            f = 1.f;
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (k0 + e >= klim) x[e] = -INFINITY;
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (u >= wch) break;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], x[u * 32 + e]);
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * f + add;
+        const float m_new = fmaxf(m_run, mx);
+        const float m_use = (m_run == -INFINITY || m_new - m_run > kRescaleLog2) ? m_new : m_run;
+        corr = (m_run == -INFINITY || m_use == m_run) ? 1.f : ex2(m_run - m_use);
+        const float nm1 = add - (m_use == -INFINITY ? 0.f : m_use);
+        const float2 nm = make_float2(nm1, nm1), f2 = make_float2(f, f);
+        m_run = m_use;
+        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if (masked) {  // hidden keys get exactly 0
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (u >= nch) break;
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float2 q = make_float2(0.f, 0.f);
+              if (u < wch) {
+                const float2 y = ffma2(make_float2(x[u * 32 + 2 * e], x[u * 32 + 2 * e + 1]), f2, nm);
+                q = make_float2(ex2(y.x), ex2(y.y));
+                sum2[e & 1] = fadd2(sum2[e & 1], q);
+              }
+              pk[e] = pack2<ET>(q.x, q.y);
+            }
+            tc::tmem_st16_nowait(t_p + u * 16, pk);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (u >= nch) break;
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 y = ffma2(make_float2(x[u * 32 + 2 * e], x[u * 32 + 2 * e + 1]), f2, nm);
+              // pairs spread evenly over the row take the polynomial
+              const float2 q = (MN_PK_POLY_PAIRS > 0 && (e * MN_PK_POLY_PAIRS) % 16 >= 16 - MN_PK_POLY_PAIRS)
+                                   ? ex2_poly2(y)
+                                   : make_float2(ex2(y.x), ex2(y.y));
+              sum2[e & 1] = fadd2(sum2[e & 1], q);
+              pk[e] = pack2<ET>(q.x, q.y);
+            }
+            tc::tmem_st16_nowait(t_p + u * 16, pk);
+          }
+        }
+        tc::tmem_wait_st();
+        const float2 ss = fadd2(sum2[0], sum2[1]);
+        l_run = l_run * corr + (ss.x + ss.y);
+        // O is at rest: with P apart P V(j - 1) was waited for above, and with
+        // P over S the commit behind S(j) covers P V(j - 1) as well
+        if (c > 0 && __any_sync(MN_FULL_MASK, corr != 1.f)) {
+          float o[32];
+#pragma unroll
+          for (int u = 0; u < DT / 32; ++u) {
+            tc::tmem_ld32(t_o + u * 32, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= corr;
+            tc::tmem_st32(t_o + u * 32, o);
+          }
+        }
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tma::arrive(bars + F::bP + i);
+    }
+    if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+    if (ok && c > 0) {
+      ok = tc::mbar_wait(bars + F::bPV + i, DT == 64 ? (c - 1) & 1 : 0, p.err);
+      tc::fence_after_sync();
+    }
+    if (ok && live) {
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // NaN stays
+      const int64_t row = (int64_t)(s.q0 + my) * G + g;     // packed row of the key head
+      const int part = SPLIT ? blockIdx.y * NQ + i : 0;
+      const int64_t rows = (int64_t)a.tq * G;
+#pragma unroll
+      for (int u = 0; u < DT / 32; ++u) {
+        float o[32];
+        if (c > 0) {
+          tc::tmem_ld32(t_o + u * 32, o);  // the whole warp takes part
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (mine && SPLIT && c > 0) {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + ((part * a.kv_heads + hk) * rows + row) * a.head_dim + u * 32);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (u * 32 + 4 * e < a.head_dim)
+              dst[e] = make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
+        }
+        if (mine && !SPLIT)
+          store32<ET>(static_cast<ET*>(a.out) + ((int64_t)(s.q0 + my) * a.heads + hk * G + g) * a.head_dim, u * 32, a.head_dim,
+                      o, inv);
+        __syncwarp();
+      }
+      if (mine) {
+        if (SPLIT)
+          p.part_lse[(part * a.kv_heads + hk) * rows + row] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run);
+        else if (a.lse)
+          a.lse[hk * rows + row] = l_run == 0.f ? INFINITY : m_run + log2f(l_run);
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, F::kCols);
+  }
+}
+
+// out = sum over the parts of 2^(lse_i - max) out_i over the sum of those
+// weights, the parts in order; one warp a row.
+template <typename ET>
+__global__ void __launch_bounds__(128) join_kernel(mn_packed_args a, int parts, const float* __restrict__ part_o,
+                                                   const float* __restrict__ part_lse) {
+  const int lane = threadIdx.x & 31, G = a.heads / a.kv_heads;
+  const int64_t rows = (int64_t)a.tq * G, all = rows * a.kv_heads;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (w >= all) return;
+  float m = -INFINITY;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, part_lse[i * all + w]);
+  m = warp_max(m);
+  const int c = lane * 4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const float lse = part_lse[i * all + w];
+    if (lse == -INFINITY) continue;  // a part without keys wrote no output
+    const float f = m == -INFINITY ? 1.f : ex2(lse - m);  // NaN stays
+    total += f;
+    if (c < a.head_dim) {
+      const float4 o = *reinterpret_cast<const float4*>(part_o + (i * all + w) * a.head_dim + c);
+      acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
+    }
+  }
+  const int hk = (int)(w / rows);
+  const int64_t row = w % rows, t = row / G, g = row % G;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  if (c < a.head_dim)
+    *reinterpret_cast<uint2*>(static_cast<ET*>(a.out) + (t * a.heads + hk * G + g) * a.head_dim + c) =
+        make_uint2(pack2<ET>(acc.x * inv, acc.y * inv), pack2<ET>(acc.z * inv, acc.w * inv));
+  if (a.lse && lane == 0) a.lse[w] = total == 0.f ? INFINITY : m + log2f(total);
+}
+
+int check(const mn_packed_args* a, Borders* bo, bool backward) {
+  if (!a || a->nseq < 1 || a->tq < 0 || a->tk < 0 || a->heads < 1 || a->kv_heads < 1) return MN_ERR_ARG;
+  if (a->heads % a->kv_heads || a->head_dim < 1 || !(a->scale > 0.f) || !(a->scale < INFINITY)) return MN_ERR_ARG;
+  if (!a->cu_q || !a->cu_k || (a->tq > 0 && (!a->q || !a->out)) || (a->tk > 0 && (!a->k || !a->v))) return MN_ERR_ARG;
+  if (backward && a->tq > 0 && (!a->dout || !a->lse || !a->dq)) return MN_ERR_ARG;
+  if (backward && a->tk > 0 && (!a->dk || !a->dv)) return MN_ERR_ARG;
+  if (a->dtype != MN_F16 && a->dtype != MN_BF16) return MN_ERR_UNSUPPORTED;
+  const int g = a->heads / a->kv_heads;
+  if (a->head_dim > 128 || a->head_dim % 8 || g > 128) return MN_ERR_UNSUPPORTED;
+  if ((int64_t)a->tq * g >= (1 << 30) || (int64_t)a->tk * g >= (1 << 30)) return MN_ERR_UNSUPPORTED;
+  if (!rows_ok(a->q, a->q_st, a->q_sh, a->tq, a->heads) || !rows_ok(a->k, a->k_st, a->k_sh, a->tk, a->kv_heads) ||
+      !rows_ok(a->v, a->v_st, a->v_sh, a->tk, a->kv_heads) ||
+      (backward && !rows_ok(a->dout, a->do_st, a->do_sh, a->tq, a->heads)))
+    return MN_ERR_UNSUPPORTED;
+  bo->n = 0;
+  if (a->bias_table) {
+    if (a->bias_dtype < 0 || a->bias_dtype > 2 || (backward && !a->dbias)) return MN_ERR_ARG;
+    if (!make_borders(bo, a->buckets, a->two_sided, a->num_borders, a->borders)) return MN_ERR_ARG;
+    const int last = bo->n ? bo->at[bo->n - 1] : 1;
+    if (a->buckets > 64 || ((a->two_sided ? 2 : 1) * (int64_t)last + 1) * g > 8192) return MN_ERR_UNSUPPORTED;
+  }
+  return MN_OK;
+}
+
+// How the call is divided: 0 parts means whole rows.
+struct Plan {
+  int ntok, parts, splits;
+};
+static Plan plan_of(const mn_packed_args* a) {
+  const int g = a->heads / a->kv_heads, slots = a->head_dim <= 64 ? 1 : 2;
+  Plan pl{128 / g, 0, 1};
+  // Tiles that have rows, at most; a call that leaves the card part empty and
+  // whose sequences are long on average is divided over the keys.
+  const int64_t tiles = ((int64_t)a->tq / pl.ntok + a->nseq) * a->kv_heads;
+  const int64_t ctas = (int64_t)sm_count() * (slots == 1 ? 2 : 1);
+  const int64_t blocks = a->tk / a->nseq / 128;
+  if (blocks >= 4 && (tiles <= ctas || (int64_t)a->tq * g <= (int64_t)a->nseq * 64)) {
+    const int64_t want = std::max<int64_t>(1, (2 * ctas + tiles - 1) / tiles);
+    pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, blocks / (2 * slots)), 64));
+    if (pl.splits * slots > 1) pl.parts = pl.splits * slots;
+  }
+  return pl;
+}
+static size_t part_bytes(const mn_packed_args* a, const Plan& pl) {
+  return (size_t)pl.parts * a->tq * a->heads * (a->head_dim + 1) * 4;
+}
+
+template <typename ET, int DT, bool BIAS, bool SPLIT>
+static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, void* ws, int* err, cudaStream_t st) {
+  using F = Fwd<DT, BIAS>;
+  constexpr bool bf16 = std::is_same<ET, __nv_bfloat16>::value;
+  CUtensorMap mq, mk, mv;
+  if (!map_q(&mq, bf16, a->q, a->q_st, a->q_sh, a->tq, a->heads, a->kv_heads, a->head_dim, pl.ntok)) return false;
+  if (!map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim)) return false;
+  if (!map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim)) return false;
+  FwdParams p;
+  p.a = *a;
+  p.group = a->heads / a->kv_heads;
+  p.ntok = pl.ntok;
+  p.splits = pl.splits;
+  p.span = p.reach = p.two_sided = 0;
+  if (BIAS) {
+    const int last = bo.n ? bo.at[bo.n - 1] : 1;
+    p.two_sided = bo.two_sided;
+    p.reach = last;
+    p.span = (bo.two_sided ? 2 : 1) * last + 1;
+  }
+  p.part_o = static_cast<float*>(ws);
+  p.part_lse = p.part_o + (size_t)pl.parts * a->tq * a->heads * a->head_dim;
+  p.err = err;
+  const size_t smem = F::bytes(p.span * p.group);
+  auto kern = forward_kernel<ET, DT, BIAS, SPLIT>;
+  if (!ensure_smem(kern, smem) || !launch_regs(kern, F::kLaunchRegs)) return false;
+  const int64_t slots = tile_slots(a->tq, a->nseq, SPLIT ? pl.ntok : F::NQ * pl.ntok) * a->kv_heads;
+  if (slots > 0x7fffffff) return false;
+  kern<<<dim3((unsigned)slots, pl.splits), F::kThreads, smem, st>>>(mq, mk, mv, p, bo);
+  if (SPLIT) {
+    const int64_t rows = (int64_t)a->tq * a->heads;
+    join_kernel<ET><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(*a, pl.parts, p.part_o, p.part_lse);
+  }
+  return true;
+}
+
+template <typename ET, int DT>
+static bool launch_d(const mn_packed_args* a, const Borders& bo, const Plan& pl, void* ws, int* err, cudaStream_t st) {
+  if (a->bias_table)
+    return pl.parts ? launch<ET, DT, true, true>(a, bo, pl, ws, err, st) : launch<ET, DT, true, false>(a, bo, pl, ws, err, st);
+  return pl.parts ? launch<ET, DT, false, true>(a, bo, pl, ws, err, st) : launch<ET, DT, false, false>(a, bo, pl, ws, err, st);
+}
+
+}  // namespace pk
+}  // namespace mn
+
+using namespace mn;
+
+extern "C" size_t mn_packed_attention_workspace_bytes(const mn_packed_args* a) {
+  Borders bo;
+  if (pk::check(a, &bo, false) != MN_OK || a->tq == 0) return 0;
+  const pk::Plan pl = pk::plan_of(a);
+  return pl.parts ? pk::part_bytes(a, pl) : 0;
+}
+
+extern "C" int mn_packed_attention(const mn_packed_args* a, void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  Borders bo;
+  const int rc = pk::check(a, &bo, false);
+  if (rc != MN_OK) return rc;
+  if (a->tq == 0) return MN_OK;
+  const pk::Plan pl = pk::plan_of(a);
+  if (pl.parts && (!workspace || workspace_bytes < pk::part_bytes(a, pl))) return MN_ERR_WORKSPACE;
+  cudaGetLastError();
+  auto st = static_cast<cudaStream_t>(stream);
+  bool done;
+  if (a->dtype == MN_F16)
+    done = a->head_dim <= 64 ? pk::launch_d<__half, 64>(a, bo, pl, workspace, status, st)
+                             : pk::launch_d<__half, 128>(a, bo, pl, workspace, status, st);
+  else
+    done = a->head_dim <= 64 ? pk::launch_d<__nv_bfloat16, 64>(a, bo, pl, workspace, status, st)
+                             : pk::launch_d<__nv_bfloat16, 128>(a, bo, pl, workspace, status, st);
+  if (!done) return MN_ERR_UNSUPPORTED;
+  return cudaGetLastError() == cudaSuccess ? MN_OK : MN_ERR_LAUNCH;
+}

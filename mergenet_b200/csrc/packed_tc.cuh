@@ -1,0 +1,192 @@
+// Tensor-core plumbing shared by the packed attention's forward and backward:
+// tensor maps of packed rows, tile lookup, the two exponentials.
+#pragma once
+
+#include <type_traits>
+
+#include "packed.cuh"
+#include "tc_common.cuh"
+#include "tma.cuh"
+
+namespace mn {
+namespace pk {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kHalfBytes = 128 * 128;  // 128 rows of 64 16-bit channels
+
+template <typename ET>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// 2^y for a pair of y <= 8 on the FMA pipe (the polynomial of
+// csrc/exp2_fit.py, relative error 2.7e-6): y = n + f with n the nearest
+// integer, taken from the low bits of y + 1.5 * 2^23.  y is clamped at -126,
+// NaN kept, so it serves unmasked scores only: 2^-126 in the place of less.
+__device__ __forceinline__ float2 ex2_poly2(float2 y) {
+  y.x = max_nan(y.x, -126.f);
+  y.y = max_nan(y.y, -126.f);
+  const float2 magic = make_float2(12582912.f, 12582912.f);
+  const float2 t = fadd2(y, magic);
+  const float2 f = fadd2(y, fadd2(magic, make_float2(-t.x, -t.y)));
+  float2 p = ffma2(f, make_float2(9.570100344717503e-03f, 9.570100344717503e-03f),
+                   make_float2(5.591786280274391e-02f, 5.591786280274391e-02f));
+  p = ffma2(p, f, make_float2(2.402474433183670e-01f, 2.402474433183670e-01f));
+  p = ffma2(p, f, make_float2(6.931217908859253e-01f, 6.931217908859253e-01f));
+  p = ffma2(p, f, make_float2(9.999992847442627e-01f, 9.999992847442627e-01f));
+  const int nx = __float_as_int(t.x) - 0x4B400000, ny = __float_as_int(t.y) - 0x4B400000;
+  return make_float2(__int_as_float(__float_as_int(p.x) + (nx << 23)), __int_as_float(__float_as_int(p.y) + (ny << 23)));
+}
+
+// Register exchange between the warp groups of a CTA (a whole group executes
+// it).  A taker waits until the givers' registers are free, so the shares may
+// not exceed what the CTA was launched with: launch_regs() on the host checks
+// the launch, a static_assert at each kernel the shares.
+template <int N>
+__device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Tiles of `m` rows of every sequence share one index space without a prefix
+// sum: sequence b's tiles begin at slot cu[b] / m + b.  A sequence of L rows
+// has ceil(L / m) tiles and at least that many slots, at most one of them
+// left empty.  Rows behind the last sequence are sequence n, with no keys.
+__device__ __forceinline__ int slot_of_seq(const int32_t* cu, int b, int m, int rows) {
+  return min(max(cu[b], 0), rows) / m + b;
+}
+inline int64_t tile_slots(int rows, int n, int m) { return (int64_t)rows / m + n + 1; }
+
+// The last sequence (0..n) whose first slot is at or below `slot`; a whole
+// warp searches, 32 probes a step.
+__device__ __forceinline__ int seq_of_slot(const int32_t* cu, int n, int m, int rows, int slot) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n + 1;  // first slot of lo <= slot; of hi > slot
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int b = lo + (lane + 1) * step;
+    const bool le = b < hi && slot_of_seq(cu, b, m, rows) <= slot;
+    const unsigned vote = __ballot_sync(MN_FULL_MASK, le);
+    const int k = vote == 0 ? 0 : 32 - __clz(vote);  // probes at or below (offsets ascend)
+    const int nlo = lo + k * step;
+    hi = min(hi, nlo + step);
+    lo = nlo;
+  }
+  return lo;
+}
+
+// Sequence n: the rows behind the last one, which see nothing.
+__device__ __forceinline__ Seq load_seq_or_tail(const mn_packed_args& a, int b) {
+  if (b < a.nseq) return load_seq(a.cu_q, a.cu_k, a.len_k, b, a.tq, a.tk);
+  Seq s;
+  s.q0 = min(max(a.cu_q[a.nseq], 0), a.tq);
+  s.nq = a.tq - s.q0;
+  s.k0 = min(max(a.cu_k[a.nseq], 0), a.tk);
+  s.slot = a.tk - s.k0;
+  s.nk = 0;
+  return s;
+}
+
+// 32 fp32 values of one row as ET, 16 bytes at a time, up to channel `d`
+template <typename ET>
+__device__ __forceinline__ void store32(ET* row, int c0, int d, const float* o, float f) {
+  uint4* dst = reinterpret_cast<uint4*>(row + c0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c0 + 8 * i < d)
+      dst[i] = make_uint4(pack2<ET>(o[8 * i] * f, o[8 * i + 1] * f), pack2<ET>(o[8 * i + 2] * f, o[8 * i + 3] * f),
+                          pack2<ET>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack2<ET>(o[8 * i + 6] * f, o[8 * i + 7] * f));
+}
+
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+
+// Zero rows [from, to) of a tile of 128-byte rows in `halves` halves (a whole
+// warp), for operand rows that a product must not read: 0 times NaN is NaN.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to, int halves) {
+  const int lane = threadIdx.x & 31, n = (to - from) * 8;
+  for (int h = 0; h < halves; ++h)
+    for (int i = lane; i < n; i += 32)
+      *reinterpret_cast<uint4*>(tile + h * kHalfBytes + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+  tc::fence_async_smem();
+  __syncwarp();
+}
+
+// ------------------------------------------------------------------- host
+// Query-side rows [rows, heads, d] as (d, g, key head, row) with boxes of 64
+// channels x g heads x n rows: row n * g + i of the tile is head i of row n.
+inline bool map_q(CUtensorMap* map, bool bf16, const void* p, int64_t st, int64_t sh, int rows, int heads, int kv_heads,
+                  int d, int n) {
+  const int g = heads / kv_heads;
+  if (heads == 1) sh = (d + 7) / 8 * 8;  // a dimension of one row has any stride
+  if (rows == 1) st = sh * heads;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)g, (cuuint64_t)kv_heads, (cuuint64_t)rows};
+  const cuuint64_t strides[3] = {(cuuint64_t)sh * 2, (cuuint64_t)sh * 2 * g, (cuuint64_t)st * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)g, 1, (cuuint32_t)n};
+  return tma::encode(map, bf16, 4, p, dims, strides, box, true, true);
+}
+// Key-side rows [rows, kv_heads, d] with boxes of 64 channels x 128 rows
+inline bool map_k(CUtensorMap* map, bool bf16, const void* p, int64_t st, int64_t sh, int rows, int kv_heads, int d) {
+  if (kv_heads == 1) sh = (d + 7) / 8 * 8;
+  if (rows == 1) st = sh * kv_heads;
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)kv_heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
+  const cuuint32_t box[3] = {64, 1, 128};
+  return tma::encode(map, bf16, 3, p, dims, strides, box, true, true);
+}
+// what a tensor map needs of a [rows, heads, d] tensor
+inline bool rows_ok(const void* p, int64_t st, int64_t sh, int rows, int heads) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || (st > 0 && st % 8 == 0)) &&
+         (heads <= 1 || (sh > 0 && sh % 8 == 0)) && st < (int64_t(1) << 38) && sh < (int64_t(1) << 31);
+}
+// The kernel was compiled to launch with at least `regs` registers a thread.
+template <typename F>
+inline bool launch_regs(F* func, int regs) {
+  static std::mutex mu;
+  static std::map<const void*, int> known;
+  const void* key = reinterpret_cast<const void*>(func);
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = known.find(key);
+  if (it == known.end()) {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, func) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    it = known.emplace(key, at.numRegs).first;
+  }
+  return it->second >= regs;
+}
+inline int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+int check(const mn_packed_args* a, Borders* bo, bool backward);  // packed_forward.cu
+
+}  // namespace pk
+}  // namespace mn
