@@ -1,124 +1,800 @@
-// Gradients of the packed attention (mn_packed_attention_backward): one warp
-// per query row and head (dq) or per key row and key head (dk, dv), the
-// channels over the lanes.
+// Gradients of the packed attention (mn_packed_attention_backward), on the
+// tensor cores:
+//
+//   p = 2^(x log2e - lse),  delta = dout . out,  ds = p (dout V^T - delta)
+//   dq = scale ds K,  dk = scale ds^T Q,  dv = p^T dout
+//   dtable[u, h] = sum of ds over the pairs of bucket u
+//
+// Two kernels, each recomputing p and ds: dq walks the keys of a query tile,
+// dk and dv walk the query tiles of a key tile.  Seven products instead of
+// the five of a single kernel, but every sum stays in one CTA's tensor
+// memory: no atomics, a fixed order, no fp32 dq in memory.  Both keep p and
+// ds in tensor memory as the 16-bit left operand of the next product (the
+// key-side kernel works on transposed scores, S^T = K Q^T, so that p^T and
+// ds^T have the keys in the lanes), so they never pass through shared memory.
+//
+// Tiles are those of the forward: 128 rows of (token, head of the group), so
+// the gradients of a shared key head are summed over its query heads by the
+// same products.  Eight warps compute, two threads to a row with 64 columns
+// each; one warp issues the MMAs and one loads.
+#include <algorithm>
+
 #include "packed_tc.cuh"
 
 namespace mn {
 namespace pk {
 
-constexpr int kThreads = 128;
+constexpr int kBwdThreads = 320;  // warps 0-7 compute, 8 MMAs, 9 loads
 
-template <typename T>
-__device__ __forceinline__ void load_row(const T* p, int d, int lane, float (&x)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = lane + 32 * i < d ? to_f32(p[lane + 32 * i]) : 0.f;
-}
-__device__ __forceinline__ float dot4(const float (&a)[4], const float (&b)[4]) {
-  return warp_sum(a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]);
-}
-template <typename T>
-__device__ __forceinline__ void store_row(T* p, int d, int lane, const float (&x)[4], float f) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < d) p[lane + 32 * i] = from_f32<T>(x[i] * f);
-}
+#ifndef MN_PK_BWD_POLY_PAIRS
+#define MN_PK_BWD_POLY_PAIRS 4  // of every 16 probability pairs, this many take the FMA-pipe exp2
+#endif
 
-// dq, each row's delta, and each row's sums of ds by bucket (part)
-template <typename T>
-__global__ void __launch_bounds__(kThreads) dq_kernel(mn_packed_args a, Borders bo, float* delta, float* part) {
-  __shared__ float hist[kThreads / 32][64];
-  const int lane = threadIdx.x & 31, wi = threadIdx.x >> 5;
-  const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + wi;
-  if (w >= (int64_t)a.tq * a.heads) return;
-  const int t = (int)(w / a.heads), h = (int)(w % a.heads), g = a.heads / a.kv_heads, hk = h / g, d = a.head_dim;
-  const int b = seq_of_row(a.cu_q, a.nseq, t);
-  for (int i = lane; i < 64; i += 32) hist[wi][i] = 0.f;
-  __syncwarp();
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, dl = 0.f;
-  if (b < a.nseq) {
-    const Seq s = load_seq(a.cu_q, a.cu_k, a.len_k, b, a.tq, a.tk);
-    const int pos = t - s.q0 + s.nk - s.nq;
-    const int end = a.causal ? min(s.nk, pos + 1) : s.nk;
-    const float lse = a.lse[((int64_t)hk * a.tq + t) * g + h % g];
-    float q[4], k[4], v[4], go[4], o[4];
-    load_row(static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh, d, lane, q);
-    load_row(static_cast<const T*>(a.dout) + t * a.do_st + h * a.do_sh, d, lane, go);
-    load_row(static_cast<const T*>(a.out) + ((int64_t)t * a.heads + h) * d, d, lane, o);
-    dl = dot4(go, o);
-    for (int j = 0; j < end; ++j) {
-      load_row(static_cast<const T*>(a.k) + (int64_t)(s.k0 + j) * a.k_st + hk * a.k_sh, d, lane, k);
-      load_row(static_cast<const T*>(a.v) + (int64_t)(s.k0 + j) * a.v_st + hk * a.v_sh, d, lane, v);
-      float x = dot4(q, k) * a.scale;
-      int u = 0;
-      if (a.bias_table) {
-        u = bucket_of(bo, j - pos);
-        x += load_any(a.bias_table, a.bias_dtype, u * a.heads + h);
-      }
-      const float ds = exp2f(x * kLog2e - lse) * (dot4(go, v) - dl);
-      if (a.bias_table && lane == 0) hist[wi][u] += ds;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] += ds * k[i];
-    }
+struct BwdParams {
+  mn_packed_args a;
+  int group, ntok;
+  int span, reach;   // bias: distances held, offset of distance 0
+  float* delta;      // [kv_heads][tq * group]
+  float* part;       // [kv_heads][slots][buckets * group] sums of ds by bucket
+  int* err;
+};
+
+// Bias tables of a CTA: bucket of each distance, value of each (head, bucket)
+struct BiasSmem {
+  uint8_t* idx;  // [span]
+  float* tab;    // [group][buckets], log2 units
+};
+__device__ __forceinline__ void fill_bias(const BwdParams& p, const Borders& bo, int hk, const BiasSmem& s) {
+  for (int i = threadIdx.x; i < p.span; i += kBwdThreads) s.idx[i] = (uint8_t)bucket_of(bo, i - p.reach);
+  for (int i = threadIdx.x; i < p.group * p.a.buckets; i += kBwdThreads) {
+    const int g = i / p.a.buckets, u = i % p.a.buckets;
+    s.tab[i] = load_any(p.a.bias_table, p.a.bias_dtype, (int64_t)u * p.a.heads + hk * p.group + g) * kLog2e;
   }
-  store_row(static_cast<T*>(a.dq) + ((int64_t)t * a.heads + h) * d, d, lane, acc, a.scale);
-  if (lane == 0) delta[((int64_t)hk * a.tq + t) * g + h % g] = dl;
-  __syncwarp();
-  if (a.bias_table)
-    for (int u = lane; u < a.buckets; u += 32) part[((int64_t)t * a.heads + h) * a.buckets + u] = hist[wi][u];
 }
 
-// dtable[u, h] = sum over t of part[t, h, u]: one block per (u, h)
-__global__ void __launch_bounds__(kThreads) dbias_kernel(const float* part, int tq, int heads, int buckets, float* out) {
-  __shared__ float scratch[32];
-  const int u = blockIdx.x, h = blockIdx.y;
-  float x = 0.f;
-  for (int t = threadIdx.x; t < tq; t += kThreads) x += part[((int64_t)t * heads + h) * buckets + u];
-  x = block_sum(x, scratch);
-  if (threadIdx.x == 0) out[u * heads + h] = x;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) dkv_kernel(mn_packed_args a, Borders bo, const float* delta) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (w >= (int64_t)a.tk * a.kv_heads) return;
-  const int row = (int)(w / a.kv_heads), hk = (int)(w % a.kv_heads), g = a.heads / a.kv_heads, d = a.head_dim;
-  const int b = seq_of_row(a.cu_k, a.nseq, row);
-  float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
-  if (b < a.nseq) {
-    const Seq s = load_seq(a.cu_q, a.cu_k, a.len_k, b, a.tq, a.tk);
-    const int j = row - s.k0;
-    if (j < s.nk) {
-      float q[4], k[4], v[4], go[4];
-      load_row(static_cast<const T*>(a.k) + row * a.k_st + hk * a.k_sh, d, lane, k);
-      load_row(static_cast<const T*>(a.v) + row * a.v_st + hk * a.v_sh, d, lane, v);
-      const int first = a.causal ? max(0, j - (s.nk - s.nq)) : 0;
-      for (int i = first; i < s.nq; ++i) {
-        const int t = s.q0 + i;
-        for (int gg = 0; gg < g; ++gg) {
-          const int h = hk * g + gg;
-          load_row(static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh, d, lane, q);
-          load_row(static_cast<const T*>(a.dout) + t * a.do_st + h * a.do_sh, d, lane, go);
-          float x = dot4(q, k) * a.scale;
-          if (a.bias_table)
-            x += load_any(a.bias_table, a.bias_dtype, bucket_of(bo, j - i - (s.nk - s.nq)) * a.heads + h);
-          const int64_t at = ((int64_t)hk * a.tq + t) * g + gg;
-          const float p = exp2f(x * kLog2e - a.lse[at]);
-          const float ds = p * (dot4(go, v) - delta[at]);
+// p = 2^y for 32 values; MASKED: y of hidden keys is -inf and gives 0
+template <bool MASKED>
+__device__ __forceinline__ void exp32(float* y) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            dk[e] += ds * q[e];
-            dv[e] += p * go[e];
+  for (int e = 0; e < 16; ++e) {
+    const float2 v = make_float2(y[2 * e], y[2 * e + 1]);
+    const float2 q = (!MASKED && MN_PK_BWD_POLY_PAIRS > 0 && (e * MN_PK_BWD_POLY_PAIRS) % 16 >= 16 - MN_PK_BWD_POLY_PAIRS)
+                         ? ex2_poly2(v)
+                         : make_float2(ex2(v.x), ex2(v.y));
+    y[2 * e] = q.x;
+    y[2 * e + 1] = q.y;
+  }
+}
+template <typename ET>
+__device__ __forceinline__ void put32(uint32_t taddr, const float* v) {
+  uint32_t w[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) w[e] = pack2<ET>(v[2 * e], v[2 * e + 1]);
+  tc::tmem_st16_nowait(taddr, w);
+}
+// left operand in tensor memory: columns 0-63 packed at +0, 64-127 at +64, so
+// that each half overwrites only what its own warps have read
+__device__ __forceinline__ uint32_t left_cols(int kk) { return (uint32_t)((kk & 3) * 8 + (kk >> 2) * 64); }
+
+// ----------------------------------------------------------------------- dq
+template <int DT, bool BIAS>
+struct Dq {
+  static constexpr int HV = DT / 64;
+  static constexpr uint32_t kTile = HV * kHalfBytes;
+  static constexpr int KS = DT == 64 || !BIAS ? 3 : 2, VS = DT == 64 || !BIAS ? 2 : 1;
+  static constexpr uint32_t oQ = 0, oDO = kTile, oK = 2 * kTile, oV = oK + KS * kTile, oBars = oV + VS * kTile;
+  static constexpr int bQ = 0, bKF = 1, bKE = bKF + KS, bVF = bKE + KS, bVE = bVF + VS, bS = bVE + VS, bDP = bS + 2, bDS = bDP + 1,
+                       bDone = bDS + 1, bDrain = bDone + 1, kNumBars = bDrain + 1;
+  static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
+  static constexpr uint32_t oDelta = oMisc + 16;             // [2][128] partial deltas
+  static constexpr uint32_t oHist = oDelta + 2 * 128 * 4;    // [2][buckets][128]
+  static constexpr uint32_t bytes(int buckets, int group, int span) {
+    return oHist + (BIAS ? buckets * 1024 + ((buckets * group * 4 + 15) / 16) * 16 + span : 0) + 1024;
+  }
+  static constexpr uint32_t cS = 0, cDP = 256, cDQ = 384;
+};
+
+template <typename ET, int DT, bool BIAS>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+              const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+              const __grid_constant__ BwdParams p, const __grid_constant__ Borders bo) {
+  using C = Dq<DT, BIAS>;
+  constexpr int HV = C::HV, KS = C::KS, VS = C::VS;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(base + C::oMisc);
+  const mn_packed_args& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
+  const int hk = blockIdx.x % a.kv_heads, slot_id = blockIdx.x / a.kv_heads;
+  float* hist = reinterpret_cast<float*>(base + C::oHist);
+  BiasSmem bs;
+  bs.tab = reinterpret_cast<float*>(base + C::oHist + (BIAS ? a.buckets * 1024 : 0));
+  bs.idx = reinterpret_cast<uint8_t*>(bs.tab) + (BIAS ? (a.buckets * G * 4 + 15) / 16 * 16 : 0);
+
+  if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
+  if (warp == 1) {
+    const int b = seq_of_slot(a.cu_q, a.nseq, p.ntok, a.tq, slot_id);
+    if (lane == 0) misc[1] = (uint32_t)b;
+  }
+  if (warp == 2 && lane == 0) {
+    for (int i = 0; i < C::kNumBars; ++i) tc::mbar_init(bars + i, i == C::bDS ? 8 : 1);
+    tc::fence_mbar_init();
+  }
+  if (warp == 3 && lane == 0) {
+    tma::prefetch_map(&tm_q);
+    tma::prefetch_map(&tm_do);
+    tma::prefetch_map(&tm_k);
+    tma::prefetch_map(&tm_v);
+  }
+  if (BIAS) {
+    fill_bias(p, bo, hk, bs);
+    for (int i = tid; i < 2 * a.buckets * 128; i += kBwdThreads) hist[i] = 0.f;
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = misc[0];
+  const int b = (int)misc[1];
+  const Seq s = load_seq_or_tail(a, b);
+  const int tiles = (s.nq + p.ntok - 1) / p.ntok;
+  const int local = slot_id - slot_of_seq(a.cu_q, b, p.ntok, a.tq);
+  const bool present = local >= 0 && local < tiles;
+  const int t0 = present ? (a.causal ? tiles - 1 - local : local) * p.ntok : 0;
+  const int shift = s.nk - s.nq;
+  const int last = min(s.nq, t0 + p.ntok) - 1;
+  const int keys = a.causal ? min(s.nk, last + shift + 1) : s.nk;
+  const int n = present && keys > 0 ? (keys + 127) >> 7 : 0;
+  constexpr int ab_bf16 = std::is_same<ET, __nv_bfloat16>::value ? 1 : 0;
+  bool ok = true;
+
+  if (warp == 9) {
+    // ---------------------------------------------------------------- loads
+    if (lane == 0 && n > 0) {
+      tma::expect_tx(bars + C::bQ, 2u * HV * 128u * (uint32_t)(G * p.ntok));
+      for (int h = 0; h < HV; ++h) {
+        tma::load_4d(tc::smem_u32(base + C::oQ + h * kHalfBytes), &tm_q, h * 64, 0, hk, s.q0 + t0, bars + C::bQ);
+        tma::load_4d(tc::smem_u32(base + C::oDO + h * kHalfBytes), &tm_do, h * 64, 0, hk, s.q0 + t0, bars + C::bQ);
+      }
+      int nk = 0, nv = 0;
+      for (int j = 0; j < n && ok; ++j) {
+        const int ks = j % KS, vs = j % VS;
+        if (j >= KS && !(ok = tc::mbar_wait(bars + C::bKE + ks, (j / KS - 1) & 1, p.err))) break;
+        tma::expect_tx(bars + C::bKF + ks, C::kTile);
+        for (int h = 0; h < HV; ++h)
+          load_3d(tc::smem_u32(base + C::oK + ks * C::kTile + h * kHalfBytes), &tm_k, h * 64, hk, s.k0 + j * 128, bars + C::bKF + ks);
+        nk = j + 1;
+        if (j >= VS && !(ok = tc::mbar_wait(bars + C::bVE + vs, (j / VS - 1) & 1, p.err))) break;
+        tma::expect_tx(bars + C::bVF + vs, C::kTile);
+        for (int h = 0; h < HV; ++h)
+          load_3d(tc::smem_u32(base + C::oV + vs * C::kTile + h * kHalfBytes), &tm_v, h * 64, hk, s.k0 + j * 128, bars + C::bVF + vs);
+        nv = j + 1;
+      }
+      if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+      // every copy issued has landed before the CTA may release its shared memory
+      tc::mbar_wait(bars + C::bQ, 0, nullptr);
+      for (int j = max(0, nk - KS); j < nk; ++j) tc::mbar_wait(bars + C::bKF + j % KS, (j / KS) & 1, nullptr);
+      for (int j = max(0, nv - VS); j < nv; ++j) tc::mbar_wait(bars + C::bVF + j % VS, (j / VS) & 1, nullptr);
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ----------------------------------------------------------------- MMAs
+    // S runs one block ahead of dP: at ds(j), dP(j + 1), dQ += ds(j) K(j) and
+    // S(j + 2) are issued while the compute warps turn S(j + 1) into p
+    constexpr uint32_t idesc_q = tc::idesc_f16(ab_bf16, 1, 128, DT);
+    auto cols_of = [&](int j) { return min(128, (s.nk - j * 128 + 31) & ~31); };
+    // D = A B^T over the channels, both operands 128-byte rows in shared memory
+    auto scores = [&](uint32_t d, const uint8_t* x, const uint8_t* y, int cols, uint64_t* bar) {
+      if (lane == 0) {
+        tc::fence_after_sync();
+        const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), 16), dy = tc::sw128_desc(tc::smem_u32(y), 16);
+        const uint32_t idesc = tc::idesc_f16(ab_bf16, 0, 128, cols);
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3);
+          tc::mma_f16_ss(d, dx + off, dy + off, idesc, kk > 0 ? 1u : 0u);
+        }
+        tc::mma_commit(bar);
+      }
+      __syncwarp();
+    };
+    auto issue_s = [&](int j) -> bool {
+      const int ks = j % KS;
+      if (!tc::mbar_wait(bars + C::bKF + ks, (j / KS) & 1, p.err)) return false;
+      uint8_t* k = base + C::oK + ks * C::kTile;
+      const int cols = cols_of(j);
+      // rows behind the last key are an operand of ds K
+      if (s.nk - j * 128 < cols) zero_rows(k, s.nk - j * 128, cols, HV);
+      scores(tmem + C::cS + (j & 1) * 128, base + C::oQ, k, cols, bars + C::bS + (j & 1));
+      return true;
+    };
+    auto issue_dp = [&](int j) -> bool {
+      const int vs = j % VS;
+      if (!tc::mbar_wait(bars + C::bVF + vs, (j / VS) & 1, p.err)) return false;
+      uint8_t* v = base + C::oV + vs * C::kTile;
+      const int cols = cols_of(j);
+      if (s.nk - j * 128 < cols) zero_rows(v, s.nk - j * 128, cols, HV);  // 0 (dP - delta) must not meet a NaN
+      scores(tmem + C::cDP, base + C::oDO, v, cols, bars + C::bDP);
+      if (lane == 0) tc::mma_commit(bars + C::bVE + vs);
+      __syncwarp();
+      return true;
+    };
+    if (n > 0) {
+      ok = tc::mbar_wait(bars + C::bQ, 0, p.err) && issue_s(0) && issue_dp(0);
+      if (ok && n > 1) ok = issue_s(1);
+      for (int j = 0; j < n && ok; ++j) {
+        if (!(ok = tc::mbar_wait(bars + C::bDS, j & 1, p.err))) break;
+        if (j + 1 < n && !(ok = issue_dp(j + 1))) break;
+        if (lane == 0) {
+          tc::fence_after_sync();
+          const int cols = cols_of(j);
+          const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + C::oK + (j % KS) * C::kTile), kHalfBytes);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            if (kk * 16 < cols)
+              tc::mma_f16_ts(tmem + C::cDQ, tmem + C::cS + (j & 1) * 128 + left_cols(kk), dk + 128 * kk, idesc_q,
+                             (j > 0 || kk > 0) ? 1u : 0u);
+          tc::mma_commit(bars + C::bKE + j % KS);
+          if (j == n - 1) tc::mma_commit(bars + C::bDone);
+        }
+        __syncwarp();
+        if (j + 2 < n) ok = issue_s(j + 2);
+      }
+      if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+      if (lane == 0) {
+        tc::mma_commit(bars + C::bDrain);
+        tc::mbar_wait(bars + C::bDrain, 0, nullptr);
+      }
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- compute
+    const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // column half, row
+    const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
+    const int my = t0 + r / G, g = r % G;
+    const bool mine = present && r < G * p.ntok && my < s.nq;
+    const int pos = my + shift;
+    const int klim = a.causal && mine ? min(s.nk, pos + 1) : s.nk;
+    const int kmin = __reduce_min_sync(MN_FULL_MASK, klim);
+    const int pmin = __reduce_min_sync(MN_FULL_MASK, mine ? pos : 0x7fffffff);
+    const int pmax = __reduce_max_sync(MN_FULL_MASK, mine ? pos : -0x7fffffff);
+    const int64_t row = (int64_t)(s.q0 + my) * G + g, rows = (int64_t)a.tq * G;
+    // delta = dout . out, the channels in 8s alternating between the row's two threads
+    float* dl = reinterpret_cast<float*>(base + C::oDelta);
+    {
+      float acc = 0.f;
+      if (mine) {
+        const ET* x = static_cast<const ET*>(a.dout) + (int64_t)(s.q0 + my) * a.do_st + (hk * G + g) * a.do_sh;
+        const ET* y = static_cast<const ET*>(a.out) + ((int64_t)(s.q0 + my) * a.heads + hk * G + g) * a.head_dim;
+        for (int c = w; c < a.head_dim / 8; c += 2) {
+          const uint4 xv = *reinterpret_cast<const uint4*>(x + c * 8), yv = *reinterpret_cast<const uint4*>(y + c * 8);
+          const ET* xe = reinterpret_cast<const ET*>(&xv);
+          const ET* ye = reinterpret_cast<const ET*>(&yv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc = fmaf(to_f32(xe[e]), to_f32(ye[e]), acc);
+        }
+      }
+      dl[w * 128 + r] = acc;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float delta = dl[r] + dl[128 + r];
+    if (mine && w == 0) p.delta[hk * rows + row] = delta;
+    const float nlse = mine ? -a.lse[hk * rows + row] : -INFINITY;
+    const float sl2 = a.scale * kLog2e;
+    const float* tab = BIAS ? bs.tab + (mine ? g : 0) * a.buckets : nullptr;
+    float* my_hist = hist + (BIAS ? w * a.buckets * 128 + r : 0);
+    float far_lo = 0.f, far_hi = 0.f;
+    for (int j = 0; j < n && ok; ++j) {
+      const int k0 = j * 128 + w * 64;  // this half's first key
+      const int chunks = max(0, min(2, (min(128, (s.nk - j * 128 + 31) & ~31) - w * 64) >> 5));
+      const uint32_t t_s = tmem + C::cS + (j & 1) * 128 + w * 64 + lane_sel, t_dp = tmem + C::cDP + w * 64 + lane_sel;
+      if (!(ok = tc::mbar_wait(bars + C::bS + (j & 1), (j >> 1) & 1, p.err))) break;
+      tc::fence_after_sync();
+      float x[64];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (u < chunks) tc::tmem_ld32_nowait(t_s + u * 32, x + u * 32);
+      tc::tmem_ld_wait<64>(x);
+      const bool masked = kmin < k0 + 64;
+      int kind = 0;  // bias: 1 all below the reach, 2 all above, 3 mixed
+      float add = nlse;
+      if (BIAS) {
+        kind = k0 + 63 - pmin <= -p.reach ? 1 : k0 - pmax >= p.span - 1 - p.reach ? 2 : 3;
+        if (kind == 1) add += tab[bs.idx[0]];
+        if (kind == 2) add += tab[bs.idx[p.span - 1]];
+      }
+      const int at = k0 - pos + p.reach;
+      if (BIAS && kind == 3) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e / 32 < chunks) x[e] = fmaf(x[e], sl2, tab[bs.idx[min(max(at + e, 0), p.span - 1)]] + add);
+      } else {
+        const float2 f2 = make_float2(sl2, sl2), a2 = make_float2(add, add);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float2 y = ffma2(make_float2(x[2 * e], x[2 * e + 1]), f2, a2);
+          x[2 * e] = y.x;
+          x[2 * e + 1] = y.y;
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (k0 + e >= klim) x[e] = -INFINITY;
+        exp32<true>(x);
+        exp32<true>(x + 32);
+      } else {
+        exp32<false>(x);
+        exp32<false>(x + 32);
+      }
+      if (!(ok = tc::mbar_wait(bars + C::bDP, j & 1, p.err))) break;
+      tc::fence_after_sync();
+      const float2 nd = make_float2(-delta, -delta);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (u >= chunks) break;
+        float d[32];
+        tc::tmem_ld32_nowait(t_dp + u * 32, d);
+        tc::tmem_ld_wait<32>(d);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 v = fmul2(make_float2(x[u * 32 + 2 * e], x[u * 32 + 2 * e + 1]), fadd2(make_float2(d[2 * e], d[2 * e + 1]), nd));
+          x[u * 32 + 2 * e] = v.x;
+          x[u * 32 + 2 * e + 1] = v.y;
+        }
+        put32<ET>(t_s + u * 16, x + u * 32);
+      }
+      tc::tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tma::arrive(bars + C::bDS);
+      if (BIAS && mine) {
+        // keys out of the mask have ds = 0 (chunks that do not exist are not added)
+        if (kind == 3) {
+          int cur = bs.idx[min(max(at, 0), p.span - 1)];
+          float acc = 0.f;
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            if (e / 32 >= chunks) break;
+            const int u = bs.idx[min(max(at + e, 0), p.span - 1)];
+            if (u != cur) {
+              my_hist[cur * 128] += acc;
+              acc = 0.f;
+              cur = u;
+            }
+            acc += x[e];
           }
+          if (chunks > 0) my_hist[cur * 128] += acc;
+        } else {
+          float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (e / 16 < chunks) acc = fadd2(acc, make_float2(x[2 * e], x[2 * e + 1]));
+          if (kind == 1) far_lo += acc.x + acc.y;
+          else far_hi += acc.x + acc.y;
         }
       }
     }
+    if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+    if (ok && n > 0) {
+      ok = tc::mbar_wait(bars + C::bDone, 0, p.err);
+      tc::fence_after_sync();
+    }
+    if (ok) {
+      ET* dst = static_cast<ET*>(a.dq) + ((int64_t)(s.q0 + my) * a.heads + hk * G + g) * a.head_dim;
+#pragma unroll
+      for (int u = 0; u < DT / 64; ++u) {
+        const int c0 = (w * (DT / 64) + u) * 32;
+        float o[32];
+        if (n > 0) {
+          tc::tmem_ld32(tmem + C::cDQ + c0 + lane_sel, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (mine) store32<ET>(dst, c0, a.head_dim, o, a.scale);
+        __syncwarp();
+      }
+    }
+    if (BIAS) {
+      if (mine) {
+        my_hist[bs.idx[0] * 128] += far_lo;
+        my_hist[bs.idx[p.span - 1] * 128] += far_hi;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const int per = a.buckets * G;
+      const int64_t slots = gridDim.x / a.kv_heads;
+      for (int i = tid; i < per; i += 256) {
+        const int u = i / G, gg = i % G;
+        float acc = 0.f;
+        for (int rr = gg; rr < 128; rr += G) acc += hist[u * 128 + rr] + hist[(a.buckets + u) * 128 + rr];
+        p.part[(hk * slots + slot_id) * per + i] = acc;
+      }
+    }
   }
-  store_row(static_cast<T*>(a.dk) + ((int64_t)row * a.kv_heads + hk) * d, d, lane, dk, a.scale);
-  store_row(static_cast<T*>(a.dv) + ((int64_t)row * a.kv_heads + hk) * d, d, lane, dv, 1.f);
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
 }
 
-static unsigned blocks(int64_t warps) { return (unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)); }
+// dtable[u, hk * G + g]: the tiles' sums in order, one block per entry
+__global__ void __launch_bounds__(128) dbias_kernel(int heads, int group, int buckets, int slots, const float* __restrict__ part,
+                                                    float* __restrict__ out) {
+  __shared__ float scratch[32];
+  const int i = blockIdx.x, hk = blockIdx.y, per = buckets * group;
+  float x = 0.f;
+  for (int t = threadIdx.x; t < slots; t += 128) x += part[((int64_t)hk * slots + t) * per + i];
+  x = block_sum(x, scratch);
+  if (threadIdx.x == 0) out[(i / group) * heads + hk * group + i % group] = x;
+}
+
+// ------------------------------------------------------------------- dk, dv
+template <int DT, bool BIAS>
+struct Dkv {
+  static constexpr int HV = DT / 64;
+  static constexpr uint32_t kTile = HV * kHalfBytes;
+  static constexpr int NS = DT == 64 ? 2 : 1;  // S^T buffers in tensor memory
+  static constexpr int QS = NS + 1;            // stages of Q, dout, lse and delta
+  static constexpr uint32_t oK = 0, oV = kTile, oRing = 2 * kTile, oRows = oRing + QS * 2 * kTile;  // rows: [QS][2][128] floats
+  static constexpr uint32_t oBars = oRows + QS * 1024;
+  static constexpr int bKV = 0, bF = 1, bE = bF + QS, bS = bE + QS, bP = bS + NS, bDP = bP + NS, bDS = bDP + 1, bDone = bDS + 1,
+                       bDrain = bDone + 1, kNumBars = bDrain + 1;
+  static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
+  static constexpr uint32_t oCol = oMisc + 16;  // [128] (token, head * buckets) of a column
+  static constexpr uint32_t oTab = oCol + 128 * 8;
+  static constexpr uint32_t bytes(int buckets, int group, int span) {
+    return oTab + (BIAS ? ((buckets * group * 4 + 15) / 16) * 16 + span : 0) + 1024;
+  }
+  static constexpr uint32_t cS = 0, cDP = NS * 128, cDV = cDP + 128, cDK = cDV + DT;
+};
+
+template <typename ET, int DT, bool BIAS>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+               const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+               const __grid_constant__ BwdParams p, const __grid_constant__ Borders bo) {
+  using C = Dkv<DT, BIAS>;
+  constexpr int HV = C::HV, NS = C::NS, QS = C::QS;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(base + C::oMisc);
+  int2* col = reinterpret_cast<int2*>(base + C::oCol);
+  const mn_packed_args& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
+  const int hk = blockIdx.x % a.kv_heads, slot_id = blockIdx.x / a.kv_heads;
+  BiasSmem bs;
+  bs.tab = reinterpret_cast<float*>(base + C::oTab);
+  bs.idx = reinterpret_cast<uint8_t*>(bs.tab) + (BIAS ? (a.buckets * G * 4 + 15) / 16 * 16 : 0);
+
+  if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
+  if (warp == 1) {
+    const int b = seq_of_slot(a.cu_k, a.nseq, 128, a.tk, slot_id);
+    if (lane == 0) misc[1] = (uint32_t)b;
+  }
+  if (warp == 2 && lane == 0) {
+    for (int i = 0; i < C::kNumBars; ++i)
+      tc::mbar_init(bars + i, i >= C::bF && i < C::bE ? 2 : (i >= C::bP && i < C::bDP) || i == C::bDS ? 8 : 1);
+    tc::fence_mbar_init();
+  }
+  if (warp == 3 && lane == 0) {
+    tma::prefetch_map(&tm_q);
+    tma::prefetch_map(&tm_do);
+    tma::prefetch_map(&tm_k);
+    tma::prefetch_map(&tm_v);
+  }
+  if (BIAS) {
+    fill_bias(p, bo, hk, bs);
+    if (tid < 128) col[tid] = make_int2(tid / G, (tid % G) * a.buckets);
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = misc[0];
+  const int b = (int)misc[1];
+  const Seq s = load_seq_or_tail(a, b);
+  const int local = slot_id - slot_of_seq(a.cu_k, b, 128, a.tk);
+  const int k0 = local * 128;
+  const bool present = local >= 0 && k0 < s.slot;
+  const int shift = s.nk - s.nq;
+  // query tiles that see a key of this tile: [i0, i0 + n)
+  const int i0 = a.causal ? max(0, k0 - shift) / p.ntok : 0;
+  const int n = present && k0 < s.nk ? max(0, (s.nq + p.ntok - 1) / p.ntok - i0) : 0;
+  constexpr int ab_bf16 = std::is_same<ET, __nv_bfloat16>::value ? 1 : 0;
+  // bias of a whole tile pair: 1 all distances below the reach, 2 all above, 3 mixed
+  auto kind_of = [&](int t0) {
+    return k0 + 127 - (t0 + shift) <= -p.reach ? 1 : k0 - (t0 + p.ntok - 1 + shift) >= p.span - 1 - p.reach ? 2 : 3;
+  };
+  bool ok = true;
+
+  if (warp == 9) {
+    // ---------------------------------------------------------------- loads
+    if (n > 0) {
+      if (lane == 0) {
+        tma::expect_tx(bars + C::bKV, 2 * C::kTile);
+        for (int h = 0; h < HV; ++h) {
+          load_3d(tc::smem_u32(base + C::oK + h * kHalfBytes), &tm_k, h * 64, hk, s.k0 + k0, bars + C::bKV);
+          load_3d(tc::smem_u32(base + C::oV + h * kHalfBytes), &tm_v, h * 64, hk, s.k0 + k0, bars + C::bKV);
+        }
+      }
+      int done = 0;
+      const int64_t rows = (int64_t)a.tq * G;
+      for (int i = 0; i < n && ok; ++i) {
+        const int st = i % QS, t0 = (i0 + i) * p.ntok;
+        if (i >= QS && !(ok = tc::mbar_wait(bars + C::bE + st, (i / QS - 1) & 1, p.err))) break;
+        uint8_t* q = base + C::oRing + st * 2 * C::kTile;
+        if (lane == 0) {
+          tma::expect_tx(bars + C::bF + st, 2u * HV * 128u * (uint32_t)(G * p.ntok));
+          for (int h = 0; h < HV; ++h) {
+            tma::load_4d(tc::smem_u32(q + h * kHalfBytes), &tm_q, h * 64, 0, hk, s.q0 + t0, bars + C::bF + st);
+            tma::load_4d(tc::smem_u32(q + C::kTile + h * kHalfBytes), &tm_do, h * 64, 0, hk, s.q0 + t0, bars + C::bF + st);
+          }
+        }
+        // -lse (with the bias where it is the same for the whole tile) and
+        // -delta of the rows; rows of no query give p = 0
+        float* x = reinterpret_cast<float*>(base + C::oRows) + st * 256;
+        const int valid = min(p.ntok, s.nq - t0) * G;
+        const int64_t first = hk * rows + (int64_t)(s.q0 + t0) * G;
+        const int kind = BIAS ? kind_of(t0) : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = e * 32 + lane;
+          float l = -INFINITY, d = 0.f;
+          if (r < valid) {
+            l = -a.lse[first + r];
+            d = -p.delta[first + r];
+            if (BIAS && kind != 3) l += bs.tab[col[r].y + bs.idx[kind == 1 ? 0 : p.span - 1]];
+          }
+          x[r] = l;
+          x[128 + r] = d;
+        }
+        __syncwarp();
+        if (lane == 0) tma::arrive(bars + C::bF + st);
+        done = i + 1;
+      }
+      if (lane == 0) {
+        if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+        // every copy issued has landed before the CTA may release its shared memory
+        tc::mbar_wait(bars + C::bKV, 0, nullptr);
+        for (int i = max(0, done - QS); i < done; ++i) tc::mbar_wait(bars + C::bF + i % QS, (i / QS) & 1, nullptr);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ----------------------------------------------------------------- MMAs
+    // While the compute warps turn S(i) into p the tensor core finishes
+    // dK += ds(i - 1) Q and dP(i); while they form ds(i), dV += p(i) dout and
+    // the next S.
+    constexpr uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, 128), idesc_g = tc::idesc_f16(ab_bf16, 1, 128, DT);
+    auto stage = [&](int i) { return base + C::oRing + (i % QS) * 2 * C::kTile; };
+    auto scores = [&](uint32_t d, const uint8_t* x, const uint8_t* y, uint64_t* bar) {
+      if (lane == 0) {
+        tc::fence_after_sync();
+        const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), 16), dy = tc::sw128_desc(tc::smem_u32(y), 16);
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3);
+          tc::mma_f16_ss(d, dx + off, dy + off, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        tc::mma_commit(bar);
+      }
+      __syncwarp();
+    };
+    auto issue_s = [&](int i) -> bool {
+      if (!tc::mbar_wait(bars + C::bF + i % QS, (i / QS) & 1, p.err)) return false;
+      const int valid = min(p.ntok, s.nq - (i0 + i) * p.ntok) * G;
+      if (valid < 128) {  // rows of no query are an operand of dK and dV
+        zero_rows(stage(i), valid, 128, HV);
+        zero_rows(stage(i) + C::kTile, valid, 128, HV);
+      }
+      scores(tmem + C::cS + (i % NS) * 128, base + C::oK, stage(i), bars + C::bS + i % NS);
+      return true;
+    };
+    auto grads = [&](uint32_t d, uint32_t left, const uint8_t* x, bool more) {  // D += left x
+      const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), kHalfBytes);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        tc::mma_f16_ts(d, left + left_cols(kk), dx + 128 * kk, idesc_g, (more || kk > 0) ? 1u : 0u);
+    };
+    if (n > 0) {
+      ok = tc::mbar_wait(bars + C::bKV, 0, p.err);
+      for (int i = 0; i < NS && i < n && ok; ++i) ok = issue_s(i);
+      if (ok) scores(tmem + C::cDP, base + C::oV, stage(0) + C::kTile, bars + C::bDP);
+      for (int i = 0; i < n && ok; ++i) {
+        if (!(ok = tc::mbar_wait(bars + C::bP + i % NS, (i / NS) & 1, p.err))) break;
+        if (lane == 0) {
+          tc::fence_after_sync();
+          grads(tmem + C::cDV, tmem + C::cS + (i % NS) * 128, stage(i) + C::kTile, i > 0);
+        }
+        __syncwarp();
+        // S(i + NS) overwrites p(i), which the product before it in order has read
+        if (i + NS < n && !(ok = issue_s(i + NS))) break;
+        if (!(ok = tc::mbar_wait(bars + C::bDS, i & 1, p.err))) break;
+        if (lane == 0) {
+          tc::fence_after_sync();
+          grads(tmem + C::cDK, tmem + C::cDP, stage(i), i > 0);
+          tc::mma_commit(bars + C::bE + i % QS);
+          if (i == n - 1) tc::mma_commit(bars + C::bDone);
+        }
+        __syncwarp();
+        if (i + 1 < n) scores(tmem + C::cDP, base + C::oV, stage(i + 1) + C::kTile, bars + C::bDP);
+      }
+      if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+      if (lane == 0) {
+        tc::mma_commit(bars + C::bDrain);
+        tc::mbar_wait(bars + C::bDrain, 0, nullptr);
+      }
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- compute
+    const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // column half, key row
+    const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
+    const int key = k0 + r;
+    const float sl2 = a.scale * kLog2e;
+    for (int i = 0; i < n && ok; ++i) {
+      const int st = i % QS, t0 = (i0 + i) * p.ntok;
+      const uint32_t t_s = tmem + C::cS + (i % NS) * 128 + w * 64 + lane_sel, t_dp = tmem + C::cDP + w * 64 + lane_sel;
+      const float* nl = reinterpret_cast<const float*>(base + C::oRows) + st * 256 + w * 64;
+      // columns from here on see this key; the warp's last key sees the latest start
+      const int c0 = a.causal ? (key - shift - t0) * G - w * 64 : 0;
+      const bool masked = a.causal && (k0 + ((warp & 3) * 32 + 31) - shift - t0) * G > w * 64;
+      if (!(ok = tc::mbar_wait(bars + C::bF + st, (i / QS) & 1, p.err))) break;  // lse and delta are there
+      if (!(ok = tc::mbar_wait(bars + C::bS + i % NS, (i / NS) & 1, p.err))) break;
+      tc::fence_after_sync();
+      float x[64];
+      tc::tmem_ld32_nowait(t_s, x);
+      tc::tmem_ld32_nowait(t_s + 32, x + 32);
+      tc::tmem_ld_wait<64>(x);
+      if (BIAS && kind_of(t0) == 3) {
+        const int at = key - t0 - shift + p.reach;
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+          const int2 c = col[w * 64 + e];
+          x[e] = fmaf(x[e], sl2, nl[e] + bs.tab[c.y + bs.idx[min(max(at - c.x, 0), p.span - 1)]]);
+        }
+      } else {
+        const float2 f2 = make_float2(sl2, sl2);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float4 l = reinterpret_cast<const float4*>(nl)[e];
+          const float2 y0 = ffma2(make_float2(x[4 * e], x[4 * e + 1]), f2, make_float2(l.x, l.y));
+          const float2 y1 = ffma2(make_float2(x[4 * e + 2], x[4 * e + 3]), f2, make_float2(l.z, l.w));
+          x[4 * e] = y0.x; x[4 * e + 1] = y0.y; x[4 * e + 2] = y1.x; x[4 * e + 3] = y1.y;
+        }
+      }
+      const bool tail = min(p.ntok, s.nq - t0) * G < 128;  // columns of no query: exactly 0
+      if (masked || tail) {
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e < c0) x[e] = -INFINITY;
+        }
+        exp32<true>(x);
+        exp32<true>(x + 32);
+      } else {
+        exp32<false>(x);
+        exp32<false>(x + 32);
+      }
+      put32<ET>(t_s, x);
+      put32<ET>(t_s + 16, x + 32);
+      tc::tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tma::arrive(bars + C::bP + i % NS);
+      if (!(ok = tc::mbar_wait(bars + C::bDP, i & 1, p.err))) break;
+      tc::fence_after_sync();
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float d[32];
+        tc::tmem_ld32_nowait(t_dp + u * 32, d);
+        tc::tmem_ld_wait<32>(d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 nd = reinterpret_cast<const float4*>(nl + 128)[u * 8 + e];
+          const int c = u * 32 + 4 * e;
+          const float2 y0 = fmul2(make_float2(x[c], x[c + 1]), fadd2(make_float2(d[4 * e], d[4 * e + 1]), make_float2(nd.x, nd.y)));
+          const float2 y1 = fmul2(make_float2(x[c + 2], x[c + 3]), fadd2(make_float2(d[4 * e + 2], d[4 * e + 3]), make_float2(nd.z, nd.w)));
+          d[4 * e] = y0.x; d[4 * e + 1] = y0.y; d[4 * e + 2] = y1.x; d[4 * e + 3] = y1.y;
+        }
+        put32<ET>(t_dp + u * 16, d);
+      }
+      tc::tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tma::arrive(bars + C::bDS);
+    }
+    if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+    if (ok && n > 0) {
+      ok = tc::mbar_wait(bars + C::bDone, 0, p.err);
+      tc::fence_after_sync();
+    }
+    if (ok) {
+      // the first half's warps store dV, the second's dK
+      const bool mine = present && key < s.slot;
+      const float f = key < s.nk ? (w == 0 ? 1.f : a.scale) : 0.f;
+      ET* dst = static_cast<ET*>(w == 0 ? a.dv : a.dk) + ((int64_t)(s.k0 + key) * a.kv_heads + hk) * a.head_dim;
+#pragma unroll
+      for (int u = 0; u < DT / 32; ++u) {
+        float o[32];
+        if (n > 0) tc::tmem_ld32(tmem + (w == 0 ? C::cDV : C::cDK) + u * 32 + lane_sel, o);
+        if (n == 0 || key >= s.nk) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (mine) store32<ET>(dst, u * 32, a.head_dim, o, f);
+        __syncwarp();
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------- host
+struct BwdSizes {
+  int ntok;
+  int64_t q_slots, k_slots;
+  size_t delta_bytes, bytes;
+};
+static BwdSizes sizes_of(const mn_packed_args* a) {
+  BwdSizes z;
+  const int g = a->heads / a->kv_heads;
+  z.ntok = 128 / g;
+  z.q_slots = tile_slots(a->tq, a->nseq, z.ntok);
+  z.k_slots = tile_slots(a->tk, a->nseq, 128);
+  z.delta_bytes = ((size_t)a->tq * a->heads * 4 + 255) / 256 * 256;
+  z.bytes = z.delta_bytes + (a->bias_table ? (size_t)z.q_slots * a->heads * a->buckets * 4 : 0);
+  return z;
+}
+
+template <typename ET, int DT, bool BIAS>
+static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSizes& z, void* ws, int* err, cudaStream_t st) {
+  constexpr bool bf16 = std::is_same<ET, __nv_bfloat16>::value;
+  BwdParams p;
+  p.a = *a;
+  p.group = a->heads / a->kv_heads;
+  p.ntok = z.ntok;
+  p.span = p.reach = 0;
+  if (BIAS) {
+    const int last = bo.n ? bo.at[bo.n - 1] : 1;
+    p.reach = last;
+    p.span = (bo.two_sided ? 2 : 1) * last + 1;
+  }
+  p.delta = static_cast<float*>(ws);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + z.delta_bytes);
+  p.err = err;
+  CUtensorMap mq, mdo, mk, mv;
+  if (!bind_context() || !map_q(&mq, bf16, a->q, a->q_st, a->q_sh, a->tq, a->heads, a->kv_heads, a->head_dim, z.ntok) ||
+      !map_q(&mdo, bf16, a->dout, a->do_st, a->do_sh, a->tq, a->heads, a->kv_heads, a->head_dim, z.ntok) ||
+      !map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim) ||
+      !map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim))
+    return false;
+  if (z.q_slots * a->kv_heads > 0x7fffffff || z.k_slots * a->kv_heads > 0x7fffffff) return false;
+  auto kq = dq_kernel<ET, DT, BIAS>;
+  auto kkv = dkv_kernel<ET, DT, BIAS>;
+  const size_t sq = Dq<DT, BIAS>::bytes(a->buckets, p.group, p.span), skv = Dkv<DT, BIAS>::bytes(a->buckets, p.group, p.span);
+  if (!ensure_smem(kq, sq) || !ensure_smem(kkv, skv)) return false;
+  kq<<<(unsigned)(z.q_slots * a->kv_heads), kBwdThreads, sq, st>>>(mq, mdo, mk, mv, p, bo);
+  if (a->tk > 0) kkv<<<(unsigned)(z.k_slots * a->kv_heads), kBwdThreads, skv, st>>>(mq, mdo, mk, mv, p, bo);
+  if (BIAS)
+    dbias_kernel<<<dim3(a->buckets * p.group, a->kv_heads), 128, 0, st>>>(a->heads, p.group, a->buckets, (int)z.q_slots, p.part,
+                                                                         a->dbias);
+  return true;
+}
+
+template <typename ET, int DT>
+static bool launch_bwd_d(const mn_packed_args* a, const Borders& bo, const BwdSizes& z, void* ws, int* err, cudaStream_t st) {
+  return a->bias_table ? launch_bwd<ET, DT, true>(a, bo, z, ws, err, st) : launch_bwd<ET, DT, false>(a, bo, z, ws, err, st);
+}
 
 }  // namespace pk
 }  // namespace mn
@@ -126,33 +802,28 @@ static unsigned blocks(int64_t warps) { return (unsigned)((warps + kThreads / 32
 using namespace mn;
 
 extern "C" size_t mn_packed_attention_backward_workspace_bytes(const mn_packed_args* a) {
-  if (!a || a->tq < 1 || a->heads < 1) return 0;
-  return (size_t)a->tq * a->heads * 4 * (1 + (a->bias_table ? a->buckets : 0));
+  Borders bo;
+  if (pk::check(a, &bo, true) != MN_OK || a->tq == 0) return 0;
+  return pk::sizes_of(a).bytes;
 }
 
-extern "C" int mn_packed_attention_backward(const mn_packed_args* args, void* workspace, size_t workspace_bytes, int* status,
+extern "C" int mn_packed_attention_backward(const mn_packed_args* a, void* workspace, size_t workspace_bytes, int* status,
                                             void* stream) {
   Borders bo;
-  const int rc = pk::check(args, &bo, true);
+  const int rc = pk::check(a, &bo, true);
   if (rc != MN_OK) return rc;
-  (void)status;
-  if (args->tq == 0 && args->tk == 0) return MN_OK;
-  if (workspace_bytes < mn_packed_attention_backward_workspace_bytes(args) || (args->tq > 0 && !workspace))
-    return MN_ERR_WORKSPACE;
+  if (a->tq == 0) return MN_ERR_ARG;  // no query: the gradients are 0, nothing to launch
+  const pk::BwdSizes z = pk::sizes_of(a);
+  if (!workspace || workspace_bytes < z.bytes) return MN_ERR_WORKSPACE;
   cudaGetLastError();
   auto st = static_cast<cudaStream_t>(stream);
-  float* delta = static_cast<float*>(workspace);
-  float* part = delta + (size_t)args->tq * args->heads;
-  const unsigned nq = pk::blocks((int64_t)args->tq * args->heads), nk = pk::blocks((int64_t)args->tk * args->kv_heads);
-  if (args->dtype == MN_F16) {
-    if (nq) pk::dq_kernel<__half><<<nq, pk::kThreads, 0, st>>>(*args, bo, delta, part);
-    if (nk) pk::dkv_kernel<__half><<<nk, pk::kThreads, 0, st>>>(*args, bo, delta);
-  } else {
-    if (nq) pk::dq_kernel<__nv_bfloat16><<<nq, pk::kThreads, 0, st>>>(*args, bo, delta, part);
-    if (nk) pk::dkv_kernel<__nv_bfloat16><<<nk, pk::kThreads, 0, st>>>(*args, bo, delta);
-  }
-  if (args->bias_table)
-    pk::dbias_kernel<<<dim3(args->buckets, args->heads), pk::kThreads, 0, st>>>(part, args->tq, args->heads, args->buckets,
-                                                                              args->dbias);
+  bool done;
+  if (a->dtype == MN_F16)
+    done = a->head_dim <= 64 ? pk::launch_bwd_d<__half, 64>(a, bo, z, workspace, status, st)
+                             : pk::launch_bwd_d<__half, 128>(a, bo, z, workspace, status, st);
+  else
+    done = a->head_dim <= 64 ? pk::launch_bwd_d<__nv_bfloat16, 64>(a, bo, z, workspace, status, st)
+                             : pk::launch_bwd_d<__nv_bfloat16, 128>(a, bo, z, workspace, status, st);
+  if (!done) return MN_ERR_UNSUPPORTED;
   return cudaGetLastError() == cudaSuccess ? MN_OK : MN_ERR_LAUNCH;
 }

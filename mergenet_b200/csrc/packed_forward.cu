@@ -485,7 +485,7 @@ int check(const mn_packed_args* a, Borders* bo, bool backward) {
   if (backward && a->tk > 0 && (!a->dk || !a->dv)) return MN_ERR_ARG;
   if (a->dtype != MN_F16 && a->dtype != MN_BF16) return MN_ERR_UNSUPPORTED;
   const int g = a->heads / a->kv_heads;
-  if (a->head_dim > 128 || a->head_dim % 8 || g > 128) return MN_ERR_UNSUPPORTED;
+  if (a->head_dim > 128 || a->head_dim % 8 || g > 128 || a->kv_heads > 65535) return MN_ERR_UNSUPPORTED;
   if ((int64_t)a->tq * g >= (1 << 30) || (int64_t)a->tk * g >= (1 << 30)) return MN_ERR_UNSUPPORTED;
   if (!rows_ok(a->q, a->q_st, a->q_sh, a->tq, a->heads) || !rows_ok(a->k, a->k_st, a->k_sh, a->tk, a->kv_heads) ||
       !rows_ok(a->v, a->v_st, a->v_sh, a->tk, a->kv_heads) ||
@@ -496,7 +496,7 @@ int check(const mn_packed_args* a, Borders* bo, bool backward) {
     if (a->bias_dtype < 0 || a->bias_dtype > 2 || (backward && !a->dbias)) return MN_ERR_ARG;
     if (!make_borders(bo, a->buckets, a->two_sided, a->num_borders, a->borders)) return MN_ERR_ARG;
     const int last = bo->n ? bo->at[bo->n - 1] : 1;
-    if (a->buckets > 64 || ((a->two_sided ? 2 : 1) * (int64_t)last + 1) * g > 8192) return MN_ERR_UNSUPPORTED;
+    if (a->buckets > 48 || a->buckets * g > 4096 || ((a->two_sided ? 2 : 1) * (int64_t)last + 1) * g > 8192) return MN_ERR_UNSUPPORTED;
   }
   return MN_OK;
 }
@@ -529,6 +529,7 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   using F = Fwd<DT, BIAS>;
   constexpr bool bf16 = std::is_same<ET, __nv_bfloat16>::value;
   CUtensorMap mq, mk, mv;
+  if (!bind_context()) return false;
   if (!map_q(&mq, bf16, a->q, a->q_st, a->q_sh, a->tq, a->heads, a->kv_heads, a->head_dim, pl.ntok)) return false;
   if (!map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim)) return false;
   if (!map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim)) return false;

@@ -136,6 +136,13 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to, int h
 }
 
 // ------------------------------------------------------------------- host
+// Tensor maps are encoded through the driver, which wants a current context;
+// a host thread that has made no runtime call yet (an autograd worker) has
+// none until its device is set.
+inline bool bind_context() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
 // Query-side rows [rows, heads, d] as (d, g, key head, row) with boxes of 64
 // channels x g heads x n rows: row n * g + i of the tile is head i of row n.
 inline bool map_q(CUtensorMap* map, bool bf16, const void* p, int64_t st, int64_t sh, int rows, int heads, int kv_heads,

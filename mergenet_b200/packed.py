@@ -26,7 +26,8 @@ from .attention import _STATUS, _status
 
 MAX_HEAD_DIM = 128
 MAX_GROUP = 128       # query heads that may share a key head
-MAX_BUCKETS = 64      # of a table used inside the attention
+MAX_BUCKETS = 48      # of a table used inside the attention
+MAX_BIAS_ENTRIES = 4096  # buckets x grouped heads
 MAX_BIAS_VALUES = 8192  # distances x grouped heads that a kernel keeps on chip
 
 
@@ -246,7 +247,7 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
     h, hk, d = q.shape[1], k.shape[1], q.shape[2]
     if d < 8 or d > MAX_HEAD_DIM or d % 8:
         raise ValueError(f"head_dim {d} is not supported: a multiple of 8 up to {MAX_HEAD_DIM}")
-    if hk < 1 or h < 1 or h % hk or h // hk > MAX_GROUP:
+    if not 1 <= hk <= 65535 or h < 1 or h % hk or h // hk > MAX_GROUP:
         raise ValueError(f"{h} query heads must be a multiple of the {hk} key heads, at most {MAX_GROUP} to one")
     if cu_seqlens_k is None:
         if q.shape[0] != k.shape[0]:
@@ -264,9 +265,9 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
     if bias_table is not None:
         _check_table(bias_table, buckets, h)
         sides = 2 if buckets.two_sided else 1
-        if buckets.num_buckets > MAX_BUCKETS or (sides * buckets.borders[-1] + 1) * (h // hk) > MAX_BIAS_VALUES:
-            raise ValueError(f"{buckets} with {h // hk} grouped heads does not fit: at most {MAX_BUCKETS} buckets, and "
-                             f"{MAX_BIAS_VALUES} distances x grouped heads")
+        if buckets.num_buckets > MAX_BUCKETS or buckets.num_buckets * (h // hk) > MAX_BIAS_ENTRIES or (sides * buckets.borders[-1] + 1) * (h // hk) > MAX_BIAS_VALUES:
+            raise ValueError(f"{buckets} with {h // hk} grouped heads does not fit: at most {MAX_BUCKETS} buckets, "
+                             f"{MAX_BIAS_ENTRIES} buckets x grouped heads and {MAX_BIAS_VALUES} distances x grouped heads")
     if max(q.shape[0], k.shape[0]) * max(h // hk, 1) >= 1 << 30:
         raise ValueError("at most 2^30 rows x grouped heads")
     L.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, bias_table)
