@@ -336,7 +336,7 @@ int mn_attention(int batch, int nq, int nk, int heads, int head_dim, int dtype,
  * strides (_st per row, _sh per head) and contiguous channels, fp16 or bf16;
  * head_dim a multiple of 8 up to 128; pointers 16-byte aligned and strides
  * multiples of 8.  out, dq, dk, dv: contiguous, of the same type.  bias_table
- * [buckets, heads] contiguous, of bias_dtype; dbias fp32, the same shape.
+ * [buckets, heads] contiguous, of bias_dtype; dbias the same.
  * lse [kv_heads, tq, heads / kv_heads] fp32: log2 of each row's sum of
  * exponentials (+inf where no key is seen); NULL when no backward follows. */
 typedef struct mn_packed_args {
@@ -349,7 +349,7 @@ typedef struct mn_packed_args {
   /* backward only */
   const void* dout;
   void *dq, *dk, *dv;
-  float* dbias;
+  void* dbias;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, do_st, do_sh;
   int32_t nseq, tq, tk, heads, kv_heads, head_dim, dtype, causal;
   int32_t bias_dtype, buckets, two_sided, num_borders;
@@ -371,9 +371,9 @@ int mn_packed_attention_backward(const mn_packed_args* args, void* workspace,
 
 /* bias[h, i, j] = table[bucket(j - (i + query_start)), h] for queries x keys
  * positions, and the table's gradient: dtable[u, h] = the sum of dbias[h, i,
- * j] over the positions of bucket u, in a fixed order and fp32.  table
- * [buckets, heads], bias and dbias [heads, queries, keys], all contiguous and
- * of one dtype; dtable fp32 [buckets, heads].  Buckets as above. */
+ * j] over the positions of bucket u, summed in fp32 in a fixed order.  table
+ * and dtable [buckets, heads], bias and dbias [heads, queries, keys], all
+ * contiguous and of one dtype.  Buckets as above. */
 int mn_relative_bias(int heads, int queries, int keys, int query_start,
                      int buckets, int two_sided, int num_borders,
                      const int32_t* borders, int dtype, const void* table,
@@ -383,7 +383,7 @@ size_t mn_relative_bias_backward_workspace_bytes(int heads, int queries,
 int mn_relative_bias_backward(int heads, int queries, int keys,
                               int query_start, int buckets, int two_sided,
                               int num_borders, const int32_t* borders,
-                              int dtype, const void* dbias, float* dtable,
+                              int dtype, const void* dbias, void* dtable,
                               void* workspace, size_t workspace_bytes,
                               void* stream);
 

@@ -7,6 +7,7 @@ point of the package raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
@@ -57,6 +58,9 @@ class PackedArgs(ctypes.Structure):
     )
 
 
+# the same bytes, several times faster to fill than the structure
+PACKED_ARGS = struct.Struct("@15P8q12ifi")
+
 _SIGNATURES = {
     "mn_version": (c_int, []),
     "mn_neighbor_table_width": (c_int, [c_int, c_int, c_double, POINTER(c_int)]),
@@ -95,10 +99,10 @@ _SIGNATURES = {
                                    c_int, c_int, c_int, c_float, _P, c_int, _P, _P]),
     "mn_attention": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, _P, c_int64, c_int64, c_int64, _P, _P,
                              c_int64, c_int64, c_int64, c_int, c_float, _P, c_int, _P, _P]),
-    "mn_packed_attention_workspace_bytes": (c_size_t, [POINTER(PackedArgs)]),
-    "mn_packed_attention": (c_int, [POINTER(PackedArgs), _P, c_size_t, _P, _P]),
-    "mn_packed_attention_backward_workspace_bytes": (c_size_t, [POINTER(PackedArgs)]),
-    "mn_packed_attention_backward": (c_int, [POINTER(PackedArgs), _P, c_size_t, _P, _P]),
+    "mn_packed_attention_workspace_bytes": (c_size_t, [_P]),
+    "mn_packed_attention": (c_int, [_P, _P, c_size_t, _P, _P]),
+    "mn_packed_attention_backward_workspace_bytes": (c_size_t, [_P]),
+    "mn_packed_attention_backward": (c_int, [_P, _P, c_size_t, _P, _P]),
     "mn_relative_bias": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, c_int, _P, _P, _P]),
     "mn_relative_bias_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "mn_relative_bias_backward": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, c_int, _P, _P, _P,

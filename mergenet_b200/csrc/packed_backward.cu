@@ -160,12 +160,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int nk = 0, nv = 0;
       for (int j = 0; j < n && ok; ++j) {
         const int ks = j % KS, vs = j % VS;
-        if (j >= KS && !(ok = tc::mbar_wait(bars + C::bKE + ks, (j / KS - 1) & 1, p.err))) break;
+        if (j >= KS && !(ok = wait(bars + C::bKE + ks, (j / KS - 1) & 1, p.err))) break;
         tma::expect_tx(bars + C::bKF + ks, C::kTile);
         for (int h = 0; h < HV; ++h)
           load_3d(tc::smem_u32(base + C::oK + ks * C::kTile + h * kHalfBytes), &tm_k, h * 64, hk, s.k0 + j * 128, bars + C::bKF + ks);
         nk = j + 1;
-        if (j >= VS && !(ok = tc::mbar_wait(bars + C::bVE + vs, (j / VS - 1) & 1, p.err))) break;
+        if (j >= VS && !(ok = wait(bars + C::bVE + vs, (j / VS - 1) & 1, p.err))) break;
         tma::expect_tx(bars + C::bVF + vs, C::kTile);
         for (int h = 0; h < HV; ++h)
           load_3d(tc::smem_u32(base + C::oV + vs * C::kTile + h * kHalfBytes), &tm_v, h * 64, hk, s.k0 + j * 128, bars + C::bVF + vs);
@@ -173,9 +173,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
       // every copy issued has landed before the CTA may release its shared memory
-      tc::mbar_wait(bars + C::bQ, 0, nullptr);
-      for (int j = max(0, nk - KS); j < nk; ++j) tc::mbar_wait(bars + C::bKF + j % KS, (j / KS) & 1, nullptr);
-      for (int j = max(0, nv - VS); j < nv; ++j) tc::mbar_wait(bars + C::bVF + j % VS, (j / VS) & 1, nullptr);
+      wait(bars + C::bQ, 0, nullptr);
+      for (int j = max(0, nk - KS); j < nk; ++j) wait(bars + C::bKF + j % KS, (j / KS) & 1, nullptr);
+      for (int j = max(0, nv - VS); j < nv; ++j) wait(bars + C::bVF + j % VS, (j / VS) & 1, nullptr);
     }
     __syncwarp();
   } else if (warp == 8) {
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     auto cols_of = [&](int j) { return min(128, (s.nk - j * 128 + 31) & ~31); };
     // D = A B^T over the channels, both operands 128-byte rows in shared memory
     auto scores = [&](uint32_t d, const uint8_t* x, const uint8_t* y, int cols, uint64_t* bar) {
-      if (lane == 0) {
+      if (elect_one()) {
         tc::fence_after_sync();
         const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), 16), dy = tc::sw128_desc(tc::smem_u32(y), 16);
         const uint32_t idesc = tc::idesc_f16(ab_bf16, 0, 128, cols);
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     };
     auto issue_s = [&](int j) -> bool {
       const int ks = j % KS;
-      if (!tc::mbar_wait(bars + C::bKF + ks, (j / KS) & 1, p.err)) return false;
+      if (!wait(bars + C::bKF + ks, (j / KS) & 1, p.err)) return false;
       uint8_t* k = base + C::oK + ks * C::kTile;
       const int cols = cols_of(j);
       // rows behind the last key are an operand of ds K
@@ -211,22 +211,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     };
     auto issue_dp = [&](int j) -> bool {
       const int vs = j % VS;
-      if (!tc::mbar_wait(bars + C::bVF + vs, (j / VS) & 1, p.err)) return false;
+      if (!wait(bars + C::bVF + vs, (j / VS) & 1, p.err)) return false;
       uint8_t* v = base + C::oV + vs * C::kTile;
       const int cols = cols_of(j);
       if (s.nk - j * 128 < cols) zero_rows(v, s.nk - j * 128, cols, HV);  // 0 (dP - delta) must not meet a NaN
       scores(tmem + C::cDP, base + C::oDO, v, cols, bars + C::bDP);
-      if (lane == 0) tc::mma_commit(bars + C::bVE + vs);
+      if (elect_one()) tc::mma_commit(bars + C::bVE + vs);
       __syncwarp();
       return true;
     };
     if (n > 0) {
-      ok = tc::mbar_wait(bars + C::bQ, 0, p.err) && issue_s(0) && issue_dp(0);
+      ok = wait(bars + C::bQ, 0, p.err) && issue_s(0) && issue_dp(0);
       if (ok && n > 1) ok = issue_s(1);
       for (int j = 0; j < n && ok; ++j) {
-        if (!(ok = tc::mbar_wait(bars + C::bDS, j & 1, p.err))) break;
+        if (!(ok = wait(bars + C::bDS, j & 1, p.err))) break;
         if (j + 1 < n && !(ok = issue_dp(j + 1))) break;
-        if (lane == 0) {
+        if (elect_one()) {
           tc::fence_after_sync();
           const int cols = cols_of(j);
           const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + C::oK + (j % KS) * C::kTile), kHalfBytes);
@@ -242,9 +242,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (j + 2 < n) ok = issue_s(j + 2);
       }
       if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
-      if (lane == 0) {
+      if (elect_one()) {
         tc::mma_commit(bars + C::bDrain);
-        tc::mbar_wait(bars + C::bDrain, 0, nullptr);
+        wait(bars + C::bDrain, 0, nullptr);
       }
     }
     __syncwarp();
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int k0 = j * 128 + w * 64;  // this half's first key
       const int chunks = max(0, min(2, (min(128, (s.nk - j * 128 + 31) & ~31) - w * 64) >> 5));
       const uint32_t t_s = tmem + C::cS + (j & 1) * 128 + w * 64 + lane_sel, t_dp = tmem + C::cDP + w * 64 + lane_sel;
-      if (!(ok = tc::mbar_wait(bars + C::bS + (j & 1), (j >> 1) & 1, p.err))) break;
+      if (!(ok = wait(bars + C::bS + (j & 1), (j >> 1) & 1, p.err))) break;
       tc::fence_after_sync();
       float x[64];
 #pragma unroll
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         exp32<false>(x);
         exp32<false>(x + 32);
       }
-      if (!(ok = tc::mbar_wait(bars + C::bDP, j & 1, p.err))) break;
+      if (!(ok = wait(bars + C::bDP, j & 1, p.err))) break;
       tc::fence_after_sync();
       const float2 nd = make_float2(-delta, -delta);
 #pragma unroll
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
     if (ok && n > 0) {
-      ok = tc::mbar_wait(bars + C::bDone, 0, p.err);
+      ok = wait(bars + C::bDone, 0, p.err);
       tc::fence_after_sync();
     }
     if (ok) {
@@ -423,13 +423,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
 // dtable[u, hk * G + g]: the tiles' sums in order, one block per entry
 __global__ void __launch_bounds__(128) dbias_kernel(int heads, int group, int buckets, int slots, const float* __restrict__ part,
-                                                    float* __restrict__ out) {
+                                                    void* __restrict__ out, int dtype) {
   __shared__ float scratch[32];
   const int i = blockIdx.x, hk = blockIdx.y, per = buckets * group;
   float x = 0.f;
   for (int t = threadIdx.x; t < slots; t += 128) x += part[((int64_t)hk * slots + t) * per + i];
   x = block_sum(x, scratch);
-  if (threadIdx.x == 0) out[(i / group) * heads + hk * group + i % group] = x;
+  if (threadIdx.x == 0) store_any(out, dtype, (i / group) * heads + hk * group + i % group, x);
 }
 
 // ------------------------------------------------------------------- dk, dv
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int64_t rows = (int64_t)a.tq * G;
       for (int i = 0; i < n && ok; ++i) {
         const int st = i % QS, t0 = (i0 + i) * p.ntok;
-        if (i >= QS && !(ok = tc::mbar_wait(bars + C::bE + st, (i / QS - 1) & 1, p.err))) break;
+        if (i >= QS && !(ok = wait(bars + C::bE + st, (i / QS - 1) & 1, p.err))) break;
         uint8_t* q = base + C::oRing + st * 2 * C::kTile;
         if (lane == 0) {
           tma::expect_tx(bars + C::bF + st, 2u * HV * 128u * (uint32_t)(G * p.ntok));
@@ -559,8 +559,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (lane == 0) {
         if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
         // every copy issued has landed before the CTA may release its shared memory
-        tc::mbar_wait(bars + C::bKV, 0, nullptr);
-        for (int i = max(0, done - QS); i < done; ++i) tc::mbar_wait(bars + C::bF + i % QS, (i / QS) & 1, nullptr);
+        wait(bars + C::bKV, 0, nullptr);
+        for (int i = max(0, done - QS); i < done; ++i) wait(bars + C::bF + i % QS, (i / QS) & 1, nullptr);
       }
     }
     __syncwarp();
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     constexpr uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, 128), idesc_g = tc::idesc_f16(ab_bf16, 1, 128, DT);
     auto stage = [&](int i) { return base + C::oRing + (i % QS) * 2 * C::kTile; };
     auto scores = [&](uint32_t d, const uint8_t* x, const uint8_t* y, uint64_t* bar) {
-      if (lane == 0) {
+      if (elect_one()) {
         tc::fence_after_sync();
         const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), 16), dy = tc::sw128_desc(tc::smem_u32(y), 16);
 #pragma unroll
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       __syncwarp();
     };
     auto issue_s = [&](int i) -> bool {
-      if (!tc::mbar_wait(bars + C::bF + i % QS, (i / QS) & 1, p.err)) return false;
+      if (!wait(bars + C::bF + i % QS, (i / QS) & 1, p.err)) return false;
       const int valid = min(p.ntok, s.nq - (i0 + i) * p.ntok) * G;
       if (valid < 128) {  // rows of no query are an operand of dK and dV
         zero_rows(stage(i), valid, 128, HV);
@@ -601,20 +601,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc::mma_f16_ts(d, left + left_cols(kk), dx + 128 * kk, idesc_g, (more || kk > 0) ? 1u : 0u);
     };
     if (n > 0) {
-      ok = tc::mbar_wait(bars + C::bKV, 0, p.err);
+      ok = wait(bars + C::bKV, 0, p.err);
       for (int i = 0; i < NS && i < n && ok; ++i) ok = issue_s(i);
       if (ok) scores(tmem + C::cDP, base + C::oV, stage(0) + C::kTile, bars + C::bDP);
       for (int i = 0; i < n && ok; ++i) {
-        if (!(ok = tc::mbar_wait(bars + C::bP + i % NS, (i / NS) & 1, p.err))) break;
-        if (lane == 0) {
+        if (!(ok = wait(bars + C::bP + i % NS, (i / NS) & 1, p.err))) break;
+        if (elect_one()) {
           tc::fence_after_sync();
           grads(tmem + C::cDV, tmem + C::cS + (i % NS) * 128, stage(i) + C::kTile, i > 0);
         }
         __syncwarp();
         // S(i + NS) overwrites p(i), which the product before it in order has read
         if (i + NS < n && !(ok = issue_s(i + NS))) break;
-        if (!(ok = tc::mbar_wait(bars + C::bDS, i & 1, p.err))) break;
-        if (lane == 0) {
+        if (!(ok = wait(bars + C::bDS, i & 1, p.err))) break;
+        if (elect_one()) {
           tc::fence_after_sync();
           grads(tmem + C::cDK, tmem + C::cDP, stage(i), i > 0);
           tc::mma_commit(bars + C::bE + i % QS);
@@ -624,9 +624,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (i + 1 < n) scores(tmem + C::cDP, base + C::oV, stage(i + 1) + C::kTile, bars + C::bDP);
       }
       if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
-      if (lane == 0) {
+      if (elect_one()) {
         tc::mma_commit(bars + C::bDrain);
-        tc::mbar_wait(bars + C::bDrain, 0, nullptr);
+        wait(bars + C::bDrain, 0, nullptr);
       }
     }
     __syncwarp();
@@ -643,8 +643,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       // columns from here on see this key; the warp's last key sees the latest start
       const int c0 = a.causal ? (key - shift - t0) * G - w * 64 : 0;
       const bool masked = a.causal && (k0 + ((warp & 3) * 32 + 31) - shift - t0) * G > w * 64;
-      if (!(ok = tc::mbar_wait(bars + C::bF + st, (i / QS) & 1, p.err))) break;  // lse and delta are there
-      if (!(ok = tc::mbar_wait(bars + C::bS + i % NS, (i / NS) & 1, p.err))) break;
+      if (!(ok = wait(bars + C::bF + st, (i / QS) & 1, p.err))) break;  // lse and delta are there
+      if (!(ok = wait(bars + C::bS + i % NS, (i / NS) & 1, p.err))) break;
       tc::fence_after_sync();
       float x[64];
       tc::tmem_ld32_nowait(t_s, x);
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tma::arrive(bars + C::bP + i % NS);
-      if (!(ok = tc::mbar_wait(bars + C::bDP, i & 1, p.err))) break;
+      if (!(ok = wait(bars + C::bDP, i & 1, p.err))) break;
       tc::fence_after_sync();
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
     if (ok && n > 0) {
-      ok = tc::mbar_wait(bars + C::bDone, 0, p.err);
+      ok = wait(bars + C::bDone, 0, p.err);
       tc::fence_after_sync();
     }
     if (ok) {
@@ -787,7 +787,7 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
   if (a->tk > 0) kkv<<<(unsigned)(z.k_slots * a->kv_heads), kBwdThreads, skv, st>>>(mq, mdo, mk, mv, p, bo);
   if (BIAS)
     dbias_kernel<<<dim3(a->buckets * p.group, a->kv_heads), 128, 0, st>>>(a->heads, p.group, a->buckets, (int)z.q_slots, p.part,
-                                                                         a->dbias);
+                                                                         a->dbias, a->bias_dtype);
   return true;
 }
 

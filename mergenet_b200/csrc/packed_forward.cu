@@ -42,7 +42,7 @@ struct Fwd {
   // holds a row of 128 scores: with two slots it takes registers from a third
   // group of four warps, whose other two are idle; the shares stay within what
   // the CTA was launched with.
-  static constexpr bool kExchange = NQ == 2;
+  static constexpr bool kExchange = NQ == 2, kTwice = NQ == 1;
   static constexpr int kThreads = NQ == 1 ? 192 : 384;
   static constexpr int kLaunchRegs = kExchange ? 168 : 0, kMore = 208, kLess = 80;
   static_assert(NQ * kMore + kLess <= 3 * 168, "register exchange");
@@ -50,7 +50,8 @@ struct Fwd {
   static constexpr uint32_t kQ = 0, kRing = NQ * kTile, kBars = kRing + kStages * kTile;
   // barriers: Q landed; ring stages full, empty; per slot S ready, S read, P ready, P V done; drain
   static constexpr int bQ = 0, bFull = 1, bEmpty = bFull + kStages, bS = bEmpty + kStages, bSFree = bS + NQ,
-                       bP = bSFree + NQ, bPV = bP + NQ, bDrain = bPV + NQ, kNumBars = bDrain + 1;
+                       bP = bSFree + NQ, bPV = bP + 2 * NQ,  // bP: keys 0-63, then 64-127
+                       bDrain = bPV + NQ, kNumBars = bDrain + 1;
   static constexpr uint32_t kMisc = kBars + ((kNumBars * 8 + 15) / 16) * 16;  // TMEM base, sequence index
   static constexpr uint32_t kLut = kMisc + 16;
   static constexpr uint32_t bytes(uint32_t lut_floats) { return kLut + lut_floats * 4 + 1024; }
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
   }
   if (warp == 2 && lane == 0) {
     for (int i = 0; i < F::kNumBars; ++i)
-      tc::mbar_init(bars + i, (i >= F::bSFree && i < F::bPV) ? 4 : 1);
+      tc::mbar_init(bars + i, (i >= F::bSFree && i < F::bPV) ? 4 : 1);  // the softmax warps' arrivals
     tc::fence_mbar_init();
   }
   if (warp == 3 && lane == 0) {
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
         for (int j = j0; j < j1 && ok; ++j) {
           for (int kv = 0; kv < 2; ++kv, ++n) {
             const int st = n % ST;
-            if (n >= ST && !(ok = tc::mbar_wait(bars + F::bEmpty + st, ((n / ST) - 1) & 1, p.err))) break;
+            if (n >= ST && !(ok = wait(bars + F::bEmpty + st, ((n / ST) - 1) & 1, p.err))) break;
             tma::expect_tx(bars + F::bFull + st, F::kTile);
             for (int h = 0; h < HV; ++h)
               load_3d(tc::smem_u32(base + F::kRing + st * F::kTile + h * kHalfBytes), kv ? &tm_v : &tm_k, h * 64, hk,
@@ -176,8 +177,8 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
         }
         if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
         // every copy issued has landed before the CTA may release its shared memory
-        tc::mbar_wait(bars + F::bQ, 0, nullptr);
-        for (int m = max(0, n - ST); m < n; ++m) tc::mbar_wait(bars + F::bFull + m % ST, (m / ST) & 1, nullptr);
+        wait(bars + F::bQ, 0, nullptr);
+        for (int m = max(0, n - ST); m < n; ++m) wait(bars + F::bFull + m % ST, (m / ST) & 1, nullptr);
       }
       __syncwarp();
     } else if (warp == 4 * NQ) {
@@ -187,11 +188,11 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
 #pragma unroll
       for (int i = 0; i < NQ; ++i) done[i] = 0;
       auto cols_of = [&](int j) { return min(128, (s.nk - j * 128 + 31) & ~31); };  // keys of block j, in 32s
-      auto full = [&](int n) { return tc::mbar_wait(bars + F::bFull + n % ST, (n / ST) & 1, p.err); };
+      auto full = [&](int n) { return wait(bars + F::bFull + n % ST, (n / ST) & 1, p.err); };
       auto issue_s = [&](int i, int j) -> bool {
         const int n = 2 * (j - j0);
         if (!full(n)) return false;
-        if (lane == 0) {
+        if (elect_one()) {
           tc::fence_after_sync();
           const uint64_t dq = tc::sw128_desc(tc::smem_u32(base + F::kQ + (SPLIT ? 0 : i) * F::kTile), 16);
           const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + F::kRing + (n % ST) * F::kTile), 16);
@@ -209,25 +210,34 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
       };
       auto issue_pv = [&](int i, int j, int c) -> bool {  // c: the slot's block count before this one
         const int n = 2 * (j - j0) + 1;
-        if (!tc::mbar_wait(bars + F::bP + i, c & 1, p.err) || !full(n)) return false;
+        if (!full(n)) return false;
         const int cols = cols_of(j);
         uint8_t* v = base + F::kRing + (n % ST) * F::kTile;
         if (s.nk - j * 128 < cols && (SPLIT || i == 0 || j >= end[0])) zero_rows(v, s.nk - j * 128, cols, HV);
-        if (lane == 0) {
+        const uint64_t dv = tc::sw128_desc(tc::smem_u32(v), kHalfBytes);
+        const uint32_t t_o = tmem + F::cO + i * DT, t_p = tmem + F::cP + i * 128;
+        // the first 64 keys while the softmax works on the others
+        if (!wait(bars + F::bP + 2 * i, c & 1, p.err)) return false;
+        if (elect_one()) {
           tc::fence_after_sync();
-          const uint64_t dv = tc::sw128_desc(tc::smem_u32(v), kHalfBytes);
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            if (kk * 16 < cols)
-              tc::mma_f16_ts(tmem + F::cO + i * DT, tmem + F::cP + i * 128 + kk * 8, dv + 128 * kk, idesc_o,
-                             (c > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk * 16 < cols) tc::mma_f16_ts(t_o, t_p + kk * 8, dv + 128 * kk, idesc_o, (c > 0 || kk > 0) ? 1u : 0u);
+        }
+        __syncwarp();
+        if (!wait(bars + F::bP + 2 * i + 1, c & 1, p.err)) return false;
+        if (elect_one()) {
+          tc::fence_after_sync();
+#pragma unroll
+          for (int kk = 4; kk < 8; ++kk)
+            if (kk * 16 < cols) tc::mma_f16_ts(t_o, t_p + kk * 8, dv + 128 * kk, idesc_o, 1u);
           if (i == last_user(j)) tc::mma_commit(bars + F::bEmpty + n % ST);
         }
         __syncwarp();
         return true;
       };
       if (j1 > j0) {
-        ok = tc::mbar_wait(bars + F::bQ, 0, p.err);
+        ok = wait(bars + F::bQ, 0, p.err);
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
           if (ok && first_of(i) < end_of(i)) ok = issue_s(i, first_of(i));
@@ -239,22 +249,22 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
             const bool more = j + kStep < end_of(i);
             if (DT == 64) {
               // P has its own columns: S(j + 1) as soon as S(j) has been read
-              if (more) ok = tc::mbar_wait(bars + F::bSFree + i, c & 1, p.err) && issue_s(i, j + kStep);
+              if (more) ok = wait(bars + F::bSFree + i, c & 1, p.err) && issue_s(i, j + kStep);
               if (ok) ok = issue_pv(i, j, c);
-              if (ok && lane == 0) tc::mma_commit(bars + F::bPV + i);
+              if (ok && elect_one()) tc::mma_commit(bars + F::bPV + i);
             } else {
               // P overlays S: the MMAs of a CTA run in the order of issue, so
               // S(j + 1) overwrites P(j) only after P V(j) has read it
               ok = issue_pv(i, j, c);
               if (ok && more) ok = issue_s(i, j + kStep);
-              if (ok && !more && lane == 0) tc::mma_commit(bars + F::bPV + i);
+              if (ok && !more && elect_one()) tc::mma_commit(bars + F::bPV + i);
             }
           }
         }
         if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
-        if (lane == 0) {  // every MMA issued has completed before the CTA may release its memory
+        if (elect_one()) {  // every MMA issued has completed before the CTA may release its memory
           tc::mma_commit(bars + F::bDrain);
-          tc::mbar_wait(bars + F::bDrain, 0, nullptr);
+          wait(bars + F::bDrain, 0, nullptr);
         }
       }
       __syncwarp();
@@ -273,7 +283,6 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     const int pos = my + shift;
     const int klim = a.causal && mine ? min(s.nk, pos + 1) : s.nk;  // keys this row sees
     const bool live = __any_sync(MN_FULL_MASK, mine);
-    // rows ascend in position: the warp's first row sees the fewest keys, the last of its own the most
     const int kmin = __reduce_min_sync(MN_FULL_MASK, klim), kmax = __reduce_max_sync(MN_FULL_MASK, mine ? klim : 0);
     const int pmin = __reduce_min_sync(MN_FULL_MASK, mine ? pos : 0x7fffffff);
     const int pmax = __reduce_max_sync(MN_FULL_MASK, mine ? pos : -0x7fffffff);
@@ -281,107 +290,85 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     float m_run = -INFINITY, l_run = 0.f;
     int c = 0;
     for (int j = first_of(i); j < end_of(i) && ok; j += kStep, ++c) {
-      ok = tc::mbar_wait(bars + F::bS + i, c & 1, p.err);
+      ok = wait(bars + F::bS + i, c & 1, p.err);
       if (!ok) break;
       tc::fence_after_sync();
       const int k0 = j * 128;
-      const int nch = (min(128, s.nk - k0) + 31) >> 5;          // chunks of 32 columns that S and P hold
-      const int wch = min(nch, max(0, (kmax - k0 + 31) >> 5));  // of those, seen by some row of the warp
-      float x[128];
-      if (live) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (u < wch) tc::tmem_ld32_nowait(t_s + u * 32, x + u * 32);
-        tc::tmem_ld_wait<128>(x);
+      const int nch = (min(128, s.nk - k0) + 31) >> 5;  // chunks of 32 columns that S and P hold
+      const bool fast = live && nch == 4 && kmin >= k0 + 128;  // the warp's rows see the whole block
+      const int wch = min(nch, max(0, (kmax - k0 + 31) >> 5));  // chunks that some row of the warp sees
+      float f = sl2, add = 0.f;  // x enters the softmax as f x + add
+      bool mixed = false;
+      if (BIAS && live) {
+        const int lo = k0 - pmax, hi = k0 + 127 - pmin;  // distances of the warp's rows
+        if (hi <= -p.reach) {
+          add = row_lut[0];
+        } else if (lo >= p.span - 1 - p.reach) {
+          add = row_lut[p.span - 1];
+        } else {
+          mixed = true;
+          f = 1.f;
+        }
       }
-      if (DT == 64) {
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tma::arrive(bars + F::bSFree + i);
-      }
-      // P V(j - 1) has read P(j - 1); a warp without rows waits too, or its
-      // arrival for P(j) could complete the phase of P(j - 1)
-      if (DT == 64 && c > 0 && !(ok = tc::mbar_wait(bars + F::bPV + i, (c - 1) & 1, p.err))) break;
-      float corr = 1.f;
-      if (live) {
-        const bool masked = kmin < k0 + nch * 32;
-        float add = 0.f;  // bias of a block whose distances all lie beyond the table's reach
-        float f = sl2;
-        if (BIAS) {
-          const int lo = k0 - pmax, hi = k0 + 127 - pmin;  // distances of the warp's rows
-          if (hi <= -p.reach) {
-            add = row_lut[0];
-          } else if (lo >= p.span - 1 - p.reach) {
-            add = row_lut[p.span - 1];
-          } else {
-            const int at = k0 - pos + p.reach;
-#pragma unroll
-            for (int e = 0; e < 128; ++e)
-              if (e / 32 < wch) x[e] = fmaf(x[e], sl2, row_lut[min(max(at + e, 0), p.span - 1)]);
-            f = 1.f;
-          }
-        }
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (k0 + e >= klim) x[e] = -INFINITY;
-        }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (u >= wch) break;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], x[u * 32 + e]);
-        }
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * f + add;
-        const float m_new = fmaxf(m_run, mx);
-        const float m_use = (m_run == -INFINITY || m_new - m_run > kRescaleLog2) ? m_new : m_run;
-        corr = (m_run == -INFINITY || m_use == m_run) ? 1.f : ex2(m_run - m_use);
-        const float nm1 = add - (m_use == -INFINITY ? 0.f : m_use);
-        const float2 nm = make_float2(nm1, nm1), f2 = make_float2(f, f);
-        m_run = m_use;
-        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        if (masked) {  // hidden keys get exactly 0
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (u >= nch) break;
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float2 q = make_float2(0.f, 0.f);
-              if (u < wch) {
-                const float2 y = ffma2(make_float2(x[u * 32 + 2 * e], x[u * 32 + 2 * e + 1]), f2, nm);
-                q = make_float2(ex2(y.x), ex2(y.y));
-                sum2[e & 1] = fadd2(sum2[e & 1], q);
-              }
-              pk[e] = pack2<ET>(q.x, q.y);
-            }
-            tc::tmem_st16_nowait(t_p + u * 16, pk);
-          }
+      // 64 scores of the row, with the bias where it differs by key and the mask
+      auto fetch = [&](float* y, int hf) {
+        if (fast) {
+          tc::tmem_ld32_nowait(t_s + hf * 64, y);
+          tc::tmem_ld32_nowait(t_s + hf * 64 + 32, y + 32);
         } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (u >= nch) break;
-            uint32_t pk[16];
+          for (int e = 0; e < 64; ++e) y[e] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 y = ffma2(make_float2(x[u * 32 + 2 * e], x[u * 32 + 2 * e + 1]), f2, nm);
-              // pairs spread evenly over the row take the polynomial
-              const float2 q = (MN_PK_POLY_PAIRS > 0 && (e * MN_PK_POLY_PAIRS) % 16 >= 16 - MN_PK_POLY_PAIRS)
-                                   ? ex2_poly2(y)
-                                   : make_float2(ex2(y.x), ex2(y.y));
-              sum2[e & 1] = fadd2(sum2[e & 1], q);
-              pk[e] = pack2<ET>(q.x, q.y);
-            }
-            tc::tmem_st16_nowait(t_p + u * 16, pk);
-          }
+          for (int u = 0; u < 2; ++u)
+            if (hf * 2 + u < wch) tc::tmem_ld32_nowait(t_s + hf * 64 + u * 32, y + u * 32);
         }
-        tc::tmem_wait_st();
-        const float2 ss = fadd2(sum2[0], sum2[1]);
-        l_run = l_run * corr + (ss.x + ss.y);
-        // O is at rest: with P apart P V(j - 1) was waited for above, and with
-        // P over S the commit behind S(j) covers P V(j - 1) as well
-        if (c > 0 && __any_sync(MN_FULL_MASK, corr != 1.f)) {
+      };
+      auto shape = [&](float* y, int hf) {
+        if (BIAS && mixed) {
+          const int at = k0 + hf * 64 - pos + p.reach;
+#pragma unroll
+          for (int e = 0; e < 64; ++e) y[e] = fmaf(y[e], sl2, row_lut[min(max(at + e, 0), p.span - 1)]);
+        }
+        if (!fast) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (k0 + hf * 64 + e >= klim) y[e] = -INFINITY;
+        }
+      };
+      float x[F::kTwice ? 64 : 128], mx = -INFINITY;
+      if (live) {
+        fetch(x, 0);
+        tc::tmem_ld_wait<64>(x);
+        if (F::kTwice) {
+          shape(x, 0);
+          mx = max64(x, mx);
+          fetch(x, 1);
+          tc::tmem_ld_wait<64>(x);
+          shape(x, 1);
+          mx = max64(x, mx);
+        } else {
+          fetch(x + 64, 1);
+          shape(x, 0);
+          mx = max64(x, mx);
+          tc::tmem_ld_wait<64>(x + 64);
+          shape(x + 64, 1);
+          mx = max64(x + 64, mx);
+        }
+        mx = mx * f + add;
+      }
+      const float m_new = fmaxf(m_run, mx);
+      const float m_use = (m_run == -INFINITY || m_new - m_run > kRescaleLog2) ? m_new : m_run;
+      const float corr = (m_run == -INFINITY || m_use == m_run) ? 1.f : ex2(m_run - m_use);
+      const float nm1 = add - (m_use == -INFINITY ? 0.f : m_use);
+      const float2 nm = make_float2(nm1, nm1), f2 = make_float2(f, f);
+      // With P apart from S, P V(j - 1) may still read P(j - 1) (a warp without
+      // rows waits too, or its arrival for P(j) could complete the phase of
+      // P(j - 1)); with P over S the commit behind S(j) covers P V(j - 1).
+      if (DT == 64 && c > 0 && !(ok = wait(bars + F::bPV + i, (c - 1) & 1, p.err))) break;
+      if (live) {
+        m_run = m_use;
+        if (c > 0 && __any_sync(MN_FULL_MASK, corr != 1.f)) {  // O is at rest
+          if (DT == 64) tc::fence_after_sync();
           float o[32];
 #pragma unroll
           for (int u = 0; u < DT / 32; ++u) {
@@ -392,13 +379,58 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
           }
         }
       }
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tma::arrive(bars + F::bP + i);
+      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t pk[32];
+        float* y = F::kTwice ? x : x + hf * 64;
+        if (F::kTwice) {
+          if (live) {  // the scores once more: a row of them does not fit the registers of two CTAs
+            fetch(y, hf);
+            tc::tmem_ld_wait<64>(y);
+            shape(y, hf);
+          }
+          if (hf == 1) {
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tma::arrive(bars + F::bSFree + i);
+          }
+        }
+        if (fast) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float2 v = ffma2(make_float2(y[2 * e], y[2 * e + 1]), f2, nm);
+            // pairs spread evenly over the row take the polynomial
+            const float2 q = (MN_PK_POLY_PAIRS > 0 && (e * MN_PK_POLY_PAIRS) % 16 >= 16 - MN_PK_POLY_PAIRS)
+                                 ? ex2_poly2(v)
+                                 : make_float2(ex2(v.x), ex2(v.y));
+            sum2[e & 1] = fadd2(sum2[e & 1], q);
+            pk[e] = pack2<ET>(q.x, q.y);
+          }
+          tc::tmem_st16_nowait(t_p + hf * 32, pk);
+          tc::tmem_st16_nowait(t_p + hf * 32 + 16, pk + 16);
+        } else if (live) {  // hidden keys get exactly 0
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float2 v = ffma2(make_float2(y[2 * e], y[2 * e + 1]), f2, nm);
+            const float2 q = make_float2(ex2(v.x), ex2(v.y));
+            sum2[e & 1] = fadd2(sum2[e & 1], q);
+            pk[e] = pack2<ET>(q.x, q.y);
+          }
+          tc::tmem_st16_nowait(t_p + hf * 32, pk);
+          tc::tmem_st16_nowait(t_p + hf * 32 + 16, pk + 16);
+        }
+        tc::tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tma::arrive(bars + F::bP + 2 * i + hf);
+      }
+      const float2 ss = fadd2(sum2[0], sum2[1]);
+      l_run = l_run * corr + (ss.x + ss.y);
     }
     if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
     if (ok && c > 0) {
-      ok = tc::mbar_wait(bars + F::bPV + i, DT == 64 ? (c - 1) & 1 : 0, p.err);
+      ok = wait(bars + F::bPV + i, DT == 64 ? (c - 1) & 1 : 0, p.err);
       tc::fence_after_sync();
     }
     if (ok && live) {

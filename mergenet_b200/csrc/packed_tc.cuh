@@ -38,6 +38,20 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ float max64(const float* x, float m) {
+  float a[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int e = 0; e < 64; e += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = max3(a[i], x[e + 2 * i], x[e + 2 * i + 1]);
+  return fmaxf(max3(a[0], a[1], a[2]), a[3]);
+}
+
 // 2^y for a pair of y <= 8 on the FMA pipe (the polynomial of
 // csrc/exp2_fit.py, relative error 2.7e-6): y = n + f with n the nearest
 // integer, taken from the low bits of y + 1.5 * 2^23.  y is clamped at -126,
@@ -55,6 +69,40 @@ __device__ __forceinline__ float2 ex2_poly2(float2 y) {
   p = ffma2(p, f, make_float2(9.999992847442627e-01f, 9.999992847442627e-01f));
   const int nx = __float_as_int(t.x) - 0x4B400000, ny = __float_as_int(t.y) - 0x4B400000;
   return make_float2(__int_as_float(__float_as_int(p.x) + (nx << 23)), __int_as_float(__float_as_int(p.y) + (ny << 23)));
+}
+
+// Wait for the phase with the given parity, bounded in time like
+// tc::mbar_wait, which looks at the clock and at *err (a trip to the L2)
+// before its second try; a hand-off between the warps of a tile is shorter
+// than that trip, so here the first 64 tries go without.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const int* err) {
+  const uint32_t addr = tc::smem_u32(bar);
+  for (int i = 0; i < 64; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return tc::mbar_wait(bar, parity, err);
+}
+
+// One lane of a converged warp, the same each time.  The compiler knows that a
+// single thread passes, so the tensor-core instructions behind it are issued
+// as they stand; behind `lane == 0` each took about 140 cycles (a product of
+// 128 x 128 x 128 was issued in 1,150 cycles and executes in about 500).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0;
 }
 
 // Register exchange between the warp groups of a CTA (a whole group executes

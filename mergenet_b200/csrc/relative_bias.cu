@@ -2,11 +2,20 @@
 // (mn_relative_bias), and the table's gradient.
 //
 // bias[h, i, j] = table[bucket(j - i - start), h] depends on h and on the
-// diagonal j - i alone, so both directions work with the queries + keys - 1
-// diagonals: the forward writes each value from one lookup, the gradient adds
-// up each diagonal over a chunk of rows (one thread per diagonal, its rows in
-// order) and then the diagonals of each bucket, all in a fixed order.
+// diagonal j - i alone, and both directions are bound by the one pass over
+// [heads, queries, keys].
+//
+// Forward: a block writes kRows x kCols of one head.  Its diagonals' values
+// (kRows + kCols - 1 of them) are looked up once into shared memory, in as
+// many copies as a 16-byte store has elements, each shifted by one more, so
+// that any run of a row is one aligned 16-byte read and one 16-byte store.
+//
+// Gradient: a block adds up 256 diagonals over kChunk rows, a thread per
+// diagonal (consecutive lanes read consecutive elements of a row), then the
+// diagonals of each bucket, which are contiguous; a second kernel adds the
+// blocks' sums.  Every sum has a fixed order.
 #include <algorithm>
+#include <cstdlib>
 
 #include "packed.cuh"
 
@@ -14,53 +23,104 @@ namespace mn {
 namespace rb {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 64;  // rows of a chunk whose diagonals one block adds up
+constexpr int kRows = 32, kCols = 1024;  // forward: rows and columns of a block
+constexpr int kChunk = 64;               // gradient: rows of a block
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) forward_kernel(int heads, int queries, int keys, int start, Borders bo,
-                                                           const T* __restrict__ table, T* __restrict__ bias) {
-  const int64_t n = (int64_t)heads * queries * keys;
-  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < n; e += (int64_t)gridDim.x * kThreads) {
-    const int j = (int)(e % keys);
-    const int64_t r = e / keys;
-    const int i = (int)(r % queries), h = (int)(r / queries);
-    bias[e] = table[bucket_of(bo, j - i - start) * heads + h];
+template <typename T>  // T: the element's bits
+__global__ void __launch_bounds__(kThreads) forward_kernel(int heads, int queries, int keys, int start,
+                                                           const __grid_constant__ Borders bo, const T* __restrict__ table,
+                                                           T* __restrict__ bias) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int kLen = kRows + kCols + V;
+  __shared__ __align__(16) T copy[V][kLen];  // copy[c][x] = value of diagonal x + c
+  const int j0 = blockIdx.x * kCols, i0 = blockIdx.y * kRows, h = blockIdx.z;
+  const int cols = min(kCols, keys - j0), rows = min(kRows, queries - i0);
+  // diagonal x of the block is j - i with i = i0 + rows - 1 - x at j = j0
+  for (int x = threadIdx.x; x < rows + cols - 1; x += kThreads) {
+    const T v = table[bucket_of(bo, j0 - (i0 + rows - 1) + x - start) * heads + h];
+#pragma unroll
+    for (int c = 0; c < V; ++c)
+      if (x >= c) copy[c][x - c] = v;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int r = threadIdx.x >> 5; r < rows; r += kThreads / 32) {
+    const int64_t first = ((int64_t)h * queries + i0 + r) * keys + j0;  // of the row's run
+    const int lead = (int)((V - first % V) % V);                       // elements before the first 16-byte boundary
+    const int x0 = rows - 1 - r;                                       // diagonal of the run's first element
+    T* row = bias + first;
+    for (int e = lane; e < min(lead, cols); e += 32) row[e] = copy[0][x0 + e];
+    const int n = cols > lead ? (cols - lead) / V : 0;
+    for (int k = lane; k < n; k += 32) {
+      const int x = x0 + lead + k * V;
+      *reinterpret_cast<uint4*>(row + lead + k * V) = *reinterpret_cast<const uint4*>(&copy[x % V][x / V * V]);
+    }
+    for (int e = lead + n * V + lane; e < cols; e += 32) row[e] = copy[0][x0 + e];
   }
 }
 
-// part[chunk, h, diag]: the sum of dbias[h, i, i + diag - (queries - 1)] over
-// the rows i of the chunk
+// part[(h, chunk, block of diagonals)][u]: the sum of dbias over the rows
+// [i0, i0 + kChunk) of the block's diagonals of bucket u
 template <typename T>
-__global__ void __launch_bounds__(kThreads) diagonal_kernel(int heads, int queries, int keys, const T* __restrict__ dbias,
+__global__ void __launch_bounds__(kThreads) diagonal_kernel(int queries, int keys, int start, int buckets,
+                                                            const __grid_constant__ Borders bo, const T* __restrict__ dbias,
                                                             float* __restrict__ part) {
-  const int diags = queries + keys - 1;
-  const int g = blockIdx.x * kThreads + threadIdx.x, h = blockIdx.y, i0 = blockIdx.z * kRows;
-  if (g >= diags) return;
+  __shared__ float sum[kThreads];
+  const int i0 = blockIdx.y * kChunk, h = blockIdx.z, rows = min(kChunk, queries - i0);
+  // the thread's diagonal: j = c + (i - i0)
+  const int c0 = blockIdx.x * kThreads - (rows - 1), c = c0 + threadIdx.x;
+  const int lo = max(0, -c), hi = min(rows, keys - c);
+  const T* at = dbias + ((int64_t)h * queries + i0) * keys + c;
   float x = 0.f;
-  for (int i = i0; i < min(queries, i0 + kRows); ++i) {
-    const int j = i + g - (queries - 1);
-    if (j >= 0 && j < keys) x += to_f32(dbias[((int64_t)h * queries + i) * keys + j]);
+  if (hi - lo == kChunk) {
+#pragma unroll 16
+    for (int i = 0; i < kChunk; ++i) x += to_f32(at[(int64_t)i * (keys + 1)]);
+  } else {
+#pragma unroll 8
+    for (int i = lo; i < hi; ++i) x += to_f32(at[(int64_t)i * (keys + 1)]);
   }
-  part[((int64_t)blockIdx.z * heads + h) * diags + g] = x;
+  sum[threadIdx.x] = x;
+  __syncthreads();
+  // relative positions of the block: first + t; bucket u of one side is the
+  // run of distances [at[u - 1], at[u])
+  const int first = c0 - i0 - start, lane = threadIdx.x & 31;
+  float* out = part + ((int64_t)(h * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * buckets;
+  for (int u = threadIdx.x >> 5; u < buckets; u += kThreads / 32) {
+    const bool ahead = u >= bo.side;
+    const int k = ahead ? u - bo.side : u;
+    const int near = k == 0 ? 0 : bo.at[k - 1], far = k < bo.n ? bo.at[k] - 1 : 0x3fffffff;
+    int a, b;  // the bucket's relative positions, both ends included
+    if (ahead) {
+      a = max(near, 1), b = far;
+    } else {
+      a = -far, b = -near;
+      if (k == 0 && !bo.two_sided) b = 0x7fffffff;  // one-sided: all that is ahead
+    }
+    const int t0 = (int)max((int64_t)a - first, (int64_t)0), t1 = (int)min((int64_t)b - first, (int64_t)kThreads - 1);
+    float s = 0.f;
+    for (int t = t0 + lane; t <= t1; t += 32) s += sum[t];
+    s = warp_sum(s);
+    if (lane == 0) out[u] = s;
+  }
 }
 
-__global__ void __launch_bounds__(kThreads) bucket_kernel(int heads, int queries, int keys, int start, Borders bo, int chunks,
-                                                          const float* __restrict__ part, float* __restrict__ dtable) {
+__global__ void __launch_bounds__(128) bucket_kernel(int heads, int buckets, int blocks, const float* __restrict__ part,
+                                                     void* __restrict__ dtable, int dtype) {
   __shared__ float scratch[32];
-  const int u = blockIdx.x, h = blockIdx.y, diags = queries + keys - 1;
+  const int u = blockIdx.x, h = blockIdx.y;
   float x = 0.f;
-  for (int g = threadIdx.x; g < diags; g += kThreads)
-    if (bucket_of(bo, g - (queries - 1) - start) == u)
-      for (int c = 0; c < chunks; ++c) x += part[((int64_t)c * heads + h) * diags + g];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < blocks; i += 128) x += part[((int64_t)h * blocks + i) * buckets + u];
   x = block_sum(x, scratch);
-  if (threadIdx.x == 0) dtable[u * heads + h] = x;
+  if (threadIdx.x == 0) store_any(dtable, dtype, u * heads + h, x);
 }
 
-static int chunks_of(int queries) { return (queries + kRows - 1) / kRows; }
+static int chunks_of(int queries) { return (queries + kChunk - 1) / kChunk; }
+static int diag_blocks(int queries, int keys) { return (keys + std::min(queries, kChunk) - 1 + kThreads - 1) / kThreads; }
 
 static bool sizes_ok(int heads, int queries, int keys, int start) {
-  return heads > 0 && queries >= 0 && keys >= 0 && queries < (1 << 30) && keys < (1 << 30) && start < (1 << 30) &&
-         start > -(1 << 30);
+  // every position and distance fits 32 bits
+  return heads > 0 && queries >= 0 && keys >= 0 && (int64_t)queries + keys + std::abs((int64_t)start) < (1 << 30);
 }
 
 }  // namespace rb
@@ -75,14 +135,15 @@ extern "C" int mn_relative_bias(int heads, int queries, int keys, int query_star
   if (!rb::sizes_ok(heads, queries, keys, query_start) || dtype < 0 || dtype > 2) return MN_ERR_ARG;
   if (!make_borders(&bo, buckets, two_sided, num_borders, borders)) return MN_ERR_ARG;
   if (queries == 0 || keys == 0) return MN_OK;
-  if (!table || !bias) return MN_ERR_ARG;
+  if (!table || !bias || reinterpret_cast<uintptr_t>(bias) % 16) return MN_ERR_ARG;
   cudaGetLastError();
-  const int64_t n = (int64_t)heads * queries * keys;
-  const unsigned grid = (unsigned)std::min<int64_t>((n + rb::kThreads - 1) / rb::kThreads, 148 * 32);
+  const dim3 grid((keys + rb::kCols - 1) / rb::kCols, (queries + rb::kRows - 1) / rb::kRows, heads);
+  if (grid.y > 65535 || grid.z > 65535) return MN_ERR_UNSUPPORTED;
   auto st = static_cast<cudaStream_t>(stream);
   if (dtype == MN_F32)
-    rb::forward_kernel<float><<<grid, rb::kThreads, 0, st>>>(heads, queries, keys, query_start, bo,
-                                                            static_cast<const float*>(table), static_cast<float*>(bias));
+    rb::forward_kernel<uint32_t><<<grid, rb::kThreads, 0, st>>>(heads, queries, keys, query_start, bo,
+                                                               static_cast<const uint32_t*>(table),
+                                                               static_cast<uint32_t*>(bias));
   else
     rb::forward_kernel<uint16_t><<<grid, rb::kThreads, 0, st>>>(heads, queries, keys, query_start, bo,
                                                                static_cast<const uint16_t*>(table),
@@ -91,14 +152,13 @@ extern "C" int mn_relative_bias(int heads, int queries, int keys, int query_star
 }
 
 extern "C" size_t mn_relative_bias_backward_workspace_bytes(int heads, int queries, int keys, int buckets) {
-  (void)buckets;
-  if (heads < 1 || queries < 1 || keys < 1) return 0;
-  return (size_t)rb::chunks_of(queries) * heads * ((size_t)queries + keys - 1) * 4;
+  if (heads < 1 || queries < 1 || keys < 1 || buckets < 1) return 0;
+  return (size_t)rb::chunks_of(queries) * rb::diag_blocks(queries, keys) * heads * buckets * 4;
 }
 
 extern "C" int mn_relative_bias_backward(int heads, int queries, int keys, int query_start, int buckets, int two_sided,
                                          int num_borders, const int32_t* borders, int dtype, const void* dbias,
-                                         float* dtable, void* workspace, size_t workspace_bytes, void* stream) {
+                                         void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
   Borders bo;
   if (!rb::sizes_ok(heads, queries, keys, query_start) || dtype < 0 || dtype > 2 || !dtable) return MN_ERR_ARG;
   if (!make_borders(&bo, buckets, two_sided, num_borders, borders)) return MN_ERR_ARG;
@@ -109,16 +169,17 @@ extern "C" int mn_relative_bias_backward(int heads, int queries, int keys, int q
     return MN_ERR_WORKSPACE;
   cudaGetLastError();
   float* part = static_cast<float*>(workspace);
-  const int chunks = rb::chunks_of(queries), diags = queries + keys - 1;
-  const dim3 grid((diags + rb::kThreads - 1) / rb::kThreads, heads, chunks);
+  const dim3 grid(rb::diag_blocks(queries, keys), rb::chunks_of(queries), heads);
   auto st = static_cast<cudaStream_t>(stream);
   if (dtype == MN_F32)
-    rb::diagonal_kernel<float><<<grid, rb::kThreads, 0, st>>>(heads, queries, keys, static_cast<const float*>(dbias), part);
+    rb::diagonal_kernel<float><<<grid, rb::kThreads, 0, st>>>(queries, keys, query_start, buckets, bo,
+                                                             static_cast<const float*>(dbias), part);
   else if (dtype == MN_F16)
-    rb::diagonal_kernel<__half><<<grid, rb::kThreads, 0, st>>>(heads, queries, keys, static_cast<const __half*>(dbias), part);
+    rb::diagonal_kernel<__half><<<grid, rb::kThreads, 0, st>>>(queries, keys, query_start, buckets, bo,
+                                                              static_cast<const __half*>(dbias), part);
   else
-    rb::diagonal_kernel<__nv_bfloat16><<<grid, rb::kThreads, 0, st>>>(heads, queries, keys,
+    rb::diagonal_kernel<__nv_bfloat16><<<grid, rb::kThreads, 0, st>>>(queries, keys, query_start, buckets, bo,
                                                                      static_cast<const __nv_bfloat16*>(dbias), part);
-  rb::bucket_kernel<<<dim3(buckets, heads), rb::kThreads, 0, st>>>(heads, queries, keys, query_start, bo, chunks, part, dtable);
+  rb::bucket_kernel<<<dim3(buckets, heads), 128, 0, st>>>(heads, buckets, (int)(grid.x * grid.y), part, dtable, dtype);
   return cudaGetLastError() == cudaSuccess ? MN_OK : MN_ERR_LAUNCH;
 }

@@ -99,60 +99,105 @@ def _check_table(table, buckets, heads=None):
     L.dtype_code(table.dtype)
 
 
-def _rows_ready(t):
-    """[rows, heads, channels] with unit channel stride and rows and heads on
-    16-byte boundaries (what the copies of a tile need); a broadcast
-    dimension (stride 0) is laid out first."""
-    st, sh, sd = t.stride()
-    return (sd == 1 and st % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0 and (st > 0 or t.shape[0] == 1)
-            and (sh > 0 or t.shape[1] == 1))
-
-
 def _ready(t):
-    return t if _rows_ready(t) else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+    """[rows, heads, channels] with unit channel stride and rows and heads on
+    16-byte boundaries (what the copies of a tile need), laid out anew where
+    it is not so, a broadcast dimension (stride 0) included."""
+    st, sh, sd = t.stride()
+    if sd == 1 and not (st % 8 or sh % 8 or t.data_ptr() % 16) and (st > 0 or t.shape[0] < 2) and (sh > 0 or t.shape[1] < 2):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _err_word(dev):
-    """The device's status word; none while a graph is being captured that
-    would have to create it."""
-    if (dev.type, dev.index) not in _STATUS and torch.cuda.is_current_stream_capturing():
-        return None
-    return _status(dev)
+    """The address of the device's status word; none while a graph is being
+    captured that would have to create it."""
+    st = _STATUS.get((dev.type, dev.index))
+    if st is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        st = _status(dev)
+    return st.data_ptr()
+
+
+class _on:
+    """Makes a device other than the current one current for the launches."""
+    __slots__ = ("index", "before")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        torch.cuda.set_device(self.before)
+
+
+def _on_device(dev, fn, *args):
+    """fn(*args, stream) with ``dev`` current; stream is its current one."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with _on(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _require(dev, *tensors):
+    """All CUDA tensors of one device (the usual case without a loop's cost)."""
+    if dev.type == "cuda":
+        for t in tensors:
+            if t is not None and t.device != dev:
+                break
+        else:
+            return
+    L.require_cuda(*tensors)
+    raise ValueError("all tensors must be on the same CUDA device")
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _args(q, k, v, cu_q, cu_k, len_k, causal, scale, table, buckets, out, lse, dout=None, dq=None, dk=None, dv=None, dbias=None):
-    """mn_packed_args in field order."""
-    st = [*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *(dout.stride()[:2] if dout is not None else (0, 0))]
-    pt = [0 if t is None else t.data_ptr() for t in (q, k, v, cu_q, cu_k, len_k, table)]
-    po = [0 if t is None else t.data_ptr() for t in (out, lse, dout, dq, dk, dv, dbias)]
+    """The bytes of mn_packed_args."""
+    tq, h, d = q.shape
+    tk, hk, _ = k.shape
     if table is None:
         bias = (0, 0, 0, 0)
         borders = 0
     else:
         bias = (L.dtype_code(table.dtype), buckets.num_buckets, int(buckets.two_sided), len(buckets.borders))
         borders = ctypes.addressof(buckets._c_borders)
-    return L.PackedArgs(*pt, borders, *po, *st, cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
-                        L.dtype_code(q.dtype), int(causal), *bias, scale, 0)
+    qs, ks, vs, ds = q.stride(), k.stride(), v.stride(), (0, 0) if dout is None else dout.stride()
+    return L.PACKED_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _at(len_k), _at(table),
+                              borders, out.data_ptr(), _at(lse), _at(dout), _at(dq), _at(dk), _at(dv), _at(dbias),
+                              qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], ds[0], ds[1],
+                              cu_q.shape[0] - 1, tq, tk, h, hk, d, L.dtype_code(q.dtype), causal, *bias, scale, 0)
 
 
-def _workspace(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _launch(fn, size, name, args, dev, stream):
+    """Sizes the workspace, allocates it on the current stream and launches."""
+    nbytes = size(args)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    rc = fn(args, None if ws is None else ws.data_ptr(), nbytes, _err_word(dev), stream)
+    if rc:
+        L.check(rc, name)
 
 
 def _forward(q, k, v, cu_q, cu_k, len_k, causal, scale, table, buckets, want_lse):
     dev = q.device
     q, k, v = _ready(q), _ready(k), _ready(v)
-    out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    lse = torch.empty(k.shape[1], q.shape[0], q.shape[1] // k.shape[1], device=dev, dtype=torch.float32) if want_lse else None
-    table = None if table is None else table.contiguous()
-    if out.numel():
-        with torch.cuda.device(dev):
-            lib = L.lib()
-            a = _args(q, k, v, cu_q, cu_k, len_k, causal, scale, table, buckets, out, lse)
-            nbytes = lib.mn_packed_attention_workspace_bytes(ctypes.byref(a))
-            ws = _workspace(nbytes, dev)
-            L.check(lib.mn_packed_attention(ctypes.byref(a), L.ptr(ws), nbytes, L.ptr(_err_word(dev)), L.stream_of(q)),
-                    "mn_packed_attention")
+    tq, h, d = q.shape
+    out = torch.empty((tq, h, d), device=dev, dtype=q.dtype)
+    hk = k.shape[1]
+    lse = torch.empty((hk, tq, h // hk), device=dev, dtype=torch.float32) if want_lse else None
+    if tq:
+        table = None if table is None else table.contiguous()
+        lib = L.lib()
+        _on_device(dev, _launch, lib.mn_packed_attention, lib.mn_packed_attention_workspace_bytes, "mn_packed_attention",
+                   _args(q, k, v, cu_q, cu_k, len_k, causal, scale, table, buckets, out, lse), dev)
     return out, lse
 
 
@@ -165,40 +210,45 @@ class _PackedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, cu_q, cu_k, len_k, out, lse = ctx.saved_tensors
-        causal, scale, buckets = ctx.call
-        dev = q.device
-        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
-        dv = torch.empty(v.shape, device=dev, dtype=v.dtype)
-        dbias = None if table is None else torch.empty(table.shape, device=dev, dtype=torch.float32)
-        if q.numel() == 0:
-            for t in (dk, dv, dbias):
-                if t is not None:
-                    t.zero_()
-        else:
-            tab = None if table is None else table.contiguous()
-            qr, kr, vr, do = _ready(q), _ready(k), _ready(v), _ready(dout)
-            with torch.cuda.device(dev):
-                lib = L.lib()
-                a = _args(qr, kr, vr, cu_q, cu_k, len_k, causal, scale, tab, buckets, out, lse, do, dq, dk, dv, dbias)
-                nbytes = lib.mn_packed_attention_backward_workspace_bytes(ctypes.byref(a))
-                ws = _workspace(nbytes, dev)
-                L.check(lib.mn_packed_attention_backward(ctypes.byref(a), L.ptr(ws), nbytes, L.ptr(_err_word(dev)),
-                                                         L.stream_of(qr)), "mn_packed_attention_backward")
-        return dq, dk, dv, None if table is None else dbias.to(table.dtype), None, None, None, None, None, None
+        return _attention_grads_once(ctx, dout) if torch.is_grad_enabled() else _attention_grads(ctx, dout)
 
 
-def _check_offsets(name, t, ndim_len=None):
-    if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
+def _attention_grads(ctx, dout):
+    q, k, v, table, cu_q, cu_k, len_k, out, lse = ctx.saved_tensors
+    causal, scale, buckets = ctx.call
+    dev = q.device
+    dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
+    dv = torch.empty(v.shape, device=dev, dtype=v.dtype)
+    dbias = None if table is None else torch.empty(table.shape, device=dev, dtype=table.dtype)
+    if q.numel() == 0:
+        for t in (dk, dv, dbias):
+            if t is not None:
+                t.zero_()
+    else:
+        tab = None if table is None else table.contiguous()
+        q, k, v, dout = _ready(q), _ready(k), _ready(v), _ready(dout)
+        lib = L.lib()
+        _on_device(dev, _launch, lib.mn_packed_attention_backward, lib.mn_packed_attention_backward_workspace_bytes,
+                   "mn_packed_attention_backward",
+                   _args(q, k, v, cu_q, cu_k, len_k, causal, scale, tab, buckets, out, lse, dout, dq, dk, dv, dbias), dev)
+    return dq, dk, dv, dbias, None, None, None, None, None, None
+
+
+_attention_grads_once = once_differentiable(_attention_grads)  # where a graph of the gradients is asked for
+
+
+def _check_offsets(name, t, entries):
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D int32 tensor, got {t.dtype} of shape {tuple(t.shape)}")
-    if ndim_len is None:
-        if t.numel() < 2:
+    n = t.shape[0]
+    if entries is None:
+        if n < 2:
             raise ValueError(f"{name} holds the sequences' ends behind a leading 0: at least two entries")
-    elif t.numel() != ndim_len:
-        raise ValueError(f"{name} must have {ndim_len} entries, got {t.numel()}")
+    elif n != entries:
+        raise ValueError(f"{name} must have {entries} entries, got {n}")
+    return n
 
 
 def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None, causal=False, scale=None, bias_table=None,
@@ -224,7 +274,7 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
 
     ``bias_table`` [num_buckets, H] (fp32, fp16 or bf16) with ``buckets``
     (RelativeBuckets) adds table[bucket(key position - query position), head].
-    Its gradient is summed in fp32 and returned in the table's type.
+    Its gradient is summed in fp32 and rounded once to the table's type.
 
     Scores, softmax statistics and sums are fp32; probabilities and their
     gradients are rounded to the input type before each tensor-core product.
@@ -236,28 +286,32 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
     Offsets are read on the device and not checked on the host: those that
     decrease or pass the tensors' ends leave the results undefined, touch no
     other memory, and set MN_STATUS_BAD_LENGTHS in attention_status()."""
-    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"q, k and v must be [rows, heads, head_dim], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape != v.shape or q.shape[2] != k.shape[2]:
+    tq, h, d = q.shape
+    tk, hk, dk = k.shape
+    if (tk, hk, dk) != tuple(v.shape) or d != dk:
         raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if not (q.dtype == k.dtype == v.dtype):
+    dtype = q.dtype
+    if not (dtype == k.dtype == v.dtype):
         raise ValueError("q/k/v must share a dtype")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"q/k/v must be float16 or bfloat16, got {q.dtype}")
-    h, hk, d = q.shape[1], k.shape[1], q.shape[2]
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise ValueError(f"q/k/v must be float16 or bfloat16, got {dtype}")
     if d < 8 or d > MAX_HEAD_DIM or d % 8:
         raise ValueError(f"head_dim {d} is not supported: a multiple of 8 up to {MAX_HEAD_DIM}")
     if not 1 <= hk <= 65535 or h < 1 or h % hk or h // hk > MAX_GROUP:
         raise ValueError(f"{h} query heads must be a multiple of the {hk} key heads, at most {MAX_GROUP} to one")
+    group = h // hk
+    entries = _check_offsets("cu_seqlens_q", cu_seqlens_q, None)
     if cu_seqlens_k is None:
-        if q.shape[0] != k.shape[0]:
+        if tq != tk:
             raise ValueError("without cu_seqlens_k the keys must have the queries' rows")
         cu_seqlens_k = cu_seqlens_q
-    _check_offsets("cu_seqlens_q", cu_seqlens_q)
-    _check_offsets("cu_seqlens_k", cu_seqlens_k, cu_seqlens_q.numel())
+    else:
+        _check_offsets("cu_seqlens_k", cu_seqlens_k, entries)
     if lengths_k is not None:
-        _check_offsets("lengths_k", lengths_k, cu_seqlens_q.numel() - 1)
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+        _check_offsets("lengths_k", lengths_k, entries - 1)
+    scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if (bias_table is None) != (buckets is None):
@@ -265,54 +319,71 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
     if bias_table is not None:
         _check_table(bias_table, buckets, h)
         sides = 2 if buckets.two_sided else 1
-        if buckets.num_buckets > MAX_BUCKETS or buckets.num_buckets * (h // hk) > MAX_BIAS_ENTRIES or (sides * buckets.borders[-1] + 1) * (h // hk) > MAX_BIAS_VALUES:
-            raise ValueError(f"{buckets} with {h // hk} grouped heads does not fit: at most {MAX_BUCKETS} buckets, "
+        if (buckets.num_buckets > MAX_BUCKETS or buckets.num_buckets * group > MAX_BIAS_ENTRIES
+                or (sides * buckets.borders[-1] + 1) * group > MAX_BIAS_VALUES):
+            raise ValueError(f"{buckets} with {group} grouped heads does not fit: at most {MAX_BUCKETS} buckets, "
                              f"{MAX_BIAS_ENTRIES} buckets x grouped heads and {MAX_BIAS_VALUES} distances x grouped heads")
-    if max(q.shape[0], k.shape[0]) * max(h // hk, 1) >= 1 << 30:
+    if max(tq, tk) * group >= 1 << 30:
         raise ValueError("at most 2^30 rows x grouped heads")
-    L.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, bias_table)
+    _require(q.device, q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, bias_table)
+    causal = bool(causal)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (bias_table is not None and bias_table.requires_grad)):
-        return _PackedAttention.apply(q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, lengths_k, bool(causal), scale, buckets)
-    return _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, bool(causal), scale, bias_table, buckets, False)[0]
+        return _PackedAttention.apply(q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, lengths_k, causal, scale, buckets)
+    return _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, causal, scale, bias_table, buckets, False)[0]
+
+
+def _bias_launch(table, out, queries, keys, start, buckets, stream):
+    rc = L.lib().mn_relative_bias(table.shape[1], queries, keys, start, buckets.num_buckets, buckets.two_sided, len(buckets.borders),
+                                  ctypes.addressof(buckets._c_borders), L.dtype_code(table.dtype), table.data_ptr(), out.data_ptr(),
+                                  stream)
+    if rc:
+        L.check(rc, "mn_relative_bias")
 
 
 def _bias_forward(table, queries, keys, start, buckets):
-    out = torch.empty(table.shape[1], queries, keys, device=table.device, dtype=table.dtype)
-    if out.numel():
-        t = table.contiguous()
-        with torch.cuda.device(table.device):
-            L.check(L.lib().mn_relative_bias(table.shape[1], queries, keys, start, buckets.num_buckets, int(buckets.two_sided),
-                                             len(buckets.borders), ctypes.addressof(buckets._c_borders), L.dtype_code(t.dtype),
-                                             L.ptr(t), L.ptr(out), L.stream_of(t)), "mn_relative_bias")
+    dev = table.device
+    out = torch.empty((table.shape[1], queries, keys), device=dev, dtype=table.dtype)
+    if queries and keys:
+        _on_device(dev, _bias_launch, table.contiguous(), out, queries, keys, start, buckets)
     return out
+
+
+def _bias_grad_launch(dbias, grad, start, buckets, stream):
+    lib = L.lib()
+    heads, queries, keys = dbias.shape
+    nb = buckets.num_buckets
+    nbytes = lib.mn_relative_bias_backward_workspace_bytes(heads, queries, keys, nb)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dbias.device)
+    rc = lib.mn_relative_bias_backward(heads, queries, keys, start, nb, buckets.two_sided, len(buckets.borders),
+                                       ctypes.addressof(buckets._c_borders), L.dtype_code(dbias.dtype), dbias.data_ptr(),
+                                       grad.data_ptr(), ws.data_ptr(), nbytes, stream)
+    if rc:
+        L.check(rc, "mn_relative_bias_backward")
+
+
+def _bias_grads(ctx, dbias):
+    start, buckets = ctx.call
+    grad = torch.empty((buckets.num_buckets, dbias.shape[0]), device=dbias.device, dtype=dbias.dtype)
+    if dbias.numel():
+        _on_device(dbias.device, _bias_grad_launch, dbias.contiguous(), grad, start, buckets)
+    else:
+        grad.zero_()
+    return grad, None, None, None, None
+
+
+_bias_grads_once = once_differentiable(_bias_grads)
 
 
 class _RelativeBias(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, queries, keys, start, buckets):
-        ctx.call = (queries, keys, start, buckets, table.shape[1], table.dtype)
+        ctx.call = (start, buckets)
         return _bias_forward(table, queries, keys, start, buckets)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dbias):
-        queries, keys, start, buckets, heads, dtype = ctx.call
-        dev = dbias.device
-        d = dbias.contiguous()
-        grad = torch.empty(buckets.num_buckets, heads, device=dev, dtype=torch.float32)
-        if d.numel() == 0:
-            grad.zero_()
-        else:
-            with torch.cuda.device(dev):
-                lib = L.lib()
-                nbytes = lib.mn_relative_bias_backward_workspace_bytes(heads, queries, keys, buckets.num_buckets)
-                ws = _workspace(nbytes, dev)
-                L.check(lib.mn_relative_bias_backward(heads, queries, keys, start, buckets.num_buckets, int(buckets.two_sided),
-                                                      len(buckets.borders), ctypes.addressof(buckets._c_borders),
-                                                      L.dtype_code(d.dtype), L.ptr(d), L.ptr(grad), L.ptr(ws), nbytes,
-                                                      L.stream_of(d)), "mn_relative_bias_backward")
-        return grad.to(dtype), None, None, None, None
+        return _bias_grads_once(ctx, dbias) if torch.is_grad_enabled() else _bias_grads(ctx, dbias)
 
 
 def relative_position_bias(table, queries, keys, buckets, query_start=None):
@@ -326,12 +397,15 @@ def relative_position_bias(table, queries, keys, buckets, query_start=None):
     _check_table(table, buckets)
     if table.shape[1] < 1:
         raise ValueError("the bias table needs a head")
+    queries, keys = operator.index(queries), operator.index(keys)
     if queries < 0 or keys < 0:
         raise ValueError(f"queries and keys must not be negative, got {queries} and {keys}")
     start = keys - queries if query_start is None else operator.index(query_start)
-    if max(queries, keys, abs(start)) >= 1 << 30:
-        raise ValueError("positions must stay below 2^30")
+    if queries + keys + abs(start) >= 1 << 30:
+        raise ValueError("positions and distances must stay below 2^30")
+    if table.shape[1] > 65535 or queries > 32 * 65535:
+        raise ValueError("at most 65535 heads and 2097120 queries")
     L.require_cuda(table)
     if torch.is_grad_enabled() and table.requires_grad:
-        return _RelativeBias.apply(table, int(queries), int(keys), start, buckets)
-    return _bias_forward(table, int(queries), int(keys), start, buckets)
+        return _RelativeBias.apply(table, queries, keys, start, buckets)
+    return _bias_forward(table, queries, keys, start, buckets)
