@@ -775,8 +775,8 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
   CUtensorMap mq, mdo, mk, mv;
   if (!bind_context() || !map_q(&mq, bf16, a->q, a->q_st, a->q_sh, a->tq, a->heads, a->kv_heads, a->head_dim, z.ntok) ||
       !map_q(&mdo, bf16, a->dout, a->do_st, a->do_sh, a->tq, a->heads, a->kv_heads, a->head_dim, z.ntok) ||
-      !map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim) ||
-      !map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim))
+      !map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, 128) ||
+      !map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, 128))
     return false;
   if (z.q_slots * a->kv_heads > 0x7fffffff || z.k_slots * a->kv_heads > 0x7fffffff) return false;
   auto kq = dq_kernel<ET, DT, BIAS>;

@@ -4,22 +4,26 @@
 //
 // A tile is 128 rows of (token, head of the group), token-major: the heads
 // that share a key head sit in one tile, so grouped heads read their keys and
-// values once and one token's form is a tile of its heads.  Per block of 128
+// values once and one token's form is a tile of its heads.  Per block of 64
 // keys:
 //
 //   * a load warp brings K and V (a ring of stages) by TMA;
-//   * an MMA warp issues S = Q K^T into tensor memory and, once the softmax
-//     warps have written the probabilities there as 16-bit values, O += P V
-//     with P read from tensor memory;
+//   * an MMA warp issues S = Q K^T into one of the slot's S buffers in tensor
+//     memory and, once the softmax warps have written the probabilities over
+//     it as 16-bit values, O += P V with P read from tensor memory;
 //   * four softmax warps a tile, one row a thread, keep the row's running
 //     maximum and sum.  O is rescaled in place only when a row's maximum has
 //     grown by more than 2^8 since its last scale, so rarely.
 //
-// Up to 64 channels one CTA works on one tile and two CTAs share an SM: P has
-// its own columns, so S(j + 1) is computed while the softmax works on S(j).
-// Up to 128 channels one CTA works on two tiles that share K and V (a single
-// tile would ask the L2 for 64 bytes a cycle and SM); P overlays S, and the
-// tensor core alternates between the tiles.
+// The next S buffer is always filled while the softmax works on one, so the
+// softmax warps run back to back.  They bound the kernel: an exponential with
+// its scaling, sum and conversion takes about 9 cycles a warp with two warps
+// to a scheduler (8 of them the special-function unit), 1,180 cycles for 128
+// rows x 128 keys, against 512 + 64 D / 16 cycles of products.
+//
+// Up to 64 channels one CTA works on one tile and two CTAs share an SM.  Up
+// to 128 channels one CTA works on two tiles that share K and V (a single
+// tile would ask the L2 for 64 bytes a cycle and SM).
 //
 // With few rows and many keys (SPLIT) the keys are divided over grid.y, and
 // within a CTA of two tile slots the blocks alternate between the slots; the
@@ -33,31 +37,26 @@ namespace pk {
 
 constexpr float kRescaleLog2 = 8.0f;  // growth of a row's maximum before O is rescaled
 
+constexpr int kKeys = 64;  // of a block
+
 template <int DT, bool BIAS>
 struct Fwd {
-  static constexpr int NQ = DT == 64 ? 1 : 2;         // tile slots of a CTA
+  static constexpr int NQ = DT == 64 ? 1 : 2;  // tile slots of a CTA
+  static constexpr int NS = DT == 64 ? 3 : 2;  // S buffers of a slot
   static constexpr int kHalves = DT / 64;
-  static constexpr int kStages = DT == 64 ? 4 : (BIAS ? 4 : 5);
-  // Four softmax warps a slot, then the MMA and the load warp.  A softmax thread
-  // holds a row of 128 scores: with two slots it takes registers from a third
-  // group of four warps, whose other two are idle; the shares stay within what
-  // the CTA was launched with.
-  static constexpr bool kExchange = NQ == 2, kTwice = NQ == 1;
-  static constexpr int kThreads = NQ == 1 ? 192 : 384;
-  static constexpr int kLaunchRegs = kExchange ? 168 : 0, kMore = 208, kLess = 80;
-  static_assert(NQ * kMore + kLess <= 3 * 168, "register exchange");
-  static constexpr uint32_t kTile = kHalves * kHalfBytes;
-  static constexpr uint32_t kQ = 0, kRing = NQ * kTile, kBars = kRing + kStages * kTile;
-  // barriers: Q landed; ring stages full, empty; per slot S ready, S read, P ready, P V done; drain
-  static constexpr int bQ = 0, bFull = 1, bEmpty = bFull + kStages, bS = bEmpty + kStages, bSFree = bS + NQ,
-                       bP = bSFree + NQ, bPV = bP + 2 * NQ,  // bP: keys 0-63, then 64-127
-                       bDrain = bPV + NQ, kNumBars = bDrain + 1;
+  static constexpr int kStages = DT == 64 ? 8 : (BIAS ? 8 : 10);
+  static constexpr int kThreads = 32 * (4 * NQ + 2);  // four softmax warps a slot, the MMA and the load warp
+  static constexpr uint32_t kTile = kHalves * kHalfBytes, kKV = kTile / 2, kKVHalf = kHalfBytes / 2;
+  static constexpr uint32_t kQ = 0, kRing = NQ * kTile, kBars = kRing + kStages * kKV;
+  // barriers: Q landed; ring stages full, empty; per slot and S buffer S ready, P ready, P V done; drain
+  static constexpr int bQ = 0, bFull = 1, bEmpty = bFull + kStages, bS = bEmpty + kStages, bP = bS + NQ * NS,
+                       bPV = bP + NQ * NS, bDrain = bPV + NQ * NS, kNumBars = bDrain + 1;
   static constexpr uint32_t kMisc = kBars + ((kNumBars * 8 + 15) / 16) * 16;  // TMEM base, sequence index
   static constexpr uint32_t kLut = kMisc + 16;
   static constexpr uint32_t bytes(uint32_t lut_floats) { return kLut + lut_floats * 4 + 1024; }
-  // TMEM columns
-  static constexpr uint32_t kCols = DT == 64 ? 256 : 512;
-  static constexpr uint32_t cS = 0, cP = DT == 64 ? 128 : 0, cO = DT == 64 ? 192 : 256;
+  // TMEM columns: the slots' S buffers, then their O
+  static constexpr uint32_t kCols = DT == 64 ? 256 : 512, cO = NQ * NS * kKeys;
+  static_assert(cO + NQ * DT <= kCols, "tensor memory");
 };
 
 struct FwdParams {
@@ -71,17 +70,13 @@ struct FwdParams {
   int* err;
 };
 
-#ifndef MN_PK_POLY_PAIRS
-#define MN_PK_POLY_PAIRS 4  // of every 16 probability pairs, this many take the FMA-pipe exp2
-#endif
-
 template <typename ET, int DT, bool BIAS, bool SPLIT>
 __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdParams p,
                    const __grid_constant__ Borders bo) {
   using F = Fwd<DT, BIAS>;
-  constexpr int NQ = F::NQ, ST = F::kStages, HV = F::kHalves;
+  constexpr int NQ = F::NQ, NS = F::NS, ST = F::kStages, HV = F::kHalves;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + F::kBars);
@@ -103,7 +98,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
   }
   if (warp == 2 && lane == 0) {
     for (int i = 0; i < F::kNumBars; ++i)
-      tc::mbar_init(bars + i, (i >= F::bSFree && i < F::bPV) ? 4 : 1);  // the softmax warps' arrivals
+      tc::mbar_init(bars + i, i >= F::bP && i < F::bPV ? 4 : 1);  // the softmax warps' arrivals
     tc::fence_mbar_init();
   }
   if (warp == 3 && lane == 0) {
@@ -136,7 +131,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     tok[i] = SPLIT ? t0 : t0 + i * p.ntok;
     const int last = min(s.nq, tok[i] + p.ntok) - 1;  // last token of the tile
     const int keys = a.causal ? min(s.nk, last + shift + 1) : s.nk;
-    end[i] = present && last >= tok[i] && keys > 0 ? (keys + 127) >> 7 : 0;
+    end[i] = present && last >= tok[i] && keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
   }
   const int nblk = max(end[0], end[NQ - 1]);
   const int j0 = SPLIT ? (int)((int64_t)nblk * blockIdx.y / p.splits) : 0;
@@ -153,7 +148,6 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
   bool ok = true;
 
   if (warp >= 4 * NQ) {
-    if (F::kExchange) regs_give<F::kLess>();
     if (warp == 4 * NQ + 1) {
       // ---------------------------------------------------------------- loads
       if (lane == 0 && j1 > j0) {
@@ -169,10 +163,10 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
           for (int kv = 0; kv < 2; ++kv, ++n) {
             const int st = n % ST;
             if (n >= ST && !(ok = wait(bars + F::bEmpty + st, ((n / ST) - 1) & 1, p.err))) break;
-            tma::expect_tx(bars + F::bFull + st, F::kTile);
+            tma::expect_tx(bars + F::bFull + st, F::kKV);
             for (int h = 0; h < HV; ++h)
-              load_3d(tc::smem_u32(base + F::kRing + st * F::kTile + h * kHalfBytes), kv ? &tm_v : &tm_k, h * 64, hk,
-                      s.k0 + j * 128, bars + F::bFull + st);
+              load_3d(tc::smem_u32(base + F::kRing + st * F::kKV + h * F::kKVHalf), kv ? &tm_v : &tm_k, h * 64, hk,
+                      s.k0 + j * kKeys, bars + F::bFull + st);
           }
         }
         if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
@@ -183,54 +177,48 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
       __syncwarp();
     } else if (warp == 4 * NQ) {
       // ----------------------------------------------------------------- MMAs
+      // S(c + NS) goes into the buffer of P(c) right behind P V(c): the products
+      // of a CTA run in the order of issue, so P(c) has been read by then
       constexpr uint32_t idesc_o = tc::idesc_f16(ab_bf16, 1, 128, DT);
-      int done[NQ];  // blocks of the slot whose S has been issued
+      int done[NQ];  // blocks of the slot so far
 #pragma unroll
       for (int i = 0; i < NQ; ++i) done[i] = 0;
-      auto cols_of = [&](int j) { return min(128, (s.nk - j * 128 + 31) & ~31); };  // keys of block j, in 32s
+      auto cols_of = [&](int j) { return min(kKeys, (s.nk - j * kKeys + 31) & ~31); };  // keys of block j, in 32s
       auto full = [&](int n) { return wait(bars + F::bFull + n % ST, (n / ST) & 1, p.err); };
-      auto issue_s = [&](int i, int j) -> bool {
+      auto s_cols = [&](int i, int c) { return tmem + (uint32_t)(i * NS + c % NS) * kKeys; };
+      auto issue_s = [&](int i, int j, int c) -> bool {  // c: the slot's count of block j
         const int n = 2 * (j - j0);
         if (!full(n)) return false;
+        const uint64_t dq = tc::sw128_desc(tc::smem_u32(base + F::kQ + (SPLIT ? 0 : i) * F::kTile), 16);
+        const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + F::kRing + (n % ST) * F::kKV), 16);
+        const uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, cols_of(j)), d = s_cols(i, c);
         if (elect_one()) {
           tc::fence_after_sync();
-          const uint64_t dq = tc::sw128_desc(tc::smem_u32(base + F::kQ + (SPLIT ? 0 : i) * F::kTile), 16);
-          const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + F::kRing + (n % ST) * F::kTile), 16);
-          const uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, cols_of(j));
 #pragma unroll
-          for (int kk = 0; kk < DT / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3);
-            tc::mma_f16_ss(tmem + F::cS + i * 128, dq + off, dk + off, idesc_s, kk > 0 ? 1u : 0u);
-          }
-          tc::mma_commit(bars + F::bS + i);
+          for (int kk = 0; kk < DT / 16; ++kk)
+            tc::mma_f16_ss(d, dq + (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3), dk + (kk >> 2) * (F::kKVHalf >> 4) + 2 * (kk & 3),
+                           idesc_s, kk > 0 ? 1u : 0u);
+          tc::mma_commit(bars + F::bS + i * NS + c % NS);
           if (i == last_user(j)) tc::mma_commit(bars + F::bEmpty + n % ST);
         }
         __syncwarp();
         return true;
       };
-      auto issue_pv = [&](int i, int j, int c) -> bool {  // c: the slot's block count before this one
+      auto issue_pv = [&](int i, int j, int c) -> bool {
         const int n = 2 * (j - j0) + 1;
         if (!full(n)) return false;
         const int cols = cols_of(j);
-        uint8_t* v = base + F::kRing + (n % ST) * F::kTile;
-        if (s.nk - j * 128 < cols && (SPLIT || i == 0 || j >= end[0])) zero_rows(v, s.nk - j * 128, cols, HV);
-        const uint64_t dv = tc::sw128_desc(tc::smem_u32(v), kHalfBytes);
-        const uint32_t t_o = tmem + F::cO + i * DT, t_p = tmem + F::cP + i * 128;
-        // the first 64 keys while the softmax works on the others
-        if (!wait(bars + F::bP + 2 * i, c & 1, p.err)) return false;
+        uint8_t* v = base + F::kRing + (n % ST) * F::kKV;
+        if (s.nk - j * kKeys < cols && (SPLIT || i == 0 || j >= end[0])) zero_rows(v, s.nk - j * kKeys, cols, HV, F::kKVHalf);
+        const uint64_t dv = tc::sw128_desc(tc::smem_u32(v), F::kKVHalf);
+        const uint32_t t_o = tmem + F::cO + i * DT, t_p = s_cols(i, c);
+        if (!wait(bars + F::bP + i * NS + c % NS, (c / NS) & 1, p.err)) return false;
         if (elect_one()) {
           tc::fence_after_sync();
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
+          for (int kk = 0; kk < kKeys / 16; ++kk)
             if (kk * 16 < cols) tc::mma_f16_ts(t_o, t_p + kk * 8, dv + 128 * kk, idesc_o, (c > 0 || kk > 0) ? 1u : 0u);
-        }
-        __syncwarp();
-        if (!wait(bars + F::bP + 2 * i + 1, c & 1, p.err)) return false;
-        if (elect_one()) {
-          tc::fence_after_sync();
-#pragma unroll
-          for (int kk = 4; kk < 8; ++kk)
-            if (kk * 16 < cols) tc::mma_f16_ts(t_o, t_p + kk * 8, dv + 128 * kk, idesc_o, 1u);
+          tc::mma_commit(bars + F::bPV + i * NS + c % NS);
           if (i == last_user(j)) tc::mma_commit(bars + F::bEmpty + n % ST);
         }
         __syncwarp();
@@ -239,26 +227,17 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
       if (j1 > j0) {
         ok = wait(bars + F::bQ, 0, p.err);
 #pragma unroll
-        for (int i = 0; i < NQ; ++i)
-          if (ok && first_of(i) < end_of(i)) ok = issue_s(i, first_of(i));
+        for (int c = 0; c < NS; ++c)
+#pragma unroll
+          for (int i = 0; i < NQ; ++i)
+            if (ok && first_of(i) + c * kStep < end_of(i)) ok = issue_s(i, first_of(i) + c * kStep, c);
         for (int j = j0; j < j1 && ok; ++j) {
 #pragma unroll
           for (int i = 0; i < NQ; ++i) {
             if (!ok || !takes(i, j)) continue;
             const int c = done[i]++;
-            const bool more = j + kStep < end_of(i);
-            if (DT == 64) {
-              // P has its own columns: S(j + 1) as soon as S(j) has been read
-              if (more) ok = wait(bars + F::bSFree + i, c & 1, p.err) && issue_s(i, j + kStep);
-              if (ok) ok = issue_pv(i, j, c);
-              if (ok && elect_one()) tc::mma_commit(bars + F::bPV + i);
-            } else {
-              // P overlays S: the MMAs of a CTA run in the order of issue, so
-              // S(j + 1) overwrites P(j) only after P V(j) has read it
-              ok = issue_pv(i, j, c);
-              if (ok && more) ok = issue_s(i, j + kStep);
-              if (ok && !more && elect_one()) tc::mma_commit(bars + F::bPV + i);
-            }
+            ok = issue_pv(i, j, c);
+            if (ok && j + NS * kStep < end_of(i)) ok = issue_s(i, j + NS * kStep, c + NS);
           }
         }
         if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
@@ -271,12 +250,10 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     }
   } else {
     // ------------------------------------------------------------- softmax
-    if (F::kExchange) regs_take<F::kMore>();
     const int i = warp >> 2, wq = warp & 3;
     const int r = wq * 32 + lane;
     const uint32_t lane_sel = (uint32_t)(wq * 32) << 16;
-    const uint32_t t_s = tmem + F::cS + i * 128 + lane_sel, t_p = tmem + F::cP + i * 128 + lane_sel,
-                   t_o = tmem + F::cO + i * DT + lane_sel;
+    const uint32_t t_o = tmem + F::cO + i * DT + lane_sel;
     const float sl2 = a.scale * kLog2e;  // scores enter the softmax in log2 units
     const int my = tok[i] + r / G, g = r % G;
     const bool mine = present && r < G * p.ntok && my < s.nq;  // a row of the sequence
@@ -289,86 +266,66 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     const float* row_lut = lut + (BIAS ? (mine ? g : 0) * p.span : 0);
     float m_run = -INFINITY, l_run = 0.f;
     int c = 0;
+    auto pv_done = [&](int b) { return wait(bars + F::bPV + i * NS + b % NS, (b / NS) & 1, p.err); };
     for (int j = first_of(i); j < end_of(i) && ok; j += kStep, ++c) {
-      ok = wait(bars + F::bS + i, c & 1, p.err);
+      const int buf = c % NS;
+      const uint32_t t_s = tmem + (uint32_t)(i * NS + buf) * kKeys + lane_sel;
+      ok = wait(bars + F::bS + i * NS + buf, (c / NS) & 1, p.err);
       if (!ok) break;
-      tc::fence_after_sync();
-      const int k0 = j * 128;
-      const int nch = (min(128, s.nk - k0) + 31) >> 5;  // chunks of 32 columns that S and P hold
-      const bool fast = live && nch == 4 && kmin >= k0 + 128;  // the warp's rows see the whole block
-      const int wch = min(nch, max(0, (kmax - k0 + 31) >> 5));  // chunks that some row of the warp sees
-      float f = sl2, add = 0.f;  // x enters the softmax as f x + add
-      bool mixed = false;
-      if (BIAS && live) {
-        const int lo = k0 - pmax, hi = k0 + 127 - pmin;  // distances of the warp's rows
-        if (hi <= -p.reach) {
-          add = row_lut[0];
-        } else if (lo >= p.span - 1 - p.reach) {
-          add = row_lut[p.span - 1];
-        } else {
-          mixed = true;
-          f = 1.f;
-        }
-      }
-      // 64 scores of the row, with the bias where it differs by key and the mask
-      auto fetch = [&](float* y, int hf) {
-        if (fast) {
-          tc::tmem_ld32_nowait(t_s + hf * 64, y);
-          tc::tmem_ld32_nowait(t_s + hf * 64 + 32, y + 32);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) y[e] = 0.f;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (hf * 2 + u < wch) tc::tmem_ld32_nowait(t_s + hf * 64 + u * 32, y + u * 32);
-        }
-      };
-      auto shape = [&](float* y, int hf) {
-        if (BIAS && mixed) {
-          const int at = k0 + hf * 64 - pos + p.reach;
-#pragma unroll
-          for (int e = 0; e < 64; ++e) y[e] = fmaf(y[e], sl2, row_lut[min(max(at + e, 0), p.span - 1)]);
-        }
-        if (!fast) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (k0 + hf * 64 + e >= klim) y[e] = -INFINITY;
-        }
-      };
-      float x[F::kTwice ? 64 : 128], mx = -INFINITY;
       if (live) {
-        fetch(x, 0);
-        tc::tmem_ld_wait<64>(x);
-        if (F::kTwice) {
-          shape(x, 0);
-          mx = max64(x, mx);
-          fetch(x, 1);
-          tc::tmem_ld_wait<64>(x);
-          shape(x, 1);
-          mx = max64(x, mx);
-        } else {
-          fetch(x + 64, 1);
-          shape(x, 0);
-          mx = max64(x, mx);
-          tc::tmem_ld_wait<64>(x + 64);
-          shape(x + 64, 1);
-          mx = max64(x + 64, mx);
+        tc::fence_after_sync();
+        const int k0 = j * kKeys;
+        const int nch = (min(kKeys, s.nk - k0) + 31) >> 5;        // chunks of 32 columns that S and P hold
+        const int wch = min(nch, max(0, (kmax - k0 + 31) >> 5));  // of those, seen by some row of the warp
+        const bool fast = nch == 2 && kmin >= k0 + kKeys;         // the warp's rows see the whole block
+        float x[kKeys];
+        if (wch > 0) tc::tmem_ld32_nowait(t_s, x);
+        if (wch > 1) tc::tmem_ld32_nowait(t_s + 32, x + 32);
+        tc::tmem_ld_wait<kKeys>(x);
+        float f = sl2, add = 0.f;  // x enters the softmax as f x + add
+        if (BIAS) {
+          const int lo = k0 - pmax, hi = k0 + kKeys - 1 - pmin;  // distances of the warp's rows
+          if (hi <= -p.reach) {
+            add = row_lut[0];
+          } else if (lo >= p.span - 1 - p.reach) {
+            add = row_lut[p.span - 1];
+          } else {
+            const int at = k0 - pos + p.reach;
+#pragma unroll
+            for (int e = 0; e < kKeys; ++e) x[e] = fmaf(x[e], sl2, row_lut[min(max(at + e, 0), p.span - 1)]);
+            f = 1.f;
+          }
         }
-        mx = mx * f + add;
-      }
-      const float m_new = fmaxf(m_run, mx);
-      const float m_use = (m_run == -INFINITY || m_new - m_run > kRescaleLog2) ? m_new : m_run;
-      const float corr = (m_run == -INFINITY || m_use == m_run) ? 1.f : ex2(m_run - m_use);
-      const float nm1 = add - (m_use == -INFINITY ? 0.f : m_use);
-      const float2 nm = make_float2(nm1, nm1), f2 = make_float2(f, f);
-      // With P apart from S, P V(j - 1) may still read P(j - 1) (a warp without
-      // rows waits too, or its arrival for P(j) could complete the phase of
-      // P(j - 1)); with P over S the commit behind S(j) covers P V(j - 1).
-      if (DT == 64 && c > 0 && !(ok = wait(bars + F::bPV + i, (c - 1) & 1, p.err))) break;
-      if (live) {
+        if (!fast) {  // hidden keys get exactly 0
+#pragma unroll
+          for (int e = 0; e < kKeys; ++e)
+            if (k0 + e >= klim) x[e] = -INFINITY;
+        }
+        const float mx = max32(x + 32, max32(x, -INFINITY)) * f + add;
+        const float m_new = fmaxf(m_run, mx);
+        const float m_use = (m_run == -INFINITY || m_new - m_run > kRescaleLog2) ? m_new : m_run;
+        const float corr = (m_run == -INFINITY || m_use == m_run) ? 1.f : ex2(m_run - m_use);
         m_run = m_use;
-        if (c > 0 && __any_sync(MN_FULL_MASK, corr != 1.f)) {  // O is at rest
-          if (DT == 64) tc::fence_after_sync();
+        const float nm1 = add - (m_use == -INFINITY ? 0.f : m_use);
+        const float2 nm = make_float2(nm1, nm1), f2 = make_float2(f, f);
+        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t pk[kKeys / 2];
+#pragma unroll
+        for (int e = 0; e < kKeys / 2; ++e) {
+          const float2 y = ffma2(make_float2(x[2 * e], x[2 * e + 1]), f2, nm);
+          const float2 q = make_float2(ex2(y.x), ex2(y.y));
+          sum2[e & 1] = fadd2(sum2[e & 1], q);
+          pk[e] = pack2<ET>(q.x, q.y);
+        }
+        tc::tmem_st16_nowait(t_s, pk);
+        if (nch > 1) tc::tmem_st16_nowait(t_s + 16, pk + 16);
+        const float2 ss = fadd2(sum2[0], sum2[1]);
+        l_run = l_run * corr + (ss.x + ss.y);
+        tc::tmem_wait_st();
+        // rescale the running output rows once P V of the block before has completed
+        if (c > 0 && __any_sync(MN_FULL_MASK, corr != 1.f)) {
+          if (!(ok = pv_done(c - 1))) break;
+          tc::fence_after_sync();
           float o[32];
 #pragma unroll
           for (int u = 0; u < DT / 32; ++u) {
@@ -379,58 +336,13 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
           }
         }
       }
-      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t pk[32];
-        float* y = F::kTwice ? x : x + hf * 64;
-        if (F::kTwice) {
-          if (live) {  // the scores once more: a row of them does not fit the registers of two CTAs
-            fetch(y, hf);
-            tc::tmem_ld_wait<64>(y);
-            shape(y, hf);
-          }
-          if (hf == 1) {
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tma::arrive(bars + F::bSFree + i);
-          }
-        }
-        if (fast) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float2 v = ffma2(make_float2(y[2 * e], y[2 * e + 1]), f2, nm);
-            // pairs spread evenly over the row take the polynomial
-            const float2 q = (MN_PK_POLY_PAIRS > 0 && (e * MN_PK_POLY_PAIRS) % 16 >= 16 - MN_PK_POLY_PAIRS)
-                                 ? ex2_poly2(v)
-                                 : make_float2(ex2(v.x), ex2(v.y));
-            sum2[e & 1] = fadd2(sum2[e & 1], q);
-            pk[e] = pack2<ET>(q.x, q.y);
-          }
-          tc::tmem_st16_nowait(t_p + hf * 32, pk);
-          tc::tmem_st16_nowait(t_p + hf * 32 + 16, pk + 16);
-        } else if (live) {  // hidden keys get exactly 0
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float2 v = ffma2(make_float2(y[2 * e], y[2 * e + 1]), f2, nm);
-            const float2 q = make_float2(ex2(v.x), ex2(v.y));
-            sum2[e & 1] = fadd2(sum2[e & 1], q);
-            pk[e] = pack2<ET>(q.x, q.y);
-          }
-          tc::tmem_st16_nowait(t_p + hf * 32, pk);
-          tc::tmem_st16_nowait(t_p + hf * 32 + 16, pk + 16);
-        }
-        tc::tmem_wait_st();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tma::arrive(bars + F::bP + 2 * i + hf);
-      }
-      const float2 ss = fadd2(sum2[0], sum2[1]);
-      l_run = l_run * corr + (ss.x + ss.y);
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tma::arrive(bars + F::bP + i * NS + buf);
     }
     if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
     if (ok && c > 0) {
-      ok = wait(bars + F::bPV + i, DT == 64 ? (c - 1) & 1 : 0, p.err);
+      ok = pv_done(c - 1);
       tc::fence_after_sync();
     }
     if (ok && live) {
@@ -563,8 +475,8 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   CUtensorMap mq, mk, mv;
   if (!bind_context()) return false;
   if (!map_q(&mq, bf16, a->q, a->q_st, a->q_sh, a->tq, a->heads, a->kv_heads, a->head_dim, pl.ntok)) return false;
-  if (!map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim)) return false;
-  if (!map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim)) return false;
+  if (!map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, kKeys)) return false;
+  if (!map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, kKeys)) return false;
   FwdParams p;
   p.a = *a;
   p.group = a->heads / a->kv_heads;
@@ -582,7 +494,7 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   p.err = err;
   const size_t smem = F::bytes(p.span * p.group);
   auto kern = forward_kernel<ET, DT, BIAS, SPLIT>;
-  if (!ensure_smem(kern, smem) || !launch_regs(kern, F::kLaunchRegs)) return false;
+  if (!ensure_smem(kern, smem)) return false;
   const int64_t slots = tile_slots(a->tq, a->nseq, SPLIT ? pl.ntok : F::NQ * pl.ntok) * a->kv_heads;
   if (slots > 0x7fffffff) return false;
   kern<<<dim3((unsigned)slots, pl.splits), F::kThreads, smem, st>>>(mq, mk, mv, p, bo);

@@ -43,10 +43,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-__device__ __forceinline__ float max64(const float* x, float m) {
+__device__ __forceinline__ float max32(const float* x, float m) {
   float a[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int e = 0; e < 64; e += 8)
+  for (int e = 0; e < 32; e += 8)
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = max3(a[i], x[e + 2 * i], x[e + 2 * i + 1]);
   return fmaxf(max3(a[0], a[1], a[2]), a[3]);
@@ -54,21 +54,22 @@ __device__ __forceinline__ float max64(const float* x, float m) {
 
 // 2^y for a pair of y <= 8 on the FMA pipe (the polynomial of
 // csrc/exp2_fit.py, relative error 2.7e-6): y = n + f with n the nearest
-// integer, taken from the low bits of y + 1.5 * 2^23.  y is clamped at -126,
+// integer.  y + 1.5 * 2^23 holds n in its low bits, and shifting it left by 23
+// leaves n in the exponent's place and nothing else.  y is clamped at -126,
 // NaN kept, so it serves unmasked scores only: 2^-126 in the place of less.
 __device__ __forceinline__ float2 ex2_poly2(float2 y) {
   y.x = max_nan(y.x, -126.f);
   y.y = max_nan(y.y, -126.f);
-  const float2 magic = make_float2(12582912.f, 12582912.f);
-  const float2 t = fadd2(y, magic);
-  const float2 f = fadd2(y, fadd2(magic, make_float2(-t.x, -t.y)));
+  const float2 t = fadd2(y, make_float2(12582912.f, 12582912.f));
+  const float2 n = fadd2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = ffma2(n, make_float2(-1.f, -1.f), y);
   float2 p = ffma2(f, make_float2(9.570100344717503e-03f, 9.570100344717503e-03f),
                    make_float2(5.591786280274391e-02f, 5.591786280274391e-02f));
   p = ffma2(p, f, make_float2(2.402474433183670e-01f, 2.402474433183670e-01f));
   p = ffma2(p, f, make_float2(6.931217908859253e-01f, 6.931217908859253e-01f));
   p = ffma2(p, f, make_float2(9.999992847442627e-01f, 9.999992847442627e-01f));
-  const int nx = __float_as_int(t.x) - 0x4B400000, ny = __float_as_int(t.y) - 0x4B400000;
-  return make_float2(__int_as_float(__float_as_int(p.x) + (nx << 23)), __int_as_float(__float_as_int(p.y) + (ny << 23)));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (int)((uint32_t)__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (int)((uint32_t)__float_as_int(t.y) << 23)));
 }
 
 // Wait for the phase with the given parity, bounded in time like
@@ -104,15 +105,6 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(is));
   return is != 0;
 }
-
-// Register exchange between the warp groups of a CTA (a whole group executes
-// it).  A taker waits until the givers' registers are free, so the shares may
-// not exceed what the CTA was launched with: launch_regs() on the host checks
-// the launch, a static_assert at each kernel the shares.
-template <int N>
-__device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // Tiles of `m` rows of every sequence share one index space without a prefix
 // sum: sequence b's tiles begin at slot cu[b] / m + b.  A sequence of L rows
@@ -172,13 +164,14 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, in
       : "memory");
 }
 
-// Zero rows [from, to) of a tile of 128-byte rows in `halves` halves (a whole
-// warp), for operand rows that a product must not read: 0 times NaN is NaN.
-__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to, int halves) {
+// Zero rows [from, to) of a tile of 128-byte rows in `halves` parts `stride`
+// bytes apart (a whole warp), for operand rows that a product must not read:
+// 0 times NaN is NaN.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to, int halves, uint32_t stride = kHalfBytes) {
   const int lane = threadIdx.x & 31, n = (to - from) * 8;
   for (int h = 0; h < halves; ++h)
     for (int i = lane; i < n; i += 32)
-      *reinterpret_cast<uint4*>(tile + h * kHalfBytes + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(tile + h * stride + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
   tc::fence_async_smem();
   __syncwarp();
 }
@@ -203,37 +196,19 @@ inline bool map_q(CUtensorMap* map, bool bf16, const void* p, int64_t st, int64_
   const cuuint32_t box[4] = {64, (cuuint32_t)g, 1, (cuuint32_t)n};
   return tma::encode(map, bf16, 4, p, dims, strides, box, true, true);
 }
-// Key-side rows [rows, kv_heads, d] with boxes of 64 channels x 128 rows
-inline bool map_k(CUtensorMap* map, bool bf16, const void* p, int64_t st, int64_t sh, int rows, int kv_heads, int d) {
+// Key-side rows [rows, kv_heads, d] with boxes of 64 channels x n rows
+inline bool map_k(CUtensorMap* map, bool bf16, const void* p, int64_t st, int64_t sh, int rows, int kv_heads, int d, int n) {
   if (kv_heads == 1) sh = (d + 7) / 8 * 8;
   if (rows == 1) st = sh * kv_heads;
   const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)kv_heads, (cuuint64_t)rows};
   const cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
-  const cuuint32_t box[3] = {64, 1, 128};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)n};
   return tma::encode(map, bf16, 3, p, dims, strides, box, true, true);
 }
 // what a tensor map needs of a [rows, heads, d] tensor
 inline bool rows_ok(const void* p, int64_t st, int64_t sh, int rows, int heads) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || (st > 0 && st % 8 == 0)) &&
          (heads <= 1 || (sh > 0 && sh % 8 == 0)) && st < (int64_t(1) << 38) && sh < (int64_t(1) << 31);
-}
-// The kernel was compiled to launch with at least `regs` registers a thread.
-template <typename F>
-inline bool launch_regs(F* func, int regs) {
-  static std::mutex mu;
-  static std::map<const void*, int> known;
-  const void* key = reinterpret_cast<const void*>(func);
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = known.find(key);
-  if (it == known.end()) {
-    cudaFuncAttributes at;
-    if (cudaFuncGetAttributes(&at, func) != cudaSuccess) {
-      cudaGetLastError();
-      return false;
-    }
-    it = known.emplace(key, at.numRegs).first;
-  }
-  return it->second >= regs;
 }
 inline int sm_count() {
   int dev = 0, sms = 148;
