@@ -4,26 +4,28 @@
 //
 // A tile is 128 rows of (token, head of the group), token-major: the heads
 // that share a key head sit in one tile, so grouped heads read their keys and
-// values once and one token's form is a tile of its heads.  Per block of 64
-// keys:
+// values once and one token's form is a tile of its heads.  Per block of keys:
 //
-//   * a load warp brings K and V (a ring of stages) by TMA;
-//   * an MMA warp issues S = Q K^T into one of the slot's S buffers in tensor
-//     memory and, once the softmax warps have written the probabilities over
-//     it as 16-bit values, O += P V with P read from tensor memory;
+//   * a load warp brings K and V (a ring of tiles) by TMA;
+//   * an MMA warp issues S = Q K^T into tensor memory and, once the softmax
+//     warps have written the probabilities over it as 16-bit values, O += P V
+//     with P read from tensor memory;
 //   * four softmax warps a tile, one row a thread, keep the row's running
 //     maximum and sum.  O is rescaled in place only when a row's maximum has
 //     grown by more than 2^8 since its last scale, so rarely.
 //
-// The next S buffer is always filled while the softmax works on one, so the
-// softmax warps run back to back.  They bound the kernel: an exponential with
-// its scaling, sum and conversion takes about 9 cycles a warp with two warps
-// to a scheduler (8 of them the special-function unit), 1,180 cycles for 128
-// rows x 128 keys, against 512 + 64 D / 16 cycles of products.
+// The softmax warps bound the kernel: an exponential with its scaling, sum and
+// conversion takes a scheduler about 9 cycles with two warps on it (8 of them
+// the special-function unit; a polynomial on the FMA pipe takes as long), so
+// 1,180 cycles for 128 rows x 128 keys, against 16 D cycles of products... 
 //
-// Up to 64 channels one CTA works on one tile and two CTAs share an SM.  Up
-// to 128 channels one CTA works on two tiles that share K and V (a single
-// tile would ask the L2 for 64 bytes a cycle and SM).
+// Up to 64 channels one CTA works on one tile and two CTAs share an SM; blocks
+// of 64 keys, three S buffers, so that the softmax warps run back to back.
+// Up to 128 channels one CTA works on two tiles that share K and V (a single
+// tile would ask the L2 for 64 bytes a cycle and SM); tensor memory then holds
+// one S a tile, and the tiles take turns: one's products run under the
+// other's softmax.  Blocks of 128 keys, since a product of 64 columns takes
+// the tensor core as long as one of 128.
 //
 // With few rows and many keys (SPLIT) the keys are divided over grid.y, and
 // within a CTA of two tile slots the blocks alternate between the slots; the
@@ -37,25 +39,34 @@ namespace pk {
 
 constexpr float kRescaleLog2 = 8.0f;  // growth of a row's maximum before O is rescaled
 
-constexpr int kKeys = 64;  // of a block
-
 template <int DT, bool BIAS>
 struct Fwd {
-  static constexpr int NQ = DT == 64 ? 1 : 2;  // tile slots of a CTA
-  static constexpr int NS = DT == 64 ? 3 : 2;  // S buffers of a slot
+  static constexpr int NQ = DT == 64 ? 1 : 2;     // tile slots of a CTA
+  static constexpr int KB = DT == 64 ? 64 : 128;  // keys of a block
+  static constexpr int NS = DT == 64 ? 3 : 1;     // S buffers of a slot
   static constexpr int kHalves = DT / 64;
-  static constexpr int kStages = DT == 64 ? 8 : (BIAS ? 8 : 10);
-  static constexpr int kThreads = 32 * (4 * NQ + 2);  // four softmax warps a slot, the MMA and the load warp
-  static constexpr uint32_t kTile = kHalves * kHalfBytes, kKV = kTile / 2, kKVHalf = kHalfBytes / 2;
+  static constexpr int kStages = DT == 64 ? 10 : (BIAS ? 4 : 5);  // ring: K and V tiles of the blocks in turn
+  static_assert(kStages >= 2 * NQ * NS, "S runs NS blocks of a slot ahead");
+  // Four softmax warps a slot, the MMA and the load warp.  A softmax thread
+  // holds a row's scores; with 128 of them it takes registers from a third
+  // group of four warps, two of them idle.  The shares stay within what the
+  // CTA was launched with.
+  static constexpr bool kExchange = KB == 128;
+  static constexpr int kThreads = kExchange ? 128 * (NQ + 1) : 32 * (4 * NQ + 2);
+  static constexpr int kLaunchRegs = kExchange ? 168 : 0, kMore = 208, kLess = 80;
+  static_assert(!kExchange || NQ * kMore + kLess <= (NQ + 1) * kLaunchRegs, "register exchange");
+  static constexpr uint32_t kTile = kHalves * kHalfBytes, kKVHalf = KB * 128, kKV = kHalves * kKVHalf;
   static constexpr uint32_t kQ = 0, kRing = NQ * kTile, kBars = kRing + kStages * kKV;
-  // barriers: Q landed; ring stages full, empty; per slot and S buffer S ready, P ready, P V done; drain
+  // barriers: Q landed; ring stages full, empty; per slot and S buffer S
+  // ready, P ready (by 64 keys), the last P V done; drain
+  static constexpr int kParts = KB / 64;
   static constexpr int bQ = 0, bFull = 1, bEmpty = bFull + kStages, bS = bEmpty + kStages, bP = bS + NQ * NS,
-                       bPV = bP + NQ * NS, bDrain = bPV + NQ * NS, kNumBars = bDrain + 1;
+                       bPV = bP + NQ * NS * kParts, bDrain = bPV + NQ * NS, kNumBars = bDrain + 1;
   static constexpr uint32_t kMisc = kBars + ((kNumBars * 8 + 15) / 16) * 16;  // TMEM base, sequence index
   static constexpr uint32_t kLut = kMisc + 16;
   static constexpr uint32_t bytes(uint32_t lut_floats) { return kLut + lut_floats * 4 + 1024; }
   // TMEM columns: the slots' S buffers, then their O
-  static constexpr uint32_t kCols = DT == 64 ? 256 : 512, cO = NQ * NS * kKeys;
+  static constexpr uint32_t kCols = DT == 64 ? 256 : 512, cO = NQ * NS * KB;
   static_assert(cO + NQ * DT <= kCols, "tensor memory");
 };
 
@@ -76,7 +87,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdParams p,
                    const __grid_constant__ Borders bo) {
   using F = Fwd<DT, BIAS>;
-  constexpr int NQ = F::NQ, NS = F::NS, ST = F::kStages, HV = F::kHalves;
+  constexpr int NQ = F::NQ, NS = F::NS, ST = F::kStages, HV = F::kHalves, kKeys = F::KB;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + F::kBars);
@@ -145,9 +156,11 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     return SPLIT ? (NQ == 1 ? 0 : (j - j0) & 1) : (NQ > 1 && j < end[NQ - 1] ? NQ - 1 : 0);
   };
   constexpr int ab_bf16 = std::is_same<ET, __nv_bfloat16>::value ? 1 : 0;
+  constexpr bool kCommitV = DT == 64 || SPLIT;  // a V tile is freed by P V's own commit
   bool ok = true;
 
   if (warp >= 4 * NQ) {
+    if (F::kExchange) regs_give<F::kLess>();
     if (warp == 4 * NQ + 1) {
       // ---------------------------------------------------------------- loads
       if (lane == 0 && j1 > j0) {
@@ -158,16 +171,14 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
           for (int h = 0; h < HV; ++h)
             tma::load_4d(tc::smem_u32(base + F::kQ + i * F::kTile + h * kHalfBytes), &tm_q, h * 64, 0, hk, s.q0 + tok[i],
                          bars + F::bQ);
-        int n = 0;
-        for (int j = j0; j < j1 && ok; ++j) {
-          for (int kv = 0; kv < 2; ++kv, ++n) {
-            const int st = n % ST;
-            if (n >= ST && !(ok = wait(bars + F::bEmpty + st, ((n / ST) - 1) & 1, p.err))) break;
-            tma::expect_tx(bars + F::bFull + st, F::kKV);
-            for (int h = 0; h < HV; ++h)
-              load_3d(tc::smem_u32(base + F::kRing + st * F::kKV + h * F::kKVHalf), kv ? &tm_v : &tm_k, h * 64, hk,
-                      s.k0 + j * kKeys, bars + F::bFull + st);
-          }
+        int n = 0;  // tiles loaded: K(j0), V(j0), K(j0 + 1), ...
+        for (; n < 2 * (j1 - j0) && ok; ++n) {
+          const int st = n % ST;
+          if (n >= ST && !(ok = wait(bars + F::bEmpty + st, (n / ST - 1) & 1, p.err))) break;
+          tma::expect_tx(bars + F::bFull + st, F::kKV);
+          for (int h = 0; h < HV; ++h)
+            load_3d(tc::smem_u32(base + F::kRing + st * F::kKV + h * F::kKVHalf), (n & 1) ? &tm_v : &tm_k, h * 64, hk,
+                    s.k0 + (j0 + n / 2) * kKeys, bars + F::bFull + st);
         }
         if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
         // every copy issued has landed before the CTA may release its shared memory
@@ -184,11 +195,10 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
 #pragma unroll
       for (int i = 0; i < NQ; ++i) done[i] = 0;
       auto cols_of = [&](int j) { return min(kKeys, (s.nk - j * kKeys + 31) & ~31); };  // keys of block j, in 32s
-      auto full = [&](int n) { return wait(bars + F::bFull + n % ST, (n / ST) & 1, p.err); };
       auto s_cols = [&](int i, int c) { return tmem + (uint32_t)(i * NS + c % NS) * kKeys; };
       auto issue_s = [&](int i, int j, int c) -> bool {  // c: the slot's count of block j
         const int n = 2 * (j - j0);
-        if (!full(n)) return false;
+        if (!wait(bars + F::bFull + n % ST, (n / ST) & 1, p.err)) return false;
         const uint64_t dq = tc::sw128_desc(tc::smem_u32(base + F::kQ + (SPLIT ? 0 : i) * F::kTile), 16);
         const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + F::kRing + (n % ST) * F::kKV), 16);
         const uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, cols_of(j)), d = s_cols(i, c);
@@ -199,29 +209,32 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
             tc::mma_f16_ss(d, dq + (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3), dk + (kk >> 2) * (F::kKVHalf >> 4) + 2 * (kk & 3),
                            idesc_s, kk > 0 ? 1u : 0u);
           tc::mma_commit(bars + F::bS + i * NS + c % NS);
-          if (i == last_user(j)) tc::mma_commit(bars + F::bEmpty + n % ST);
         }
         __syncwarp();
         return true;
       };
       auto issue_pv = [&](int i, int j, int c) -> bool {
-        const int n = 2 * (j - j0) + 1;
-        if (!full(n)) return false;
-        const int cols = cols_of(j);
+        const int n = 2 * (j - j0) + 1, cols = cols_of(j);
+        if (!wait(bars + F::bFull + n % ST, (n / ST) & 1, p.err)) return false;
         uint8_t* v = base + F::kRing + (n % ST) * F::kKV;
         if (s.nk - j * kKeys < cols && (SPLIT || i == 0 || j >= end[0])) zero_rows(v, s.nk - j * kKeys, cols, HV, F::kKVHalf);
         const uint64_t dv = tc::sw128_desc(tc::smem_u32(v), F::kKVHalf);
         const uint32_t t_o = tmem + F::cO + i * DT, t_p = s_cols(i, c);
-        if (!wait(bars + F::bP + i * NS + c % NS, (c / NS) & 1, p.err)) return false;
-        if (elect_one()) {
-          tc::fence_after_sync();
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            if (kk * 16 < cols) tc::mma_f16_ts(t_o, t_p + kk * 8, dv + 128 * kk, idesc_o, (c > 0 || kk > 0) ? 1u : 0u);
-          tc::mma_commit(bars + F::bPV + i * NS + c % NS);
-          if (i == last_user(j)) tc::mma_commit(bars + F::bEmpty + n % ST);
+        for (int part = 0; part < F::kParts; ++part) {  // 64 keys while the softmax works on the next
+          if (!wait(bars + F::bP + (i * NS + c % NS) * F::kParts + part, (c / NS) & 1, p.err)) return false;
+          if (elect_one()) {
+            tc::fence_after_sync();
+#pragma unroll
+            for (int kk = part * 4; kk < part * 4 + 4; ++kk)
+              if (kk * 16 < cols) tc::mma_f16_ts(t_o, t_p + kk * 8, dv + 128 * kk, idesc_o, (c > 0 || kk > 0) ? 1u : 0u);
+            // a commit takes its thread some 200 cycles: where the products bound the
+            // kernel only the one that no S behind it replaces
+            if (kCommitV && part == F::kParts - 1 && i == last_user(j)) tc::mma_commit(bars + F::bEmpty + n % ST);
+            if (part == F::kParts - 1 && j + NS * kStep >= end_of(i)) tc::mma_commit(bars + F::bPV + i * NS + c % NS);
+          }
+          __syncwarp();
         }
-        __syncwarp();
         return true;
       };
       if (j1 > j0) {
@@ -250,6 +263,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     }
   } else {
     // ------------------------------------------------------------- softmax
+    if (F::kExchange) regs_take<F::kMore>();
     const int i = warp >> 2, wq = warp & 3;
     const int r = wq * 32 + lane;
     const uint32_t lane_sel = (uint32_t)(wq * 32) << 16;
@@ -266,23 +280,50 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     const float* row_lut = lut + (BIAS ? (mine ? g : 0) * p.span : 0);
     float m_run = -INFINITY, l_run = 0.f;
     int c = 0;
-    auto pv_done = [&](int b) { return wait(bars + F::bPV + i * NS + b % NS, (b / NS) & 1, p.err); };
+    const int total = first_of(i) < end_of(i) ? (end_of(i) - first_of(i) + kStep - 1) / kStep : 0;
+    // P V of the slot's block b has completed: S(b + NS) is behind it, or its own commit
+    auto pv_done = [&](int b) {
+      return b + NS < total ? wait(bars + F::bS + i * NS + b % NS, (b / NS + 1) & 1, p.err)
+                            : wait(bars + F::bPV + i * NS + b % NS, 0, p.err);
+    };
     for (int j = first_of(i); j < end_of(i) && ok; j += kStep, ++c) {
       const int buf = c % NS;
       const uint32_t t_s = tmem + (uint32_t)(i * NS + buf) * kKeys + lane_sel;
       ok = wait(bars + F::bS + i * NS + buf, (c / NS) & 1, p.err);
       if (!ok) break;
-      if (live) {
-        tc::fence_after_sync();
-        const int k0 = j * kKeys;
-        const int nch = (min(kKeys, s.nk - k0) + 31) >> 5;        // chunks of 32 columns that S and P hold
-        const int wch = min(nch, max(0, (kmax - k0 + 31) >> 5));  // of those, seen by some row of the warp
-        const bool fast = nch == 2 && kmin >= k0 + kKeys;         // the warp's rows see the whole block
-        float x[kKeys];
-        if (wch > 0) tc::tmem_ld32_nowait(t_s, x);
-        if (wch > 1) tc::tmem_ld32_nowait(t_s + 32, x + 32);
+      // S(j) is there: K(j) has been read, and V of the block whose P V came before S(j)
+      if (wq == 0 && lane == 0) {
+        const int jp = j - NS * kStep;
+        if (i == last_user(j)) tma::arrive(bars + F::bEmpty + (2 * (j - j0)) % ST);
+        if (!kCommitV && c >= NS && i == last_user(jp)) tma::arrive(bars + F::bEmpty + (2 * (jp - j0) + 1) % ST);
+      }
+      tc::fence_after_sync();
+      const int k0 = j * kKeys;
+      const int nch = (min(kKeys, s.nk - k0) + 31) >> 5;              // chunks of 32 columns that S and P hold
+      const bool fast = nch == kKeys / 32 && kmin >= k0 + kKeys;      // the warp's rows see the whole block
+      float x[kKeys], mx = -INFINITY;
+      float f = sl2, add = 0.f;  // x enters the softmax as f x + add
+      if (__builtin_expect(fast, 1)) {
+        if (live) {
+          tc::tmem_ld32_nowait(t_s, x);
+          tc::tmem_ld32_nowait(t_s + 32, x + 32);
+          tc::tmem_ld_wait<64>(x);
+          if constexpr (kKeys == 128) {
+            tc::tmem_ld32_nowait(t_s + 64, x + 64);
+            tc::tmem_ld32_nowait(t_s + 96, x + 96);
+            if (!BIAS) mx = max32(x + 32, max32(x, mx));
+            tc::tmem_ld_wait<64>(x + 64);
+          }
+        }
+      } else if (live) {
+        const int wch = min(nch, max(0, (kmax - k0 + 31) >> 5));  // chunks that some row of the warp sees
+#pragma unroll
+        for (int u = 0; u < kKeys / 32; ++u)
+          if (u < wch) tc::tmem_ld32_nowait(t_s + u * 32, x + u * 32);
         tc::tmem_ld_wait<kKeys>(x);
-        float f = sl2, add = 0.f;  // x enters the softmax as f x + add
+      }
+      float corr = 1.f;
+      if (live) {
         if (BIAS) {
           const int lo = k0 - pmax, hi = k0 + kKeys - 1 - pmin;  // distances of the warp's rows
           if (hi <= -p.reach) {
@@ -296,34 +337,20 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
             f = 1.f;
           }
         }
-        if (!fast) {  // hidden keys get exactly 0
+        if (__builtin_expect(!fast, 0)) {  // hidden keys get exactly 0
 #pragma unroll
           for (int e = 0; e < kKeys; ++e)
             if (k0 + e >= klim) x[e] = -INFINITY;
         }
-        const float mx = max32(x + 32, max32(x, -INFINITY)) * f + add;
+        if (kKeys == 64 || BIAS || !fast) mx = max32(x + 32, max32(x, mx));
+        if constexpr (kKeys == 128) mx = max32(x + 96, max32(x + 64, mx));
+        mx = mx * f + add;
         const float m_new = fmaxf(m_run, mx);
         const float m_use = (m_run == -INFINITY || m_new - m_run > kRescaleLog2) ? m_new : m_run;
-        const float corr = (m_run == -INFINITY || m_use == m_run) ? 1.f : ex2(m_run - m_use);
+        corr = (m_run == -INFINITY || m_use == m_run) ? 1.f : ex2(m_run - m_use);
         m_run = m_use;
-        const float nm1 = add - (m_use == -INFINITY ? 0.f : m_use);
-        const float2 nm = make_float2(nm1, nm1), f2 = make_float2(f, f);
-        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t pk[kKeys / 2];
-#pragma unroll
-        for (int e = 0; e < kKeys / 2; ++e) {
-          const float2 y = ffma2(make_float2(x[2 * e], x[2 * e + 1]), f2, nm);
-          const float2 q = make_float2(ex2(y.x), ex2(y.y));
-          sum2[e & 1] = fadd2(sum2[e & 1], q);
-          pk[e] = pack2<ET>(q.x, q.y);
-        }
-        tc::tmem_st16_nowait(t_s, pk);
-        if (nch > 1) tc::tmem_st16_nowait(t_s + 16, pk + 16);
-        const float2 ss = fadd2(sum2[0], sum2[1]);
-        l_run = l_run * corr + (ss.x + ss.y);
-        tc::tmem_wait_st();
-        // rescale the running output rows once P V of the block before has completed
-        if (c > 0 && __any_sync(MN_FULL_MASK, corr != 1.f)) {
+        // rescale the running output rows, at rest once P V of the block before has completed
+        if (__builtin_expect(c > 0 && __any_sync(MN_FULL_MASK, corr != 1.f), 0)) {
           if (!(ok = pv_done(c - 1))) break;
           tc::fence_after_sync();
           float o[32];
@@ -336,9 +363,30 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
           }
         }
       }
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tma::arrive(bars + F::bP + i * NS + buf);
+      const float nm1 = add - (m_run == -INFINITY ? 0.f : m_run);
+      const float2 nm = make_float2(nm1, nm1), f2 = make_float2(f, f);
+      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int part = 0; part < F::kParts; ++part) {
+        if (live) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float2 y = ffma2(make_float2(x[part * 64 + 2 * e], x[part * 64 + 2 * e + 1]), f2, nm);
+            const float2 q = make_float2(ex2(y.x), ex2(y.y));
+            sum2[e & 1] = fadd2(sum2[e & 1], q);
+            pk[e] = pack2<ET>(q.x, q.y);
+          }
+          tc::tmem_st16_nowait(t_s + part * 32, pk);
+          tc::tmem_st16_nowait(t_s + part * 32 + 16, pk + 16);
+          tc::tmem_wait_st();
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tma::arrive(bars + F::bP + (i * NS + buf) * F::kParts + part);
+      }
+      const float2 ss = fadd2(sum2[0], sum2[1]);
+      l_run = l_run * corr + (ss.x + ss.y);
     }
     if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
     if (ok && c > 0) {
@@ -475,8 +523,8 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   CUtensorMap mq, mk, mv;
   if (!bind_context()) return false;
   if (!map_q(&mq, bf16, a->q, a->q_st, a->q_sh, a->tq, a->heads, a->kv_heads, a->head_dim, pl.ntok)) return false;
-  if (!map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, kKeys)) return false;
-  if (!map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, kKeys)) return false;
+  if (!map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, F::KB)) return false;
+  if (!map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, F::KB)) return false;
   FwdParams p;
   p.a = *a;
   p.group = a->heads / a->kv_heads;
@@ -494,7 +542,7 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   p.err = err;
   const size_t smem = F::bytes(p.span * p.group);
   auto kern = forward_kernel<ET, DT, BIAS, SPLIT>;
-  if (!ensure_smem(kern, smem)) return false;
+  if (!ensure_smem(kern, smem) || !launch_regs(kern, F::kLaunchRegs)) return false;
   const int64_t slots = tile_slots(a->tq, a->nseq, SPLIT ? pl.ntok : F::NQ * pl.ntok) * a->kv_heads;
   if (slots > 0x7fffffff) return false;
   kern<<<dim3((unsigned)slots, pl.splits), F::kThreads, smem, st>>>(mq, mk, mv, p, bo);

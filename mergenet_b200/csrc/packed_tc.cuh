@@ -106,6 +106,15 @@ __device__ __forceinline__ bool elect_one() {
   return is != 0;
 }
 
+// Register exchange between the warp groups of a CTA (a whole group executes
+// it).  A taker waits until the givers' registers are free, so the shares may
+// not exceed what the CTA was launched with: launch_regs() on the host checks
+// the launch, a static_assert at each kernel the shares.
+template <int N>
+__device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // Tiles of `m` rows of every sequence share one index space without a prefix
 // sum: sequence b's tiles begin at slot cu[b] / m + b.  A sequence of L rows
 // has ceil(L / m) tiles and at least that many slots, at most one of them
@@ -209,6 +218,24 @@ inline bool map_k(CUtensorMap* map, bool bf16, const void* p, int64_t st, int64_
 inline bool rows_ok(const void* p, int64_t st, int64_t sh, int rows, int heads) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || (st > 0 && st % 8 == 0)) &&
          (heads <= 1 || (sh > 0 && sh % 8 == 0)) && st < (int64_t(1) << 38) && sh < (int64_t(1) << 31);
+}
+// The kernel was compiled to launch with at least `regs` registers a thread.
+template <typename F>
+inline bool launch_regs(F* func, int regs) {
+  static std::mutex mu;
+  static std::map<const void*, int> known;
+  const void* key = reinterpret_cast<const void*>(func);
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = known.find(key);
+  if (it == known.end()) {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, func) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    it = known.emplace(key, at.numRegs).first;
+  }
+  return it->second >= regs;
 }
 inline int sm_count() {
   int dev = 0, sms = 148;
