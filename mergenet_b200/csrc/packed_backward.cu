@@ -24,12 +24,6 @@
 namespace mn {
 namespace pk {
 
-constexpr int kBwdThreads = 320;  // warps 0-7 compute, 8 MMAs, 9 loads
-
-#ifndef MN_PK_BWD_POLY_PAIRS
-#define MN_PK_BWD_POLY_PAIRS 4  // of every 16 probability pairs, this many take the FMA-pipe exp2
-#endif
-
 struct BwdParams {
   mn_packed_args a;
   int group, ntok;
@@ -44,27 +38,14 @@ struct BiasSmem {
   uint8_t* idx;  // [span]
   float* tab;    // [group][buckets], log2 units
 };
-__device__ __forceinline__ void fill_bias(const BwdParams& p, const Borders& bo, int hk, const BiasSmem& s) {
-  for (int i = threadIdx.x; i < p.span; i += kBwdThreads) s.idx[i] = (uint8_t)bucket_of(bo, i - p.reach);
-  for (int i = threadIdx.x; i < p.group * p.a.buckets; i += kBwdThreads) {
+__device__ __forceinline__ void fill_bias(const BwdParams& p, const Borders& bo, int hk, const BiasSmem& s, int threads) {
+  for (int i = threadIdx.x; i < p.span; i += threads) s.idx[i] = (uint8_t)bucket_of(bo, i - p.reach);
+  for (int i = threadIdx.x; i < p.group * p.a.buckets; i += threads) {
     const int g = i / p.a.buckets, u = i % p.a.buckets;
     s.tab[i] = load_any(p.a.bias_table, p.a.bias_dtype, (int64_t)u * p.a.heads + hk * p.group + g) * kLog2e;
   }
 }
 
-// p = 2^y for 32 values; MASKED: y of hidden keys is -inf and gives 0
-template <bool MASKED>
-__device__ __forceinline__ void exp32(float* y) {
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float2 v = make_float2(y[2 * e], y[2 * e + 1]);
-    const float2 q = (!MASKED && MN_PK_BWD_POLY_PAIRS > 0 && (e * MN_PK_BWD_POLY_PAIRS) % 16 >= 16 - MN_PK_BWD_POLY_PAIRS)
-                         ? ex2_poly2(v)
-                         : make_float2(ex2(v.x), ex2(v.y));
-    y[2 * e] = q.x;
-    y[2 * e + 1] = q.y;
-  }
-}
 template <typename ET>
 __device__ __forceinline__ void put32(uint32_t taddr, const float* v) {
   uint32_t w[16];
@@ -72,13 +53,17 @@ __device__ __forceinline__ void put32(uint32_t taddr, const float* v) {
   for (int e = 0; e < 16; ++e) w[e] = pack2<ET>(v[2 * e], v[2 * e + 1]);
   tc::tmem_st16_nowait(taddr, w);
 }
-// left operand in tensor memory: columns 0-63 packed at +0, 64-127 at +64, so
-// that each half overwrites only what its own warps have read
-__device__ __forceinline__ uint32_t left_cols(int kk) { return (uint32_t)((kk & 3) * 8 + (kk >> 2) * 64); }
+// left operand in tensor memory: the columns of each of a row's threads packed
+// over the first half of their own, so that it overwrites only what that thread
+// has read; the column of K step kk (16 columns of scores)
+template <int CW>
+__device__ __forceinline__ uint32_t left_cols(int kk) { return (uint32_t)(kk * 16 / CW * CW + kk * 16 % CW / 2); }
 
 // ----------------------------------------------------------------------- dq
 template <int DT, bool BIAS>
 struct Dq {
+  static constexpr int W = BIAS ? 2 : 4;  // threads to a row; the sums by bucket take shared memory for each
+  static constexpr int CW = 128 / W, kThreads = 32 * (4 * W + 2);
   static constexpr int HV = DT / 64;
   static constexpr uint32_t kTile = HV * kHalfBytes;
   static constexpr int KS = DT == 64 || !BIAS ? 3 : 2, VS = DT == 64 || !BIAS ? 2 : 1;
@@ -87,20 +72,20 @@ struct Dq {
                        bDone = bDS + 1, bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
   static constexpr uint32_t oDelta = oMisc + 16;             // [2][128] partial deltas
-  static constexpr uint32_t oHist = oDelta + 2 * 128 * 4;    // [2][buckets][128]
+  static constexpr uint32_t oHist = oDelta + 2 * 128 * 4;    // [W][buckets][128]
   static constexpr uint32_t bytes(int buckets, int group, int span) {
-    return oHist + (BIAS ? buckets * 1024 + ((buckets * group * 4 + 15) / 16) * 16 + span : 0) + 1024;
+    return oHist + (BIAS ? W * buckets * 512 + ((buckets * group * 4 + 15) / 16) * 16 + span : 0) + 1024;
   }
   static constexpr uint32_t cS = 0, cDP = 256, cDQ = 384;
 };
 
 template <typename ET, int DT, bool BIAS>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
               const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
               const __grid_constant__ BwdParams p, const __grid_constant__ Borders bo) {
   using C = Dq<DT, BIAS>;
-  constexpr int HV = C::HV, KS = C::KS, VS = C::VS;
+  constexpr int HV = C::HV, KS = C::KS, VS = C::VS, W = C::W, CW = C::CW;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
@@ -110,7 +95,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int hk = blockIdx.x % a.kv_heads, slot_id = blockIdx.x / a.kv_heads;
   float* hist = reinterpret_cast<float*>(base + C::oHist);
   BiasSmem bs;
-  bs.tab = reinterpret_cast<float*>(base + C::oHist + (BIAS ? a.buckets * 1024 : 0));
+  bs.tab = reinterpret_cast<float*>(base + C::oHist + (BIAS ? W * a.buckets * 512 : 0));
   bs.idx = reinterpret_cast<uint8_t*>(bs.tab) + (BIAS ? (a.buckets * G * 4 + 15) / 16 * 16 : 0);
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
@@ -119,7 +104,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (lane == 0) misc[1] = (uint32_t)b;
   }
   if (warp == 2 && lane == 0) {
-    for (int i = 0; i < C::kNumBars; ++i) tc::mbar_init(bars + i, i == C::bDS ? 8 : 1);
+    for (int i = 0; i < C::kNumBars; ++i) tc::mbar_init(bars + i, i == C::bDS ? 4 * W : 1);
     tc::fence_mbar_init();
   }
   if (warp == 3 && lane == 0) {
@@ -129,8 +114,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tma::prefetch_map(&tm_v);
   }
   if (BIAS) {
-    fill_bias(p, bo, hk, bs);
-    for (int i = tid; i < 2 * a.buckets * 128; i += kBwdThreads) hist[i] = 0.f;
+    fill_bias(p, bo, hk, bs, C::kThreads);
+    for (int i = tid; i < W * a.buckets * 128; i += C::kThreads) hist[i] = 0.f;
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -149,7 +134,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   constexpr int ab_bf16 = std::is_same<ET, __nv_bfloat16>::value ? 1 : 0;
   bool ok = true;
 
-  if (warp == 9) {
+  if (warp == 4 * W + 1) {
     // ---------------------------------------------------------------- loads
     if (lane == 0 && n > 0) {
       tma::expect_tx(bars + C::bQ, 2u * HV * 128u * (uint32_t)(G * p.ntok));
@@ -178,7 +163,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int j = max(0, nv - VS); j < nv; ++j) wait(bars + C::bVF + j % VS, (j / VS) & 1, nullptr);
     }
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == 4 * W) {
     // ----------------------------------------------------------------- MMAs
     // S runs one block ahead of dP: at ds(j), dP(j + 1), dQ += ds(j) K(j) and
     // S(j + 2) are issued while the compute warps turn S(j + 1) into p
@@ -216,8 +201,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int cols = cols_of(j);
       if (s.nk - j * 128 < cols) zero_rows(v, s.nk - j * 128, cols, HV);  // 0 (dP - delta) must not meet a NaN
       scores(tmem + C::cDP, base + C::oDO, v, cols, bars + C::bDP);
-      if (elect_one()) tc::mma_commit(bars + C::bVE + vs);
-      __syncwarp();
       return true;
     };
     if (n > 0) {
@@ -233,7 +216,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             if (kk * 16 < cols)
-              tc::mma_f16_ts(tmem + C::cDQ, tmem + C::cS + (j & 1) * 128 + left_cols(kk), dk + 128 * kk, idesc_q,
+              tc::mma_f16_ts(tmem + C::cDQ, tmem + C::cS + (j & 1) * 128 + left_cols<CW>(kk), dk + 128 * kk, idesc_q,
                              (j > 0 || kk > 0) ? 1u : 0u);
           tc::mma_commit(bars + C::bKE + j % KS);
           if (j == n - 1) tc::mma_commit(bars + C::bDone);
@@ -250,7 +233,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     __syncwarp();
   } else {
     // -------------------------------------------------------------- compute
-    const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // column half, row
+    const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // part of the columns, row
     const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
     const int my = t0 + r / G, g = r % G;
     const bool mine = present && r < G * p.ntok && my < s.nq;
@@ -260,14 +243,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int pmin = __reduce_min_sync(MN_FULL_MASK, mine ? pos : 0x7fffffff);
     const int pmax = __reduce_max_sync(MN_FULL_MASK, mine ? pos : -0x7fffffff);
     const int64_t row = (int64_t)(s.q0 + my) * G + g, rows = (int64_t)a.tq * G;
-    // delta = dout . out, the channels in 8s alternating between the row's two threads
+    // delta = dout . out, the channels in 8s in turn to the row's threads
     float* dl = reinterpret_cast<float*>(base + C::oDelta);
     {
       float acc = 0.f;
       if (mine) {
         const ET* x = static_cast<const ET*>(a.dout) + (int64_t)(s.q0 + my) * a.do_st + (hk * G + g) * a.do_sh;
         const ET* y = static_cast<const ET*>(a.out) + ((int64_t)(s.q0 + my) * a.heads + hk * G + g) * a.head_dim;
-        for (int c = w; c < a.head_dim / 8; c += 2) {
+        for (int c = w; c < a.head_dim / 8; c += W) {
           const uint4 xv = *reinterpret_cast<const uint4*>(x + c * 8), yv = *reinterpret_cast<const uint4*>(y + c * 8);
           const ET* xe = reinterpret_cast<const ET*>(&xv);
           const ET* ye = reinterpret_cast<const ET*>(&yv);
@@ -275,9 +258,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           for (int e = 0; e < 8; ++e) acc = fmaf(to_f32(xe[e]), to_f32(ye[e]), acc);
         }
       }
-      dl[w * 128 + r] = acc;
+      auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(128 * W) : "memory"); };
+      if (W == 4) {  // room for two partial sums a row
+        if (w >= 2) dl[(w - 2) * 128 + r] = acc;
+        sync();
+        if (w < 2) acc += dl[w * 128 + r];
+        sync();
+      }
+      if (w < 2) dl[w * 128 + r] = acc;
+      sync();
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
     const float delta = dl[r] + dl[128 + r];
     if (mine && w == 0) p.delta[hk * rows + row] = delta;
     const float nlse = mine ? -a.lse[hk * rows + row] : -INFINITY;
@@ -286,53 +276,51 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     float* my_hist = hist + (BIAS ? w * a.buckets * 128 + r : 0);
     float far_lo = 0.f, far_hi = 0.f;
     for (int j = 0; j < n && ok; ++j) {
-      const int k0 = j * 128 + w * 64;  // this half's first key
-      const int chunks = max(0, min(2, (min(128, (s.nk - j * 128 + 31) & ~31) - w * 64) >> 5));
-      const uint32_t t_s = tmem + C::cS + (j & 1) * 128 + w * 64 + lane_sel, t_dp = tmem + C::cDP + w * 64 + lane_sel;
+      const int k0 = j * 128 + w * CW;  // this thread's first key
+      const int chunks = max(0, min(CW / 32, (min(128, (s.nk - j * 128 + 31) & ~31) - w * CW) >> 5));
+      const uint32_t t_s = tmem + C::cS + (j & 1) * 128 + w * CW + lane_sel, t_dp = tmem + C::cDP + w * CW + lane_sel;
       if (!(ok = wait(bars + C::bS + (j & 1), (j >> 1) & 1, p.err))) break;
       tc::fence_after_sync();
-      float x[64];
+      float x[CW];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < CW / 32; ++u)
         if (u < chunks) tc::tmem_ld32_nowait(t_s + u * 32, x + u * 32);
-      tc::tmem_ld_wait<64>(x);
-      const bool masked = kmin < k0 + 64;
+      tc::tmem_ld_wait<CW>(x);
+      const bool masked = kmin < k0 + CW;
       int kind = 0;  // bias: 1 all below the reach, 2 all above, 3 mixed
       float add = nlse;
       if (BIAS) {
-        kind = k0 + 63 - pmin <= -p.reach ? 1 : k0 - pmax >= p.span - 1 - p.reach ? 2 : 3;
+        kind = k0 + CW - 1 - pmin <= -p.reach ? 1 : k0 - pmax >= p.span - 1 - p.reach ? 2 : 3;
         if (kind == 1) add += tab[bs.idx[0]];
         if (kind == 2) add += tab[bs.idx[p.span - 1]];
       }
       const int at = k0 - pos + p.reach;
       if (BIAS && kind == 3) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
+        for (int e = 0; e < CW; ++e)
           if (e / 32 < chunks) x[e] = fmaf(x[e], sl2, tab[bs.idx[min(max(at + e, 0), p.span - 1)]] + add);
       } else {
         const float2 f2 = make_float2(sl2, sl2), a2 = make_float2(add, add);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < CW / 2; ++e) {
           const float2 y = ffma2(make_float2(x[2 * e], x[2 * e + 1]), f2, a2);
           x[2 * e] = y.x;
           x[2 * e + 1] = y.y;
         }
       }
-      if (masked) {
+      if (__builtin_expect(masked, 0)) {  // hidden keys get exactly 0
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
+        for (int e = 0; e < CW; ++e)
           if (k0 + e >= klim) x[e] = -INFINITY;
-        exp32<true>(x);
-        exp32<true>(x + 32);
-      } else {
-        exp32<false>(x);
-        exp32<false>(x + 32);
       }
+#pragma unroll
+      for (int e = 0; e < CW; ++e) x[e] = ex2(x[e]);
       if (!(ok = wait(bars + C::bDP, j & 1, p.err))) break;
+      if (tid == 0) tma::arrive(bars + C::bVE + j % VS);  // dP has read V (a commit would cost the MMA warp 200 cycles)
       tc::fence_after_sync();
       const float2 nd = make_float2(-delta, -delta);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < CW / 32; ++u) {
         if (u >= chunks) break;
         float d[32];
         tc::tmem_ld32_nowait(t_dp + u * 32, d);
@@ -355,7 +343,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           int cur = bs.idx[min(max(at, 0), p.span - 1)];
           float acc = 0.f;
 #pragma unroll
-          for (int e = 0; e < 64; ++e) {
+          for (int e = 0; e < CW; ++e) {
             if (e / 32 >= chunks) break;
             const int u = bs.idx[min(max(at + e, 0), p.span - 1)];
             if (u != cur) {
@@ -369,7 +357,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         } else {
           float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
+          for (int e = 0; e < CW / 2; ++e)
             if (e / 16 < chunks) acc = fadd2(acc, make_float2(x[2 * e], x[2 * e + 1]));
           if (kind == 1) far_lo += acc.x + acc.y;
           else far_hi += acc.x + acc.y;
@@ -384,8 +372,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (ok) {
       ET* dst = static_cast<ET*>(a.dq) + ((int64_t)(s.q0 + my) * a.heads + hk * G + g) * a.head_dim;
 #pragma unroll
-      for (int u = 0; u < DT / 64; ++u) {
-        const int c0 = (w * (DT / 64) + u) * 32;
+      for (int u = w; u < DT / 32; u += W) {
+        const int c0 = u * 32;
         float o[32];
         if (n > 0) {
           tc::tmem_ld32(tmem + C::cDQ + c0 + lane_sel, o);
@@ -402,13 +390,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         my_hist[bs.idx[0] * 128] += far_lo;
         my_hist[bs.idx[p.span - 1] * 128] += far_hi;
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(128 * W) : "memory");
       const int per = a.buckets * G;
       const int64_t slots = gridDim.x / a.kv_heads;
-      for (int i = tid; i < per; i += 256) {
+      for (int i = tid; i < per; i += 128 * W) {
         const int u = i / G, gg = i % G;
         float acc = 0.f;
-        for (int rr = gg; rr < 128; rr += G) acc += hist[u * 128 + rr] + hist[(a.buckets + u) * 128 + rr];
+        for (int rr = gg; rr < 128; rr += G)
+#pragma unroll
+          for (int ww = 0; ww < W; ++ww) acc += hist[(ww * a.buckets + u) * 128 + rr];
         p.part[(hk * slots + slot_id) * per + i] = acc;
       }
     }
@@ -435,6 +425,7 @@ __global__ void __launch_bounds__(128) dbias_kernel(int heads, int group, int bu
 // ------------------------------------------------------------------- dk, dv
 template <int DT, bool BIAS>
 struct Dkv {
+  static constexpr int W = 4, CW = 128 / W, kThreads = 32 * (4 * W + 2);
   static constexpr int HV = DT / 64;
   static constexpr uint32_t kTile = HV * kHalfBytes;
   static constexpr int NS = DT == 64 ? 2 : 1;  // S^T buffers in tensor memory
@@ -453,12 +444,12 @@ struct Dkv {
 };
 
 template <typename ET, int DT, bool BIAS>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
     dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const __grid_constant__ BwdParams p, const __grid_constant__ Borders bo) {
   using C = Dkv<DT, BIAS>;
-  constexpr int HV = C::HV, NS = C::NS, QS = C::QS;
+  constexpr int HV = C::HV, NS = C::NS, QS = C::QS, W = C::W, CW = C::CW;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
@@ -478,7 +469,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   }
   if (warp == 2 && lane == 0) {
     for (int i = 0; i < C::kNumBars; ++i)
-      tc::mbar_init(bars + i, i >= C::bF && i < C::bE ? 2 : (i >= C::bP && i < C::bDP) || i == C::bDS ? 8 : 1);
+      tc::mbar_init(bars + i, i >= C::bF && i < C::bE ? 2 : (i >= C::bP && i < C::bDP) || i == C::bDS ? 4 * W : 1);
     tc::fence_mbar_init();
   }
   if (warp == 3 && lane == 0) {
@@ -488,7 +479,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tma::prefetch_map(&tm_v);
   }
   if (BIAS) {
-    fill_bias(p, bo, hk, bs);
+    fill_bias(p, bo, hk, bs, C::kThreads);
     if (tid < 128) col[tid] = make_int2(tid / G, (tid % G) * a.buckets);
   }
   tc::fence_before_sync();
@@ -511,7 +502,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   };
   bool ok = true;
 
-  if (warp == 9) {
+  if (warp == 4 * W + 1) {
     // ---------------------------------------------------------------- loads
     if (n > 0) {
       if (lane == 0) {
@@ -564,7 +555,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == 4 * W) {
     // ----------------------------------------------------------------- MMAs
     // While the compute warps turn S(i) into p the tensor core finishes
     // dK += ds(i - 1) Q and dP(i); while they form ds(i), dV += p(i) dout and
@@ -598,7 +589,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), kHalfBytes);
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk)
-        tc::mma_f16_ts(d, left + left_cols(kk), dx + 128 * kk, idesc_g, (more || kk > 0) ? 1u : 0u);
+        tc::mma_f16_ts(d, left + left_cols<CW>(kk), dx + 128 * kk, idesc_g, (more || kk > 0) ? 1u : 0u);
     };
     if (n > 0) {
       ok = wait(bars + C::bKV, 0, p.err);
@@ -632,77 +623,65 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     __syncwarp();
   } else {
     // -------------------------------------------------------------- compute
-    const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // column half, key row
+    const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // part of the columns, key row
     const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
     const int key = k0 + r;
     const float sl2 = a.scale * kLog2e;
     for (int i = 0; i < n && ok; ++i) {
       const int st = i % QS, t0 = (i0 + i) * p.ntok;
-      const uint32_t t_s = tmem + C::cS + (i % NS) * 128 + w * 64 + lane_sel, t_dp = tmem + C::cDP + w * 64 + lane_sel;
-      const float* nl = reinterpret_cast<const float*>(base + C::oRows) + st * 256 + w * 64;
+      const uint32_t t_s = tmem + C::cS + (i % NS) * 128 + w * CW + lane_sel, t_dp = tmem + C::cDP + w * CW + lane_sel;
+      const float* nl = reinterpret_cast<const float*>(base + C::oRows) + st * 256 + w * CW;
       // columns from here on see this key; the warp's last key sees the latest start
-      const int c0 = a.causal ? (key - shift - t0) * G - w * 64 : 0;
-      const bool masked = a.causal && (k0 + ((warp & 3) * 32 + 31) - shift - t0) * G > w * 64;
+      const int c0 = a.causal ? (key - shift - t0) * G - w * CW : 0;
+      const bool masked = a.causal && (k0 + ((warp & 3) * 32 + 31) - shift - t0) * G > w * CW;
       if (!(ok = wait(bars + C::bF + st, (i / QS) & 1, p.err))) break;  // lse and delta are there
       if (!(ok = wait(bars + C::bS + i % NS, (i / NS) & 1, p.err))) break;
       tc::fence_after_sync();
-      float x[64];
+      float x[CW];
       tc::tmem_ld32_nowait(t_s, x);
-      tc::tmem_ld32_nowait(t_s + 32, x + 32);
-      tc::tmem_ld_wait<64>(x);
+      tc::tmem_ld_wait<CW>(x);
       if (BIAS && kind_of(t0) == 3) {
         const int at = key - t0 - shift + p.reach;
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          const int2 c = col[w * 64 + e];
+        for (int e = 0; e < CW; ++e) {
+          const int2 c = col[w * CW + e];
           x[e] = fmaf(x[e], sl2, nl[e] + bs.tab[c.y + bs.idx[min(max(at - c.x, 0), p.span - 1)]]);
         }
       } else {
         const float2 f2 = make_float2(sl2, sl2);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < CW / 4; ++e) {
           const float4 l = reinterpret_cast<const float4*>(nl)[e];
           const float2 y0 = ffma2(make_float2(x[4 * e], x[4 * e + 1]), f2, make_float2(l.x, l.y));
           const float2 y1 = ffma2(make_float2(x[4 * e + 2], x[4 * e + 3]), f2, make_float2(l.z, l.w));
           x[4 * e] = y0.x; x[4 * e + 1] = y0.y; x[4 * e + 2] = y1.x; x[4 * e + 3] = y1.y;
         }
       }
-      const bool tail = min(p.ntok, s.nq - t0) * G < 128;  // columns of no query: exactly 0
-      if (masked || tail) {
-        if (masked) {
+      if (__builtin_expect(masked, 0)) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e < c0) x[e] = -INFINITY;
-        }
-        exp32<true>(x);
-        exp32<true>(x + 32);
-      } else {
-        exp32<false>(x);
-        exp32<false>(x + 32);
+        for (int e = 0; e < CW; ++e)
+          if (e < c0) x[e] = -INFINITY;
       }
+#pragma unroll
+      for (int e = 0; e < CW; ++e) x[e] = ex2(x[e]);  // hidden keys and columns of no query: exactly 0
       put32<ET>(t_s, x);
-      put32<ET>(t_s + 16, x + 32);
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tma::arrive(bars + C::bP + i % NS);
       if (!(ok = wait(bars + C::bDP, i & 1, p.err))) break;
       tc::fence_after_sync();
+      float d[CW];
+      tc::tmem_ld32_nowait(t_dp, d);
+      tc::tmem_ld_wait<CW>(d);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float d[32];
-        tc::tmem_ld32_nowait(t_dp + u * 32, d);
-        tc::tmem_ld_wait<32>(d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 nd = reinterpret_cast<const float4*>(nl + 128)[u * 8 + e];
-          const int c = u * 32 + 4 * e;
-          const float2 y0 = fmul2(make_float2(x[c], x[c + 1]), fadd2(make_float2(d[4 * e], d[4 * e + 1]), make_float2(nd.x, nd.y)));
-          const float2 y1 = fmul2(make_float2(x[c + 2], x[c + 3]), fadd2(make_float2(d[4 * e + 2], d[4 * e + 3]), make_float2(nd.z, nd.w)));
-          d[4 * e] = y0.x; d[4 * e + 1] = y0.y; d[4 * e + 2] = y1.x; d[4 * e + 3] = y1.y;
-        }
-        put32<ET>(t_dp + u * 16, d);
+      for (int e = 0; e < CW / 4; ++e) {
+        const float4 nd = reinterpret_cast<const float4*>(nl + 128)[e];
+        const float2 y0 = fmul2(make_float2(x[4 * e], x[4 * e + 1]), fadd2(make_float2(d[4 * e], d[4 * e + 1]), make_float2(nd.x, nd.y)));
+        const float2 y1 = fmul2(make_float2(x[4 * e + 2], x[4 * e + 3]), fadd2(make_float2(d[4 * e + 2], d[4 * e + 3]), make_float2(nd.z, nd.w)));
+        d[4 * e] = y0.x; d[4 * e + 1] = y0.y; d[4 * e + 2] = y1.x; d[4 * e + 3] = y1.y;
       }
+      put32<ET>(t_dp, d);
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
@@ -714,19 +693,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc::fence_after_sync();
     }
     if (ok) {
-      // the first half's warps store dV, the second's dK
       const bool mine = present && key < s.slot;
-      const float f = key < s.nk ? (w == 0 ? 1.f : a.scale) : 0.f;
-      ET* dst = static_cast<ET*>(w == 0 ? a.dv : a.dk) + ((int64_t)(s.k0 + key) * a.kv_heads + hk) * a.head_dim;
 #pragma unroll
-      for (int u = 0; u < DT / 32; ++u) {
+      for (int q = w; q < DT / 16; q += W) {  // chunks of dV, then of dK
+        const bool is_v = q < DT / 32;
+        const int c0 = (is_v ? q : q - DT / 32) * 32;
         float o[32];
-        if (n > 0) tc::tmem_ld32(tmem + (w == 0 ? C::cDV : C::cDK) + u * 32 + lane_sel, o);
+        if (n > 0) tc::tmem_ld32(tmem + (is_v ? C::cDV : C::cDK) + c0 + lane_sel, o);
         if (n == 0 || key >= s.nk) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
         }
-        if (mine) store32<ET>(dst, u * 32, a.head_dim, o, f);
+        if (mine)
+          store32<ET>(static_cast<ET*>(is_v ? a.dv : a.dk) + ((int64_t)(s.k0 + key) * a.kv_heads + hk) * a.head_dim, c0, a.head_dim,
+                      o, is_v ? 1.f : a.scale);
         __syncwarp();
       }
     }
@@ -783,8 +763,8 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
   auto kkv = dkv_kernel<ET, DT, BIAS>;
   const size_t sq = Dq<DT, BIAS>::bytes(a->buckets, p.group, p.span), skv = Dkv<DT, BIAS>::bytes(a->buckets, p.group, p.span);
   if (!ensure_smem(kq, sq) || !ensure_smem(kkv, skv)) return false;
-  kq<<<(unsigned)(z.q_slots * a->kv_heads), kBwdThreads, sq, st>>>(mq, mdo, mk, mv, p, bo);
-  if (a->tk > 0) kkv<<<(unsigned)(z.k_slots * a->kv_heads), kBwdThreads, skv, st>>>(mq, mdo, mk, mv, p, bo);
+  kq<<<(unsigned)(z.q_slots * a->kv_heads), Dq<DT, BIAS>::kThreads, sq, st>>>(mq, mdo, mk, mv, p, bo);
+  if (a->tk > 0) kkv<<<(unsigned)(z.k_slots * a->kv_heads), Dkv<DT, BIAS>::kThreads, skv, st>>>(mq, mdo, mk, mv, p, bo);
   if (BIAS)
     dbias_kernel<<<dim3(a->buckets * p.group, a->kv_heads), 128, 0, st>>>(a->heads, p.group, a->buckets, (int)z.q_slots, p.part,
                                                                          a->dbias, a->bias_dtype);

@@ -32,12 +32,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -50,26 +44,6 @@ __device__ __forceinline__ float max32(const float* x, float m) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = max3(a[i], x[e + 2 * i], x[e + 2 * i + 1]);
   return fmaxf(max3(a[0], a[1], a[2]), a[3]);
-}
-
-// 2^y for a pair of y <= 8 on the FMA pipe (the polynomial of
-// csrc/exp2_fit.py, relative error 2.7e-6): y = n + f with n the nearest
-// integer.  y + 1.5 * 2^23 holds n in its low bits, and shifting it left by 23
-// leaves n in the exponent's place and nothing else.  y is clamped at -126,
-// NaN kept, so it serves unmasked scores only: 2^-126 in the place of less.
-__device__ __forceinline__ float2 ex2_poly2(float2 y) {
-  y.x = max_nan(y.x, -126.f);
-  y.y = max_nan(y.y, -126.f);
-  const float2 t = fadd2(y, make_float2(12582912.f, 12582912.f));
-  const float2 n = fadd2(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = ffma2(n, make_float2(-1.f, -1.f), y);
-  float2 p = ffma2(f, make_float2(9.570100344717503e-03f, 9.570100344717503e-03f),
-                   make_float2(5.591786280274391e-02f, 5.591786280274391e-02f));
-  p = ffma2(p, f, make_float2(2.402474433183670e-01f, 2.402474433183670e-01f));
-  p = ffma2(p, f, make_float2(6.931217908859253e-01f, 6.931217908859253e-01f));
-  p = ffma2(p, f, make_float2(9.999992847442627e-01f, 9.999992847442627e-01f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (int)((uint32_t)__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (int)((uint32_t)__float_as_int(t.y) << 23)));
 }
 
 // Wait for the phase with the given parity, bounded in time like
