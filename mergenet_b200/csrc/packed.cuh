@@ -47,28 +47,6 @@ struct Seq {
   int q0, nq, k0, nk, slot;
 };
 
-__device__ __forceinline__ Seq load_seq(const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, int b, int tq,
-                                        int tk) {
-  Seq s;
-  s.q0 = min(max(cu_q[b], 0), tq);
-  s.nq = min(max(cu_q[b + 1], s.q0), tq) - s.q0;
-  s.k0 = min(max(cu_k[b], 0), tk);
-  s.slot = min(max(cu_k[b + 1], s.k0), tk) - s.k0;
-  s.nk = len_k ? min(max(len_k[b], 0), s.slot) : s.slot;
-  return s;
-}
-
-// Index of the sequence that holds `row` by the ends cu[1..n], or n.
-__device__ __forceinline__ int seq_of_row(const int32_t* cu, int n, int row) {
-  int lo = 0, hi = n;  // first b with cu[b + 1] > row
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid + 1] > row) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
-}
-
 // Data condition of the offsets, looked at by one thread block.
 __device__ __forceinline__ bool bad_lengths(const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, int n, int tq,
                                             int tk, int first, int step) {

@@ -71,7 +71,7 @@ struct Dq {
   static constexpr int bQ = 0, bKF = 1, bKE = bKF + KS, bVF = bKE + KS, bVE = bVF + VS, bS = bVE + VS, bDP = bS + 2, bDS = bDP + 1,
                        bDone = bDS + 1, bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
-  static constexpr uint32_t oDelta = oMisc + 16;             // [2][128] partial deltas
+  static constexpr uint32_t oDelta = oMisc + 32;             // [2][128] partial deltas
   static constexpr uint32_t oHist = oDelta + 2 * 128 * 4;    // [W][buckets][128]
   static constexpr uint32_t bytes(int buckets, int group, int span) {
     return oHist + (BIAS ? W * buckets * 512 + ((buckets * group * 4 + 15) / 16) * 16 + span : 0) + 1024;
@@ -100,8 +100,7 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
   if (warp == 1) {
-    const int b = seq_of_slot(a.cu_q, a.nseq, p.ntok, a.tq, slot_id);
-    if (lane == 0) misc[1] = (uint32_t)b;
+    put_found(misc + 1, seq_of_slot<false>(a, p.ntok, slot_id));
   }
   if (warp == 2 && lane == 0) {
     for (int i = 0; i < C::kNumBars; ++i) tc::mbar_init(bars + i, i == C::bDS ? 4 * W : 1);
@@ -121,10 +120,9 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = misc[0];
-  const int b = (int)misc[1];
-  const Seq s = load_seq_or_tail(a, b);
-  const int tiles = (s.nq + p.ntok - 1) / p.ntok;
-  const int local = slot_id - slot_of_seq(a.cu_q, b, p.ntok, a.tq);
+  const Found found = get_found(misc + 1);
+  const Seq& s = found.s;
+  const int tiles = (s.nq + p.ntok - 1) / p.ntok, local = found.local;
   const bool present = local >= 0 && local < tiles;
   const int t0 = present ? (a.causal ? tiles - 1 - local : local) * p.ntok : 0;
   const int shift = s.nk - s.nq;
@@ -435,7 +433,7 @@ struct Dkv {
   static constexpr int bKV = 0, bF = 1, bE = bF + QS, bS = bE + QS, bP = bS + NS, bDP = bP + NS, bDS = bDP + 1, bDone = bDS + 1,
                        bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
-  static constexpr uint32_t oCol = oMisc + 16;  // [128] (token, head * buckets) of a column
+  static constexpr uint32_t oCol = oMisc + 32;  // [128] (token, head * buckets) of a column
   static constexpr uint32_t oTab = oCol + 128 * 8;
   static constexpr uint32_t bytes(int buckets, int group, int span) {
     return oTab + (BIAS ? ((buckets * group * 4 + 15) / 16) * 16 + span : 0) + 1024;
@@ -464,8 +462,7 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
   if (warp == 1) {
-    const int b = seq_of_slot(a.cu_k, a.nseq, 128, a.tk, slot_id);
-    if (lane == 0) misc[1] = (uint32_t)b;
+    put_found(misc + 1, seq_of_slot<true>(a, 128, slot_id));
   }
   if (warp == 2 && lane == 0) {
     for (int i = 0; i < C::kNumBars; ++i)
@@ -486,10 +483,9 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = misc[0];
-  const int b = (int)misc[1];
-  const Seq s = load_seq_or_tail(a, b);
-  const int local = slot_id - slot_of_seq(a.cu_k, b, 128, a.tk);
-  const int k0 = local * 128;
+  const Found found = get_found(misc + 1);
+  const Seq& s = found.s;
+  const int local = found.local, k0 = local * 128;
   const bool present = local >= 0 && k0 < s.slot;
   const int shift = s.nk - s.nq;
   // query tiles that see a key of this tile: [i0, i0 + n)

@@ -62,8 +62,8 @@ struct Fwd {
   static constexpr int kParts = KB / 64;
   static constexpr int bQ = 0, bFull = 1, bEmpty = bFull + kStages, bS = bEmpty + kStages, bP = bS + NQ * NS,
                        bPV = bP + NQ * NS * kParts, bDrain = bPV + NQ * NS, kNumBars = bDrain + 1;
-  static constexpr uint32_t kMisc = kBars + ((kNumBars * 8 + 15) / 16) * 16;  // TMEM base, sequence index
-  static constexpr uint32_t kLut = kMisc + 16;
+  static constexpr uint32_t kMisc = kBars + ((kNumBars * 8 + 15) / 16) * 16;  // TMEM base, sequence
+  static constexpr uint32_t kLut = kMisc + 32;
   static constexpr uint32_t bytes(uint32_t lut_floats) { return kLut + lut_floats * 4 + 1024; }
   // TMEM columns: the slots' S buffers, then their O
   static constexpr uint32_t kCols = DT == 64 ? 256 : 512, cO = NQ * NS * KB;
@@ -101,8 +101,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), F::kCols);
   if (warp == 1) {
-    const int b = seq_of_slot(a.cu_q, a.nseq, tile_tokens, a.tq, slot_id);
-    if (lane == 0) misc[1] = (uint32_t)b;
+    put_found(misc + 1, seq_of_slot<false>(a, tile_tokens, slot_id));
     if (blockIdx.x == 0 && blockIdx.y == 0 && p.err &&
         bad_lengths(a.cu_q, a.cu_k, a.len_k, a.nseq, a.tq, a.tk, lane, 32))
       atomicOr(p.err, MN_STATUS_BAD_LENGTHS);
@@ -126,10 +125,9 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = misc[0];
-  const int b = (int)misc[1];
-  const Seq s = load_seq_or_tail(a, b);
-  const int tiles = (s.nq + tile_tokens - 1) / tile_tokens;
-  const int local = slot_id - slot_of_seq(a.cu_q, b, tile_tokens, a.tq);
+  const Found found = get_found(misc + 1);
+  const Seq& s = found.s;
+  const int tiles = (s.nq + tile_tokens - 1) / tile_tokens, local = found.local;
   const bool present = local >= 0 && local < tiles;
   // the last tiles see the most keys under a causal mask: they go first
   const int t0 = present ? (a.causal ? tiles - 1 - local : local) * tile_tokens : 0;
@@ -436,37 +434,52 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
 }
 
 // out = sum over the parts of 2^(lse_i - max) out_i over the sum of those
-// weights, the parts in order; one warp a row.
+// weights; one block a row.  Its warps take the parts in turn and their sums
+// are added in order.
+constexpr int kJoinWarps = 8;
 template <typename ET>
-__global__ void __launch_bounds__(128) join_kernel(mn_packed_args a, int parts, const float* __restrict__ part_o,
-                                                   const float* __restrict__ part_lse) {
-  const int lane = threadIdx.x & 31, G = a.heads / a.kv_heads;
-  const int64_t rows = (int64_t)a.tq * G, all = rows * a.kv_heads;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= all) return;
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ mn_packed_args a, int parts,
+                                                               const float* __restrict__ part_o,
+                                                               const float* __restrict__ part_lse) {
+  __shared__ float4 sums[kJoinWarps][32];
+  __shared__ float totals[kJoinWarps];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5, G = a.heads / a.kv_heads;
+  const int64_t rows = (int64_t)a.tq * G, all = rows * a.kv_heads, at = blockIdx.x;
   float m = -INFINITY;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, part_lse[i * all + w]);
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, part_lse[i * all + at]);
   m = warp_max(m);
   const int c = lane * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float total = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float lse = part_lse[i * all + w];
-    if (lse == -INFINITY) continue;  // a part without keys wrote no output
-    const float f = m == -INFINITY ? 1.f : ex2(lse - m);  // NaN stays
+#pragma unroll 4
+  for (int i = w; i < parts; i += nw) {
+    const float lse = part_lse[i * all + at];
+    // a part without keys has no weight and wrote no output; NaN stays
+    const float f = lse == -INFINITY ? 0.f : m == -INFINITY ? 1.f : ex2(lse - m);
     total += f;
-    if (c < a.head_dim) {
-      const float4 o = *reinterpret_cast<const float4*>(part_o + (i * all + w) * a.head_dim + c);
+    if (c < a.head_dim && f != 0.f) {
+      const float4 o = *reinterpret_cast<const float4*>(part_o + (i * all + at) * a.head_dim + c);
       acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
     }
   }
-  const int hk = (int)(w / rows);
-  const int64_t row = w % rows, t = row / G, g = row % G;
+  if (nw > 1) {
+    sums[w][lane] = acc;
+    if (lane == 0) totals[w] = total;
+    __syncthreads();
+    if (w > 0) return;
+    for (int i = 1; i < nw; ++i) {
+      const float4 o = sums[i][lane];
+      acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+      total += totals[i];
+    }
+  }
+  const int hk = (int)(at / rows);
+  const int64_t row = at % rows, t = row / G, g = row % G;
   const float inv = total == 0.f ? 0.f : 1.f / total;
   if (c < a.head_dim)
     *reinterpret_cast<uint2*>(static_cast<ET*>(a.out) + (t * a.heads + hk * G + g) * a.head_dim + c) =
         make_uint2(pack2<ET>(acc.x * inv, acc.y * inv), pack2<ET>(acc.z * inv, acc.w * inv));
-  if (a.lse && lane == 0) a.lse[w] = total == 0.f ? INFINITY : m + log2f(total);
+  if (a.lse && lane == 0) a.lse[at] = total == 0.f ? INFINITY : m + log2f(total);
 }
 
 int check(const mn_packed_args* a, Borders* bo, bool backward) {
@@ -500,14 +513,23 @@ struct Plan {
 static Plan plan_of(const mn_packed_args* a) {
   const int g = a->heads / a->kv_heads, slots = a->head_dim <= 64 ? 1 : 2;
   Plan pl{128 / g, 0, 1};
-  // Tiles that have rows, at most; a call that leaves the card part empty and
-  // whose sequences are long on average is divided over the keys.
+  // Tiles that have rows, at most; a call that leaves the card part empty, or
+  // whose tiles are mostly empty rows, and whose sequences are long on average
+  // is divided over the keys.
   const int64_t tiles = ((int64_t)a->tq / pl.ntok + a->nseq) * a->kv_heads;
   const int64_t ctas = (int64_t)sm_count() * (slots == 1 ? 2 : 1);
   const int64_t blocks = a->tk / a->nseq / 128;
   if (blocks >= 4 && (tiles <= ctas || (int64_t)a->tq * g <= (int64_t)a->nseq * 64)) {
-    const int64_t want = std::max<int64_t>(1, (2 * ctas + tiles - 1) / tiles);
-    pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, blocks / (2 * slots)), 64));
+    // the division whose waves of CTAs end first; a CTA's start and end take
+    // it about as long as four blocks of 128 keys
+    double best = 0;
+    for (int64_t n = 1; n <= 64 && (n == 1 || n * 2 * slots <= blocks); ++n) {
+      const double cost = (double)((tiles * n + ctas - 1) / ctas) * ((double)blocks / n + 4);
+      if (n == 1 || cost < best) {
+        best = cost;
+        pl.splits = (int)n;
+      }
+    }
     if (pl.splits * slots > 1) pl.parts = pl.splits * slots;
   }
   return pl;
@@ -540,6 +562,7 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   p.part_o = static_cast<float*>(ws);
   p.part_lse = p.part_o + (size_t)pl.parts * a->tq * a->heads * a->head_dim;
   p.err = err;
+  if ((int64_t)a->tq * a->heads > 0x7fffffff) return false;
   const size_t smem = F::bytes(p.span * p.group);
   auto kern = forward_kernel<ET, DT, BIAS, SPLIT>;
   if (!ensure_smem(kern, smem) || !launch_regs(kern, F::kLaunchRegs)) return false;
@@ -548,7 +571,7 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   kern<<<dim3((unsigned)slots, pl.splits), F::kThreads, smem, st>>>(mq, mk, mv, p, bo);
   if (SPLIT) {
     const int64_t rows = (int64_t)a->tq * a->heads;
-    join_kernel<ET><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(*a, pl.parts, p.part_o, p.part_lse);
+    join_kernel<ET><<<(unsigned)rows, 32 * std::min(kJoinWarps, (pl.parts + 3) / 4), 0, st>>>(*a, pl.parts, p.part_o, p.part_lse);
   }
   return true;
 }

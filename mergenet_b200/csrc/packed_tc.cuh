@@ -98,34 +98,58 @@ __device__ __forceinline__ int slot_of_seq(const int32_t* cu, int b, int m, int 
 }
 inline int64_t tile_slots(int rows, int n, int m) { return (int64_t)rows / m + n + 1; }
 
-// The last sequence (0..n) whose first slot is at or below `slot`; a whole
-// warp searches, 32 probes a step.
-__device__ __forceinline__ int seq_of_slot(const int32_t* cu, int n, int m, int rows, int slot) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, hi = n + 1;  // first slot of lo <= slot; of hi > slot
-  while (hi - lo > 1) {
+// The sequence of tile slot `slot` of the query rows (of the key rows when
+// KEYS), by a whole warp: the last sequence b in 0..n whose first slot is at or
+// below it.  Sequence n is the rows behind the last one, which see nothing.
+// 32 probes a step narrow the range to 32 sequences, whose offsets are then
+// all read at once (a trip to memory a step; one for up to 32 sequences).
+struct Found {
+  Seq s;
+  int local;  // the slot's place among the sequence's own
+};
+template <bool KEYS>
+__device__ __forceinline__ Found seq_of_slot(const mn_packed_args& a, int m, int slot) {
+  const int32_t* cu = KEYS ? a.cu_k : a.cu_q;
+  const int rows = KEYS ? a.tk : a.tq, n = a.nseq, lane = threadIdx.x & 31;
+  int lo = 0, hi = n + 1;  // the first slot of lo is at or below `slot`, that of hi is not
+  while (hi - lo > 32) {
     const int step = (hi - lo + 31) / 32;
     const int b = lo + (lane + 1) * step;
     const bool le = b < hi && slot_of_seq(cu, b, m, rows) <= slot;
     const unsigned vote = __ballot_sync(MN_FULL_MASK, le);
-    const int k = vote == 0 ? 0 : 32 - __clz(vote);  // probes at or below (offsets ascend)
-    const int nlo = lo + k * step;
+    const int nlo = lo + (vote == 0 ? 0 : 32 - __clz(vote)) * step;  // offsets ascend
     hi = min(hi, nlo + step);
     lo = nlo;
   }
-  return lo;
+  const int b = min(lo + lane, hi - 1), e = min(b + 1, n);
+  const int q0 = a.cu_q[b], q1 = a.cu_q[e], k0 = a.cu_k[b], k1 = a.cu_k[e], len = a.len_k && b < n ? a.len_k[b] : 0x7fffffff;
+  Found f;
+  f.s.q0 = min(max(q0, 0), a.tq);
+  f.s.nq = (b < n ? min(max(q1, f.s.q0), a.tq) : a.tq) - f.s.q0;
+  f.s.k0 = min(max(k0, 0), a.tk);
+  f.s.slot = (b < n ? min(max(k1, f.s.k0), a.tk) : a.tk) - f.s.k0;
+  f.s.nk = b < n ? min(max(len, 0), f.s.slot) : 0;
+  const int first = (KEYS ? f.s.k0 : f.s.q0) / m + b;
+  const unsigned vote = __ballot_sync(MN_FULL_MASK, first <= slot);
+  const int src = vote == 0 ? 0 : 31 - __clz(vote);
+  f.s.q0 = __shfl_sync(MN_FULL_MASK, f.s.q0, src);
+  f.s.nq = __shfl_sync(MN_FULL_MASK, f.s.nq, src);
+  f.s.k0 = __shfl_sync(MN_FULL_MASK, f.s.k0, src);
+  f.s.slot = __shfl_sync(MN_FULL_MASK, f.s.slot, src);
+  f.s.nk = __shfl_sync(MN_FULL_MASK, f.s.nk, src);
+  f.local = slot - __shfl_sync(MN_FULL_MASK, first, src);
+  return f;
 }
-
-// Sequence n: the rows behind the last one, which see nothing.
-__device__ __forceinline__ Seq load_seq_or_tail(const mn_packed_args& a, int b) {
-  if (b < a.nseq) return load_seq(a.cu_q, a.cu_k, a.len_k, b, a.tq, a.tk);
-  Seq s;
-  s.q0 = min(max(a.cu_q[a.nseq], 0), a.tq);
-  s.nq = a.tq - s.q0;
-  s.k0 = min(max(a.cu_k[a.nseq], 0), a.tk);
-  s.slot = a.tk - s.k0;
-  s.nk = 0;
-  return s;
+// handed to the CTA through shared memory
+__device__ __forceinline__ void put_found(volatile uint32_t* at, const Found& f) {
+  if ((threadIdx.x & 31) == 0) {
+    at[0] = f.s.q0; at[1] = f.s.nq; at[2] = f.s.k0; at[3] = f.s.nk; at[4] = f.s.slot; at[5] = f.local;
+  }
+}
+__device__ __forceinline__ Found get_found(const volatile uint32_t* at) {
+  Found f;
+  f.s.q0 = at[0]; f.s.nq = at[1]; f.s.k0 = at[2]; f.s.nk = at[3]; f.s.slot = at[4]; f.local = at[5];
+  return f;
 }
 
 // 32 fp32 values of one row as ET, 16 bytes at a time, up to channel `d`
