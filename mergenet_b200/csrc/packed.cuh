@@ -25,6 +25,16 @@ __device__ __forceinline__ int bucket_of(const Borders& b, int r) {
   return u + (b.two_sided && r > 0 ? b.side : 0);
 }
 
+// First and last relative position of bucket u (empty where borders coincide):
+// one side's bucket k is the run of distances [at[k - 1], at[k]).
+__device__ __forceinline__ int2 bucket_range(const Borders& b, int u) {
+  const bool ahead = u >= b.side;
+  const int k = ahead ? u - b.side : u;
+  const int near = k == 0 ? 0 : b.at[k - 1], far = k < b.n ? b.at[k] - 1 : 0x3fffffff;
+  if (ahead) return make_int2(max(near, 1), far);
+  return make_int2(-far, k == 0 && !b.two_sided ? 0x3fffffff : -near);  // one-sided: all that is ahead as well
+}
+
 // false when the arguments describe no valid buckets
 inline bool make_borders(Borders* b, int buckets, int two_sided, int num_borders, const int32_t* at) {
   b->two_sided = two_sided ? 1 : 0;

@@ -33,17 +33,30 @@ struct BwdParams {
   int* err;
 };
 
-// Bias tables of a CTA: bucket of each distance, value of each (head, bucket)
+// Bias tables of a CTA: value of each (head, bucket) in log2 units, first and
+// last relative position of each bucket, bucket of each distance held.
 struct BiasSmem {
+  float* tab;    // [group][buckets]
+  int2* range;   // [buckets]
   uint8_t* idx;  // [span]
-  float* tab;    // [group][buckets], log2 units
 };
+__host__ __device__ constexpr uint32_t bias_bytes(int buckets, int group, int span) {
+  return (buckets * group * 4 + 15) / 16 * 16 + buckets * 8 + span;
+}
+__device__ __forceinline__ BiasSmem bias_at(uint8_t* at, int buckets, int group) {
+  BiasSmem s;
+  s.tab = reinterpret_cast<float*>(at);
+  s.range = reinterpret_cast<int2*>(at + (buckets * group * 4 + 15) / 16 * 16);
+  s.idx = reinterpret_cast<uint8_t*>(s.range + buckets);
+  return s;
+}
 __device__ __forceinline__ void fill_bias(const BwdParams& p, const Borders& bo, int hk, const BiasSmem& s, int threads) {
   for (int i = threadIdx.x; i < p.span; i += threads) s.idx[i] = (uint8_t)bucket_of(bo, i - p.reach);
   for (int i = threadIdx.x; i < p.group * p.a.buckets; i += threads) {
     const int g = i / p.a.buckets, u = i % p.a.buckets;
     s.tab[i] = load_any(p.a.bias_table, p.a.bias_dtype, (int64_t)u * p.a.heads + hk * p.group + g) * kLog2e;
   }
+  for (int u = threadIdx.x; u < p.a.buckets; u += threads) s.range[u] = bucket_range(bo, u);
 }
 
 template <typename ET>
@@ -62,7 +75,7 @@ __device__ __forceinline__ uint32_t left_cols(int kk) { return (uint32_t)(kk * 1
 // ----------------------------------------------------------------------- dq
 template <int DT, bool BIAS>
 struct Dq {
-  static constexpr int W = BIAS ? 2 : 4;  // threads to a row; the sums by bucket take shared memory for each
+  static constexpr int W = BIAS && DT == 128 ? 2 : 4;  // threads to a row; the sums by bucket take shared memory a warp
   static constexpr int CW = 128 / W, kThreads = 32 * (4 * W + 2);
   static constexpr int HV = DT / 64;
   static constexpr uint32_t kTile = HV * kHalfBytes;
@@ -72,9 +85,12 @@ struct Dq {
                        bDone = bDS + 1, bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
   static constexpr uint32_t oDelta = oMisc + 32;             // [2][128] partial deltas
-  static constexpr uint32_t oHist = oDelta + 2 * 128 * 4;    // [W][buckets][128]
+  // bias: per warp the sums by (head, bucket) and by (head, distance of a block); the bias tables
+  static constexpr uint32_t oHist = oDelta + 2 * 128 * 4;
+  static constexpr int diags(int group) { return CW + 32 / group + 1; }  // distances of a warp's rows to CW keys
+  static constexpr uint32_t warp_floats(int buckets, int group) { return buckets * group + group * diags(group) + group; }
   static constexpr uint32_t bytes(int buckets, int group, int span) {
-    return oHist + (BIAS ? W * buckets * 512 + ((buckets * group * 4 + 15) / 16) * 16 + span : 0) + 1024;
+    return oHist + (BIAS ? 4 * W * warp_floats(buckets, group) * 4 + bias_bytes(buckets, group, span) : 0) + 1024;
   }
   static constexpr uint32_t cS = 0, cDP = 256, cDQ = 384;
 };
@@ -94,9 +110,9 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
   const int hk = blockIdx.x % a.kv_heads, slot_id = blockIdx.x / a.kv_heads;
   float* hist = reinterpret_cast<float*>(base + C::oHist);
+  const int per_warp = BIAS ? C::warp_floats(a.buckets, G) : 0;
   BiasSmem bs;
-  bs.tab = reinterpret_cast<float*>(base + C::oHist + (BIAS ? W * a.buckets * 512 : 0));
-  bs.idx = reinterpret_cast<uint8_t*>(bs.tab) + (BIAS ? (a.buckets * G * 4 + 15) / 16 * 16 : 0);
+  if (BIAS) bs = bias_at(base + C::oHist + 4 * W * per_warp * 4, a.buckets, G);
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
   if (warp == 1) {
@@ -114,7 +130,7 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
   }
   if (BIAS) {
     fill_bias(p, bo, hk, bs, C::kThreads);
-    for (int i = tid; i < W * a.buckets * 128; i += C::kThreads) hist[i] = 0.f;
+    for (int i = tid; i < 4 * W * per_warp; i += C::kThreads) hist[i] = 0.f;
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -271,7 +287,11 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
     const float nlse = mine ? -a.lse[hk * rows + row] : -INFINITY;
     const float sl2 = a.scale * kLog2e;
     const float* tab = BIAS ? bs.tab + (mine ? g : 0) * a.buckets : nullptr;
-    float* my_hist = hist + (BIAS ? w * a.buckets * 128 + r : 0);
+    // bias: the warp's sums by (head, bucket), its block's by (head, distance), and each head's first distance
+    float* my_hist = hist + warp * per_warp;
+    float* diag = my_hist + a.buckets * G;
+    const int dist = BIAS ? C::diags(G) : 0, above = (31 - lane) / G;  // lanes of the same head above this one
+    int* first = reinterpret_cast<int*>(diag + G * dist);
     float far_lo = 0.f, far_hi = 0.f;
     for (int j = 0; j < n && ok; ++j) {
       const int k0 = j * 128 + w * CW;  // this thread's first key
@@ -335,24 +355,35 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tma::arrive(bars + C::bDS);
-      if (BIAS && mine) {
-        // keys out of the mask have ds = 0 (chunks that do not exist are not added)
+      if (BIAS) {
+        // Sums of ds by bucket; hidden keys have ds = 0, rows of no query and
+        // chunks that do not exist are left out.
         if (kind == 3) {
-          int cur = bs.idx[min(max(at, 0), p.span - 1)];
+          // Rows of one head are G lanes apart and one position on, so a
+          // distance's sum moves up G lanes a key: a shuffle and an addition
+          // a key for the whole warp, and the uppermost lane of each head has
+          // the sum of the next distance (the lower lanes hold the last ones).
           float acc = 0.f;
 #pragma unroll
           for (int e = 0; e < CW; ++e) {
-            if (e / 32 >= chunks) break;
-            const int u = bs.idx[min(max(at + e, 0), p.span - 1)];
-            if (u != cur) {
-              my_hist[cur * 128] += acc;
-              acc = 0.f;
-              cur = u;
-            }
-            acc += x[e];
+            const float below = __shfl_up_sync(MN_FULL_MASK, acc, G);
+            acc = (lane < G ? 0.f : below) + (mine && e / 32 < chunks ? x[e] : 0.f);
+            if (lane >= 32 - G) diag[g * dist + e] = acc;
           }
-          if (chunks > 0) my_hist[cur * 128] += acc;
-        } else {
+          diag[g * dist + CW - 1 + above] = acc;
+          if (above == 0) first[g] = k0 - pos;
+          __syncwarp();
+          // a bucket's distances are contiguous: a lane a (head, bucket)
+          for (int i = lane; i < a.buckets * G; i += 32) {
+            const int gg = i / a.buckets;
+            const int2 range = bs.range[i - gg * a.buckets];
+            const int o = first[gg], t1 = min(range.y - o, CW - 1 + 31 / G);
+            float sum = 0.f;
+            for (int t = max(range.x - o, 0); t <= t1; ++t) sum += diag[gg * dist + t];
+            my_hist[i] += sum;
+          }
+          __syncwarp();
+        } else if (mine) {
           float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < CW / 2; ++e)
@@ -384,19 +415,26 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
       }
     }
     if (BIAS) {
-      if (mine) {
-        my_hist[bs.idx[0] * 128] += far_lo;
-        my_hist[bs.idx[p.span - 1] * 128] += far_hi;
+      __syncwarp();
+      diag[lane] = far_lo;
+      diag[32 + lane] = far_hi;
+      __syncwarp();
+      if (lane < min(G, 32)) {  // the head of this lane: its rows are G lanes apart
+        float lo = 0.f, hi = 0.f;
+        for (int l = lane; l < 32; l += G) {
+          lo += diag[l];
+          hi += diag[32 + l];
+        }
+        my_hist[g * a.buckets + bs.idx[0]] += lo;
+        my_hist[g * a.buckets + bs.idx[p.span - 1]] += hi;
       }
       asm volatile("bar.sync 1, %0;" ::"n"(128 * W) : "memory");
       const int per = a.buckets * G;
       const int64_t slots = gridDim.x / a.kv_heads;
-      for (int i = tid; i < per; i += 128 * W) {
-        const int u = i / G, gg = i % G;
+      for (int i = tid; i < per; i += 128 * W) {  // in the order of dbias_kernel: [bucket][head]
+        const int at = i % G * a.buckets + i / G;
         float acc = 0.f;
-        for (int rr = gg; rr < 128; rr += G)
-#pragma unroll
-          for (int ww = 0; ww < W; ++ww) acc += hist[(ww * a.buckets + u) * 128 + rr];
+        for (int ww = 0; ww < 4 * W; ++ww) acc += hist[ww * per_warp + at];
         p.part[(hk * slots + slot_id) * per + i] = acc;
       }
     }
@@ -436,7 +474,7 @@ struct Dkv {
   static constexpr uint32_t oCol = oMisc + 32;  // [128] (token, head * buckets) of a column
   static constexpr uint32_t oTab = oCol + 128 * 8;
   static constexpr uint32_t bytes(int buckets, int group, int span) {
-    return oTab + (BIAS ? ((buckets * group * 4 + 15) / 16) * 16 + span : 0) + 1024;
+    return oTab + (BIAS ? bias_bytes(buckets, group, span) : 0) + 1024;
   }
   static constexpr uint32_t cS = 0, cDP = NS * 128, cDV = cDP + 128, cDK = cDV + DT;
 };
@@ -457,8 +495,7 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
   const int hk = blockIdx.x % a.kv_heads, slot_id = blockIdx.x / a.kv_heads;
   BiasSmem bs;
-  bs.tab = reinterpret_cast<float*>(base + C::oTab);
-  bs.idx = reinterpret_cast<uint8_t*>(bs.tab) + (BIAS ? (a.buckets * G * 4 + 15) / 16 * 16 : 0);
+  if (BIAS) bs = bias_at(base + C::oTab, a.buckets, G);
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
   if (warp == 1) {

@@ -501,7 +501,7 @@ int check(const mn_packed_args* a, Borders* bo, bool backward) {
     if (a->bias_dtype < 0 || a->bias_dtype > 2 || (backward && !a->dbias)) return MN_ERR_ARG;
     if (!make_borders(bo, a->buckets, a->two_sided, a->num_borders, a->borders)) return MN_ERR_ARG;
     const int last = bo->n ? bo->at[bo->n - 1] : 1;
-    if (a->buckets > 48 || a->buckets * g > 4096 || ((a->two_sided ? 2 : 1) * (int64_t)last + 1) * g > 8192) return MN_ERR_UNSUPPORTED;
+    if (g > 16 || a->buckets > 48 || ((a->two_sided ? 2 : 1) * (int64_t)last + 1) * g > 8192) return MN_ERR_UNSUPPORTED;
   }
   return MN_OK;
 }

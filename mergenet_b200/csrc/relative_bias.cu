@@ -86,17 +86,8 @@ __global__ void __launch_bounds__(kThreads) diagonal_kernel(int queries, int key
   const int first = c0 - i0 - start, lane = threadIdx.x & 31;
   float* out = part + ((int64_t)(h * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * buckets;
   for (int u = threadIdx.x >> 5; u < buckets; u += kThreads / 32) {
-    const bool ahead = u >= bo.side;
-    const int k = ahead ? u - bo.side : u;
-    const int near = k == 0 ? 0 : bo.at[k - 1], far = k < bo.n ? bo.at[k] - 1 : 0x3fffffff;
-    int a, b;  // the bucket's relative positions, both ends included
-    if (ahead) {
-      a = max(near, 1), b = far;
-    } else {
-      a = -far, b = -near;
-      if (k == 0 && !bo.two_sided) b = 0x7fffffff;  // one-sided: all that is ahead
-    }
-    const int t0 = (int)max((int64_t)a - first, (int64_t)0), t1 = (int)min((int64_t)b - first, (int64_t)kThreads - 1);
+    const int2 range = bucket_range(bo, u);
+    const int t0 = max(range.x - first, 0), t1 = min(range.y - first, kThreads - 1);
     float s = 0.f;
     for (int t = t0 + lane; t <= t1; t += 32) s += sum[t];
     s = warp_sum(s);

@@ -27,7 +27,7 @@ from .attention import _STATUS, _status
 MAX_HEAD_DIM = 128
 MAX_GROUP = 128       # query heads that may share a key head
 MAX_BUCKETS = 48      # of a table used inside the attention
-MAX_BIAS_ENTRIES = 4096  # buckets x grouped heads
+MAX_BIAS_GROUP = 16   # query heads that may share a key head then
 MAX_BIAS_VALUES = 8192  # distances x grouped heads that a kernel keeps on chip
 
 
@@ -319,10 +319,10 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
     if bias_table is not None:
         _check_table(bias_table, buckets, h)
         sides = 2 if buckets.two_sided else 1
-        if (buckets.num_buckets > MAX_BUCKETS or buckets.num_buckets * group > MAX_BIAS_ENTRIES
+        if (buckets.num_buckets > MAX_BUCKETS or group > MAX_BIAS_GROUP
                 or (sides * buckets.borders[-1] + 1) * group > MAX_BIAS_VALUES):
             raise ValueError(f"{buckets} with {group} grouped heads does not fit: at most {MAX_BUCKETS} buckets, "
-                             f"{MAX_BIAS_ENTRIES} buckets x grouped heads and {MAX_BIAS_VALUES} distances x grouped heads")
+                             f"{MAX_BIAS_GROUP} grouped heads and {MAX_BIAS_VALUES} distances x grouped heads")
     if max(tq, tk) * group >= 1 << 30:
         raise ValueError("at most 2^30 rows x grouped heads")
     _require(q.device, q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, bias_table)
