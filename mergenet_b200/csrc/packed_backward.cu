@@ -73,14 +73,14 @@ template <int CW>
 __device__ __forceinline__ uint32_t left_cols(int kk) { return (uint32_t)(kk * 16 / CW * CW + kk * 16 % CW / 2); }
 
 // ----------------------------------------------------------------------- dq
-template <int DT, bool BIAS>
+template <int DT, int NB, bool BIAS>
 struct Dq {
-  static constexpr int W = BIAS && DT == 128 ? 2 : 4;  // threads to a row; the sums by bucket take shared memory a warp
-  static constexpr int CW = 128 / W, kThreads = 32 * (4 * W + 2);
+  static constexpr int W = NB == 64 || BIAS ? 2 : 4;  // threads to a row; the sums by bucket take shared memory a warp
+  static constexpr int CW = NB / W, kThreads = 32 * (4 * W + 2), kPerSM = NB == 64 ? 2 : 1;
   static constexpr int HV = DT / 64;
-  static constexpr uint32_t kTile = HV * kHalfBytes;
+  static constexpr uint32_t kTile = HV * kHalfBytes, kKVHalf = NB * 128, kKV = HV * kKVHalf;
   static constexpr int KS = DT == 64 || !BIAS ? 3 : 2, VS = DT == 64 || !BIAS ? 2 : 1;
-  static constexpr uint32_t oQ = 0, oDO = kTile, oK = 2 * kTile, oV = oK + KS * kTile, oBars = oV + VS * kTile;
+  static constexpr uint32_t oQ = 0, oDO = kTile, oK = 2 * kTile, oV = oK + KS * kKV, oBars = oV + VS * kKV;
   static constexpr int bQ = 0, bKF = 1, bKE = bKF + KS, bVF = bKE + KS, bVE = bVF + VS, bS = bVE + VS, bDP = bS + 2, bDS = bDP + 1,
                        bDone = bDS + 1, bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
@@ -92,15 +92,16 @@ struct Dq {
   static constexpr uint32_t bytes(int buckets, int group, int span) {
     return oHist + (BIAS ? 4 * W * warp_floats(buckets, group) * 4 + bias_bytes(buckets, group, span) : 0) + 1024;
   }
-  static constexpr uint32_t cS = 0, cDP = 256, cDQ = 384;
+  static constexpr uint32_t cS = 0, cDP = 2 * NB, cDQ = 3 * NB, kCols = NB == 64 ? 256 : 512;
+  static_assert(cDQ + DT <= kCols, "tensor memory");
 };
 
-template <typename ET, int DT, bool BIAS>
-__global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
+template <typename ET, int DT, int NB, bool BIAS>
+__global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::kPerSM)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
               const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
               const __grid_constant__ BwdParams p, const __grid_constant__ Borders bo) {
-  using C = Dq<DT, BIAS>;
+  using C = Dq<DT, NB, BIAS>;
   constexpr int HV = C::HV, KS = C::KS, VS = C::VS, W = C::W, CW = C::CW;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
   BiasSmem bs;
   if (BIAS) bs = bias_at(base + C::oHist + 4 * W * per_warp * 4, a.buckets, G);
 
-  if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
+  if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), C::kCols);
   if (warp == 1) {
     put_found(misc + 1, seq_of_slot<false>(a, p.ntok, slot_id));
   }
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
   const int shift = s.nk - s.nq;
   const int last = min(s.nq, t0 + p.ntok) - 1;
   const int keys = a.causal ? min(s.nk, last + shift + 1) : s.nk;
-  const int n = present && keys > 0 ? (keys + 127) >> 7 : 0;
+  const int n = present && keys > 0 ? (keys + NB - 1) / NB : 0;
   constexpr int ab_bf16 = std::is_same<ET, __nv_bfloat16>::value ? 1 : 0;
   bool ok = true;
 
@@ -160,14 +161,14 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
       for (int j = 0; j < n && ok; ++j) {
         const int ks = j % KS, vs = j % VS;
         if (j >= KS && !(ok = wait(bars + C::bKE + ks, (j / KS - 1) & 1, p.err))) break;
-        tma::expect_tx(bars + C::bKF + ks, C::kTile);
+        tma::expect_tx(bars + C::bKF + ks, C::kKV);
         for (int h = 0; h < HV; ++h)
-          load_3d(tc::smem_u32(base + C::oK + ks * C::kTile + h * kHalfBytes), &tm_k, h * 64, hk, s.k0 + j * 128, bars + C::bKF + ks);
+          load_3d(tc::smem_u32(base + C::oK + ks * C::kKV + h * C::kKVHalf), &tm_k, h * 64, hk, s.k0 + j * NB, bars + C::bKF + ks);
         nk = j + 1;
         if (j >= VS && !(ok = wait(bars + C::bVE + vs, (j / VS - 1) & 1, p.err))) break;
-        tma::expect_tx(bars + C::bVF + vs, C::kTile);
+        tma::expect_tx(bars + C::bVF + vs, C::kKV);
         for (int h = 0; h < HV; ++h)
-          load_3d(tc::smem_u32(base + C::oV + vs * C::kTile + h * kHalfBytes), &tm_v, h * 64, hk, s.k0 + j * 128, bars + C::bVF + vs);
+          load_3d(tc::smem_u32(base + C::oV + vs * C::kKV + h * C::kKVHalf), &tm_v, h * 64, hk, s.k0 + j * NB, bars + C::bVF + vs);
         nv = j + 1;
       }
       if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
     // S runs one block ahead of dP: at ds(j), dP(j + 1), dQ += ds(j) K(j) and
     // S(j + 2) are issued while the compute warps turn S(j + 1) into p
     constexpr uint32_t idesc_q = tc::idesc_f16(ab_bf16, 1, 128, DT);
-    auto cols_of = [&](int j) { return min(128, (s.nk - j * 128 + 31) & ~31); };
+    auto cols_of = [&](int j) { return min(NB, (s.nk - j * NB + 31) & ~31); };
     // D = A B^T over the channels, both operands 128-byte rows in shared memory
     auto scores = [&](uint32_t d, const uint8_t* x, const uint8_t* y, int cols, uint64_t* bar) {
       if (elect_one()) {
@@ -191,8 +192,8 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
         const uint32_t idesc = tc::idesc_f16(ab_bf16, 0, 128, cols);
 #pragma unroll
         for (int kk = 0; kk < DT / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3);
-          tc::mma_f16_ss(d, dx + off, dy + off, idesc, kk > 0 ? 1u : 0u);
+          tc::mma_f16_ss(d, dx + (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3), dy + (kk >> 2) * (C::kKVHalf >> 4) + 2 * (kk & 3), idesc,
+                         kk > 0 ? 1u : 0u);
         }
         tc::mma_commit(bar);
       }
@@ -201,19 +202,19 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
     auto issue_s = [&](int j) -> bool {
       const int ks = j % KS;
       if (!wait(bars + C::bKF + ks, (j / KS) & 1, p.err)) return false;
-      uint8_t* k = base + C::oK + ks * C::kTile;
+      uint8_t* k = base + C::oK + ks * C::kKV;
       const int cols = cols_of(j);
       // rows behind the last key are an operand of ds K
-      if (s.nk - j * 128 < cols) zero_rows(k, s.nk - j * 128, cols, HV);
-      scores(tmem + C::cS + (j & 1) * 128, base + C::oQ, k, cols, bars + C::bS + (j & 1));
+      if (s.nk - j * NB < cols) zero_rows(k, s.nk - j * NB, cols, HV, C::kKVHalf);
+      scores(tmem + C::cS + (j & 1) * NB, base + C::oQ, k, cols, bars + C::bS + (j & 1));
       return true;
     };
     auto issue_dp = [&](int j) -> bool {
       const int vs = j % VS;
       if (!wait(bars + C::bVF + vs, (j / VS) & 1, p.err)) return false;
-      uint8_t* v = base + C::oV + vs * C::kTile;
+      uint8_t* v = base + C::oV + vs * C::kKV;
       const int cols = cols_of(j);
-      if (s.nk - j * 128 < cols) zero_rows(v, s.nk - j * 128, cols, HV);  // 0 (dP - delta) must not meet a NaN
+      if (s.nk - j * NB < cols) zero_rows(v, s.nk - j * NB, cols, HV, C::kKVHalf);  // 0 (dP - delta) must not meet a NaN
       scores(tmem + C::cDP, base + C::oDO, v, cols, bars + C::bDP);
       return true;
     };
@@ -226,11 +227,11 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
         if (elect_one()) {
           tc::fence_after_sync();
           const int cols = cols_of(j);
-          const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + C::oK + (j % KS) * C::kTile), kHalfBytes);
+          const uint64_t dk = tc::sw128_desc(tc::smem_u32(base + C::oK + (j % KS) * C::kKV), C::kKVHalf);
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
+          for (int kk = 0; kk < NB / 16; ++kk)
             if (kk * 16 < cols)
-              tc::mma_f16_ts(tmem + C::cDQ, tmem + C::cS + (j & 1) * 128 + left_cols<CW>(kk), dk + 128 * kk, idesc_q,
+              tc::mma_f16_ts(tmem + C::cDQ, tmem + C::cS + (j & 1) * NB + left_cols<CW>(kk), dk + 128 * kk, idesc_q,
                              (j > 0 || kk > 0) ? 1u : 0u);
           tc::mma_commit(bars + C::bKE + j % KS);
           if (j == n - 1) tc::mma_commit(bars + C::bDone);
@@ -294,9 +295,9 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
     int* first = reinterpret_cast<int*>(diag + G * dist);
     float far_lo = 0.f, far_hi = 0.f;
     for (int j = 0; j < n && ok; ++j) {
-      const int k0 = j * 128 + w * CW;  // this thread's first key
-      const int chunks = max(0, min(CW / 32, (min(128, (s.nk - j * 128 + 31) & ~31) - w * CW) >> 5));
-      const uint32_t t_s = tmem + C::cS + (j & 1) * 128 + w * CW + lane_sel, t_dp = tmem + C::cDP + w * CW + lane_sel;
+      const int k0 = j * NB + w * CW;  // this thread's first key
+      const int chunks = max(0, min(CW / 32, (min(NB, (s.nk - j * NB + 31) & ~31) - w * CW) >> 5));
+      const uint32_t t_s = tmem + C::cS + (j & 1) * NB + w * CW + lane_sel, t_dp = tmem + C::cDP + w * CW + lane_sel;
       if (!(ok = wait(bars + C::bS + (j & 1), (j >> 1) & 1, p.err))) break;
       tc::fence_after_sync();
       float x[CW];
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(Dq<DT, BIAS>::kThreads, 1)
   __syncthreads();
   if (warp == 0) {
     tc::fence_after_sync();
-    tc::tmem_dealloc(tmem, 512);
+    tc::tmem_dealloc(tmem, C::kCols);
   }
 }
 
@@ -459,32 +460,33 @@ __global__ void __launch_bounds__(128) dbias_kernel(int heads, int group, int bu
 }
 
 // ------------------------------------------------------------------- dk, dv
-template <int DT, bool BIAS>
+template <int DT, int NB, bool BIAS>
 struct Dkv {
-  static constexpr int W = 4, CW = 128 / W, kThreads = 32 * (4 * W + 2);
+  static constexpr int W = NB / 32, CW = 32, kThreads = 32 * (4 * W + 2), kPerSM = NB == 64 ? 2 : 1;
   static constexpr int HV = DT / 64;
-  static constexpr uint32_t kTile = HV * kHalfBytes;
-  static constexpr int NS = DT == 64 ? 2 : 1;  // S^T buffers in tensor memory
-  static constexpr int QS = NS + 1;            // stages of Q, dout, lse and delta
-  static constexpr uint32_t oK = 0, oV = kTile, oRing = 2 * kTile, oRows = oRing + QS * 2 * kTile;  // rows: [QS][2][128] floats
-  static constexpr uint32_t oBars = oRows + QS * 1024;
+  static constexpr uint32_t kTile = HV * kHalfBytes, kQHalf = NB * 128, kQ = HV * kQHalf;
+  static constexpr int NS = DT == 64 && NB == 128 ? 2 : 1;  // S^T buffers in tensor memory
+  static constexpr int QS = NB == 64 ? 3 : NS + 1;  // stages of Q, dout, lse and delta
+  static constexpr uint32_t oK = 0, oV = kTile, oRing = 2 * kTile, oRows = oRing + QS * 2 * kQ;  // rows: [QS][2][NB] floats
+  static constexpr uint32_t oBars = oRows + QS * NB * 8;
   static constexpr int bKV = 0, bF = 1, bE = bF + QS, bS = bE + QS, bP = bS + NS, bDP = bP + NS, bDS = bDP + 1, bDone = bDS + 1,
                        bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
-  static constexpr uint32_t oCol = oMisc + 32;  // [128] (token, head * buckets) of a column
-  static constexpr uint32_t oTab = oCol + 128 * 8;
+  static constexpr uint32_t oCol = oMisc + 32;  // [NB] (token, head * buckets) of a column
+  static constexpr uint32_t oTab = oCol + NB * 8;
   static constexpr uint32_t bytes(int buckets, int group, int span) {
     return oTab + (BIAS ? bias_bytes(buckets, group, span) : 0) + 1024;
   }
-  static constexpr uint32_t cS = 0, cDP = NS * 128, cDV = cDP + 128, cDK = cDV + DT;
+  static constexpr uint32_t cS = 0, cDP = NS * NB, cDV = cDP + NB, cDK = cDV + DT, kCols = NB == 64 ? 256 : 512;
+  static_assert(cDK + DT <= kCols, "tensor memory");
 };
 
-template <typename ET, int DT, bool BIAS>
-__global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
+template <typename ET, int DT, int NB, bool BIAS>
+__global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>::kPerSM)
     dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const __grid_constant__ BwdParams p, const __grid_constant__ Borders bo) {
-  using C = Dkv<DT, BIAS>;
+  using C = Dkv<DT, NB, BIAS>;
   constexpr int HV = C::HV, NS = C::NS, QS = C::QS, W = C::W, CW = C::CW;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
   BiasSmem bs;
   if (BIAS) bs = bias_at(base + C::oTab, a.buckets, G);
 
-  if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), 512);
+  if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), C::kCols);
   if (warp == 1) {
     put_found(misc + 1, seq_of_slot<true>(a, 128, slot_id));
   }
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
   }
   if (BIAS) {
     fill_bias(p, bo, hk, bs, C::kThreads);
-    if (tid < 128) col[tid] = make_int2(tid / G, (tid % G) * a.buckets);
+    if (tid < NB) col[tid] = make_int2(tid / G, (tid % G) * a.buckets);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -550,22 +552,22 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
       for (int i = 0; i < n && ok; ++i) {
         const int st = i % QS, t0 = (i0 + i) * p.ntok;
         if (i >= QS && !(ok = wait(bars + C::bE + st, (i / QS - 1) & 1, p.err))) break;
-        uint8_t* q = base + C::oRing + st * 2 * C::kTile;
+        uint8_t* q = base + C::oRing + st * 2 * C::kQ;
         if (lane == 0) {
           tma::expect_tx(bars + C::bF + st, 2u * HV * 128u * (uint32_t)(G * p.ntok));
           for (int h = 0; h < HV; ++h) {
-            tma::load_4d(tc::smem_u32(q + h * kHalfBytes), &tm_q, h * 64, 0, hk, s.q0 + t0, bars + C::bF + st);
-            tma::load_4d(tc::smem_u32(q + C::kTile + h * kHalfBytes), &tm_do, h * 64, 0, hk, s.q0 + t0, bars + C::bF + st);
+            tma::load_4d(tc::smem_u32(q + h * C::kQHalf), &tm_q, h * 64, 0, hk, s.q0 + t0, bars + C::bF + st);
+            tma::load_4d(tc::smem_u32(q + C::kQ + h * C::kQHalf), &tm_do, h * 64, 0, hk, s.q0 + t0, bars + C::bF + st);
           }
         }
         // -lse (with the bias where it is the same for the whole tile) and
         // -delta of the rows; rows of no query give p = 0
-        float* x = reinterpret_cast<float*>(base + C::oRows) + st * 256;
+        float* x = reinterpret_cast<float*>(base + C::oRows) + st * 2 * NB;
         const int valid = min(p.ntok, s.nq - t0) * G;
         const int64_t first = hk * rows + (int64_t)(s.q0 + t0) * G;
         const int kind = BIAS ? kind_of(t0) : 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < NB / 32; ++e) {
           const int r = e * 32 + lane;
           float l = -INFINITY, d = 0.f;
           if (r < valid) {
@@ -574,7 +576,7 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
             if (BIAS && kind != 3) l += bs.tab[col[r].y + bs.idx[kind == 1 ? 0 : p.span - 1]];
           }
           x[r] = l;
-          x[128 + r] = d;
+          x[NB + r] = d;
         }
         __syncwarp();
         if (lane == 0) tma::arrive(bars + C::bF + st);
@@ -593,16 +595,16 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
     // While the compute warps turn S(i) into p the tensor core finishes
     // dK += ds(i - 1) Q and dP(i); while they form ds(i), dV += p(i) dout and
     // the next S.
-    constexpr uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, 128), idesc_g = tc::idesc_f16(ab_bf16, 1, 128, DT);
-    auto stage = [&](int i) { return base + C::oRing + (i % QS) * 2 * C::kTile; };
+    constexpr uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, NB), idesc_g = tc::idesc_f16(ab_bf16, 1, 128, DT);
+    auto stage = [&](int i) { return base + C::oRing + (i % QS) * 2 * C::kQ; };
     auto scores = [&](uint32_t d, const uint8_t* x, const uint8_t* y, uint64_t* bar) {
       if (elect_one()) {
         tc::fence_after_sync();
         const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), 16), dy = tc::sw128_desc(tc::smem_u32(y), 16);
 #pragma unroll
         for (int kk = 0; kk < DT / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3);
-          tc::mma_f16_ss(d, dx + off, dy + off, idesc_s, kk > 0 ? 1u : 0u);
+          tc::mma_f16_ss(d, dx + (kk >> 2) * (kHalfBytes >> 4) + 2 * (kk & 3), dy + (kk >> 2) * (C::kQHalf >> 4) + 2 * (kk & 3), idesc_s,
+                         kk > 0 ? 1u : 0u);
         }
         tc::mma_commit(bar);
       }
@@ -611,28 +613,28 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
     auto issue_s = [&](int i) -> bool {
       if (!wait(bars + C::bF + i % QS, (i / QS) & 1, p.err)) return false;
       const int valid = min(p.ntok, s.nq - (i0 + i) * p.ntok) * G;
-      if (valid < 128) {  // rows of no query are an operand of dK and dV
-        zero_rows(stage(i), valid, 128, HV);
-        zero_rows(stage(i) + C::kTile, valid, 128, HV);
+      if (valid < NB) {  // rows of no query are an operand of dK and dV
+        zero_rows(stage(i), valid, NB, HV, C::kQHalf);
+        zero_rows(stage(i) + C::kQ, valid, NB, HV, C::kQHalf);
       }
-      scores(tmem + C::cS + (i % NS) * 128, base + C::oK, stage(i), bars + C::bS + i % NS);
+      scores(tmem + C::cS + (i % NS) * NB, base + C::oK, stage(i), bars + C::bS + i % NS);
       return true;
     };
     auto grads = [&](uint32_t d, uint32_t left, const uint8_t* x, bool more) {  // D += left x
-      const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), kHalfBytes);
+      const uint64_t dx = tc::sw128_desc(tc::smem_u32(x), C::kQHalf);
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
+      for (int kk = 0; kk < NB / 16; ++kk)
         tc::mma_f16_ts(d, left + left_cols<CW>(kk), dx + 128 * kk, idesc_g, (more || kk > 0) ? 1u : 0u);
     };
     if (n > 0) {
       ok = wait(bars + C::bKV, 0, p.err);
       for (int i = 0; i < NS && i < n && ok; ++i) ok = issue_s(i);
-      if (ok) scores(tmem + C::cDP, base + C::oV, stage(0) + C::kTile, bars + C::bDP);
+      if (ok) scores(tmem + C::cDP, base + C::oV, stage(0) + C::kQ, bars + C::bDP);
       for (int i = 0; i < n && ok; ++i) {
         if (!(ok = wait(bars + C::bP + i % NS, (i / NS) & 1, p.err))) break;
         if (elect_one()) {
           tc::fence_after_sync();
-          grads(tmem + C::cDV, tmem + C::cS + (i % NS) * 128, stage(i) + C::kTile, i > 0);
+          grads(tmem + C::cDV, tmem + C::cS + (i % NS) * NB, stage(i) + C::kQ, i > 0);
         }
         __syncwarp();
         // S(i + NS) overwrites p(i), which the product before it in order has read
@@ -645,7 +647,7 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
           if (i == n - 1) tc::mma_commit(bars + C::bDone);
         }
         __syncwarp();
-        if (i + 1 < n) scores(tmem + C::cDP, base + C::oV, stage(i + 1) + C::kTile, bars + C::bDP);
+        if (i + 1 < n) scores(tmem + C::cDP, base + C::oV, stage(i + 1) + C::kQ, bars + C::bDP);
       }
       if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
       if (elect_one()) {
@@ -662,8 +664,8 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
     const float sl2 = a.scale * kLog2e;
     for (int i = 0; i < n && ok; ++i) {
       const int st = i % QS, t0 = (i0 + i) * p.ntok;
-      const uint32_t t_s = tmem + C::cS + (i % NS) * 128 + w * CW + lane_sel, t_dp = tmem + C::cDP + w * CW + lane_sel;
-      const float* nl = reinterpret_cast<const float*>(base + C::oRows) + st * 256 + w * CW;
+      const uint32_t t_s = tmem + C::cS + (i % NS) * NB + w * CW + lane_sel, t_dp = tmem + C::cDP + w * CW + lane_sel;
+      const float* nl = reinterpret_cast<const float*>(base + C::oRows) + st * 2 * NB + w * CW;
       // columns from here on see this key; the warp's last key sees the latest start
       const int c0 = a.causal ? (key - shift - t0) * G - w * CW : 0;
       const bool masked = a.causal && (k0 + ((warp & 3) * 32 + 31) - shift - t0) * G > w * CW;
@@ -709,7 +711,7 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
       tc::tmem_ld_wait<CW>(d);
 #pragma unroll
       for (int e = 0; e < CW / 4; ++e) {
-        const float4 nd = reinterpret_cast<const float4*>(nl + 128)[e];
+        const float4 nd = reinterpret_cast<const float4*>(nl + NB)[e];
         const float2 y0 = fmul2(make_float2(x[4 * e], x[4 * e + 1]), fadd2(make_float2(d[4 * e], d[4 * e + 1]), make_float2(nd.x, nd.y)));
         const float2 y1 = fmul2(make_float2(x[4 * e + 2], x[4 * e + 3]), fadd2(make_float2(d[4 * e + 2], d[4 * e + 3]), make_float2(nd.z, nd.w)));
         d[4 * e] = y0.x; d[4 * e + 1] = y0.y; d[4 * e + 2] = y1.x; d[4 * e + 3] = y1.y;
@@ -748,20 +750,25 @@ __global__ void __launch_bounds__(Dkv<DT, BIAS>::kThreads, 1)
   __syncthreads();
   if (warp == 0) {
     tc::fence_after_sync();
-    tc::tmem_dealloc(tmem, 512);
+    tc::tmem_dealloc(tmem, C::kCols);
   }
 }
 
 // ------------------------------------------------------------------- host
 struct BwdSizes {
-  int ntok;
+  int ntok, ntok_k;  // tokens to a tile of the query side, to a block of the key side
   int64_t q_slots, k_slots;
   size_t delta_bytes, bytes;
 };
+// Up to 64 channels: blocks of 64 columns and two CTAs to an SM, so that one's
+// start and end run under the other's products; not where a token's heads
+// would fill such a block badly.
+static bool small_blocks(const mn_packed_args* a) { return a->head_dim <= 64 && a->heads / a->kv_heads <= 32; }
 static BwdSizes sizes_of(const mn_packed_args* a) {
   BwdSizes z;
   const int g = a->heads / a->kv_heads;
   z.ntok = 128 / g;
+  z.ntok_k = small_blocks(a) ? 64 / g : z.ntok;
   z.q_slots = tile_slots(a->tq, a->nseq, z.ntok);
   z.k_slots = tile_slots(a->tk, a->nseq, 128);
   z.delta_bytes = ((size_t)a->tq * a->heads * 4 + 255) / 256 * 256;
@@ -769,7 +776,7 @@ static BwdSizes sizes_of(const mn_packed_args* a) {
   return z;
 }
 
-template <typename ET, int DT, bool BIAS>
+template <typename ET, int DT, int NB, bool BIAS>
 static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSizes& z, void* ws, int* err, cudaStream_t st) {
   constexpr bool bf16 = std::is_same<ET, __nv_bfloat16>::value;
   BwdParams p;
@@ -785,19 +792,27 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
   p.delta = static_cast<float*>(ws);
   p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + z.delta_bytes);
   p.err = err;
-  CUtensorMap mq, mdo, mk, mv;
+  CUtensorMap mq, mdo, mk, mv, nq, ndo, nk, nv;  // m: the query-side kernel's, n: the key-side kernel's
+  const void *k = a->tk ? a->k : a->q, *v = a->tk ? a->v : a->q;
+  const int tk = std::max(a->tk, 1);
   if (!bind_context() || !map_q(&mq, bf16, a->q, a->q_st, a->q_sh, a->tq, a->heads, a->kv_heads, a->head_dim, z.ntok) ||
       !map_q(&mdo, bf16, a->dout, a->do_st, a->do_sh, a->tq, a->heads, a->kv_heads, a->head_dim, z.ntok) ||
-      !map_k(&mk, bf16, a->tk ? a->k : a->q, a->k_st, a->k_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, 128) ||
-      !map_k(&mv, bf16, a->tk ? a->v : a->q, a->v_st, a->v_sh, std::max(a->tk, 1), a->kv_heads, a->head_dim, 128))
+      !map_k(&mk, bf16, k, a->k_st, a->k_sh, tk, a->kv_heads, a->head_dim, NB) ||
+      !map_k(&mv, bf16, v, a->v_st, a->v_sh, tk, a->kv_heads, a->head_dim, NB) ||
+      !map_q(&nq, bf16, a->q, a->q_st, a->q_sh, a->tq, a->heads, a->kv_heads, a->head_dim, z.ntok_k) ||
+      !map_q(&ndo, bf16, a->dout, a->do_st, a->do_sh, a->tq, a->heads, a->kv_heads, a->head_dim, z.ntok_k) ||
+      !map_k(&nk, bf16, k, a->k_st, a->k_sh, tk, a->kv_heads, a->head_dim, 128) ||
+      !map_k(&nv, bf16, v, a->v_st, a->v_sh, tk, a->kv_heads, a->head_dim, 128))
     return false;
   if (z.q_slots * a->kv_heads > 0x7fffffff || z.k_slots * a->kv_heads > 0x7fffffff) return false;
-  auto kq = dq_kernel<ET, DT, BIAS>;
-  auto kkv = dkv_kernel<ET, DT, BIAS>;
-  const size_t sq = Dq<DT, BIAS>::bytes(a->buckets, p.group, p.span), skv = Dkv<DT, BIAS>::bytes(a->buckets, p.group, p.span);
+  auto kq = dq_kernel<ET, DT, NB, BIAS>;
+  auto kkv = dkv_kernel<ET, DT, NB, BIAS>;
+  const size_t sq = Dq<DT, NB, BIAS>::bytes(a->buckets, p.group, p.span), skv = Dkv<DT, NB, BIAS>::bytes(a->buckets, p.group, p.span);
   if (!ensure_smem(kq, sq) || !ensure_smem(kkv, skv)) return false;
-  kq<<<(unsigned)(z.q_slots * a->kv_heads), Dq<DT, BIAS>::kThreads, sq, st>>>(mq, mdo, mk, mv, p, bo);
-  if (a->tk > 0) kkv<<<(unsigned)(z.k_slots * a->kv_heads), Dkv<DT, BIAS>::kThreads, skv, st>>>(mq, mdo, mk, mv, p, bo);
+  kq<<<(unsigned)(z.q_slots * a->kv_heads), Dq<DT, NB, BIAS>::kThreads, sq, st>>>(mq, mdo, mk, mv, p, bo);
+  BwdParams pk = p;
+  pk.ntok = z.ntok_k;
+  if (a->tk > 0) kkv<<<(unsigned)(z.k_slots * a->kv_heads), Dkv<DT, NB, BIAS>::kThreads, skv, st>>>(nq, ndo, nk, nv, pk, bo);
   if (BIAS)
     dbias_kernel<<<dim3(a->buckets * p.group, a->kv_heads), 128, 0, st>>>(a->heads, p.group, a->buckets, (int)z.q_slots, p.part,
                                                                          a->dbias, a->bias_dtype);
@@ -806,7 +821,13 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
 
 template <typename ET, int DT>
 static bool launch_bwd_d(const mn_packed_args* a, const Borders& bo, const BwdSizes& z, void* ws, int* err, cudaStream_t st) {
-  return a->bias_table ? launch_bwd<ET, DT, true>(a, bo, z, ws, err, st) : launch_bwd<ET, DT, false>(a, bo, z, ws, err, st);
+  if constexpr (DT == 64) {
+    if (small_blocks(a))
+      return a->bias_table ? launch_bwd<ET, DT, 64, true>(a, bo, z, ws, err, st) : launch_bwd<ET, DT, 64, false>(a, bo, z, ws, err, st);
+    return launch_bwd<ET, DT, 128, false>(a, bo, z, ws, err, st);  // a bias comes with at most 16 grouped heads
+  } else {
+    return a->bias_table ? launch_bwd<ET, DT, 128, true>(a, bo, z, ws, err, st) : launch_bwd<ET, DT, 128, false>(a, bo, z, ws, err, st);
+  }
 }
 
 }  // namespace pk
