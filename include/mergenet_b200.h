@@ -334,11 +334,18 @@ int mn_attention(int batch, int nq, int nk, int heads, int head_dim, int dtype,
  *
  * q [tq, heads, head_dim], k and v [tk, kv_heads, head_dim] with element
  * strides (_st per row, _sh per head) and contiguous channels, fp16 or bf16;
- * head_dim a multiple of 8 up to 128; pointers 16-byte aligned and strides
- * multiples of 8.  out, dq, dk, dv: contiguous, of the same type.  bias_table
+ * head_dim a multiple of 8 up to 128; at most 128 query heads to a key head;
+ * pointers 16-byte aligned and strides positive multiples of 8.  With a bias
+ * at most 16 query heads to a key head, 48 buckets, and 8192 distances x
+ * grouped heads (distances: up to the last border, on each side).  Anything
+ * else returns MN_ERR_UNSUPPORTED.  out, dq, dk, dv: contiguous, of the same
+ * type.  bias_table
  * [buckets, heads] contiguous, of bias_dtype; dbias the same.
  * lse [kv_heads, tq, heads / kv_heads] fp32: log2 of each row's sum of
- * exponentials (+inf where no key is seen); NULL when no backward follows. */
+ * exponentials (+inf where no key is seen); NULL when no backward follows.
+ * status: MN_STATUS_BAD_LENGTHS for offsets that decrease or leave the tensors
+ * and lengths that leave their slots (no access follows them out), and
+ * MN_STATUS_TC_TIMEOUT. */
 typedef struct mn_packed_args {
   const void *q, *k, *v;
   const int32_t *cu_q, *cu_k, *len_k;
@@ -363,7 +370,8 @@ int mn_packed_attention(const mn_packed_args* args, void* workspace,
 
 /* Gradients of mn_packed_attention: reads its out and lse and dout, writes
  * dq, dk, dv (rows of no sequence and unused key rows get 0) and, with a
- * bias_table, dbias.  Every sum has a fixed order. */
+ * bias_table, dbias.  Every sum has a fixed order.  tq is at least 1 (without
+ * a query every gradient is 0). */
 size_t mn_packed_attention_backward_workspace_bytes(const mn_packed_args* args);
 int mn_packed_attention_backward(const mn_packed_args* args, void* workspace,
                                  size_t workspace_bytes, int* status,

@@ -15,17 +15,24 @@
 //     grown by more than 2^8 since its last scale, so rarely.
 //
 // The softmax warps bound the kernel: an exponential with its scaling, sum and
-// conversion takes a scheduler about 9 cycles with two warps on it (8 of them
-// the special-function unit; a polynomial on the FMA pipe takes as long), so
-// 1,180 cycles for 128 rows x 128 keys, against 16 D cycles of products... 
+// conversion takes a scheduler about 9 cycles with two warps on it, 8 of them
+// the special-function unit (a polynomial on the FMA pipe takes as long: a
+// packed FMA of two values issues in two cycles), so 1,180 cycles for 128 rows
+// x 128 keys, against 8 D = 1,024 cycles of products at 128 channels.
 //
 // Up to 64 channels one CTA works on one tile and two CTAs share an SM; blocks
 // of 64 keys, three S buffers, so that the softmax warps run back to back.
 // Up to 128 channels one CTA works on two tiles that share K and V (a single
 // tile would ask the L2 for 64 bytes a cycle and SM); tensor memory then holds
 // one S a tile, and the tiles take turns: one's products run under the
-// other's softmax.  Blocks of 128 keys, since a product of 64 columns takes
-// the tensor core as long as one of 128.
+// other's softmax.  Blocks of 128 keys: with two S buffers of 64 keys instead
+// the products of 64 columns became the bound (16,384 causal tokens, 16 heads
+// of 128: 1.13 ms against 0.97-1.04 ms).
+//
+// Measured: 16,384 causal tokens, 16 heads of 128 on 4 key heads, bf16: 0.97
+// to 1.04 ms, 1,060-1,140 TFLOP/s; 128 images of 393-785 tokens, 6 heads of 64,
+// fp16: 0.19 ms; 64 tokens against caches of up to 8,192, 32 heads on 8 of 128:
+// 0.235 ms, 5.4 TB/s.
 //
 // With few rows and many keys (SPLIT) the keys are divided over grid.y, and
 // within a CTA of two tile slots the blocks alternate between the slots; the
@@ -521,10 +528,10 @@ static Plan plan_of(const mn_packed_args* a) {
   const int64_t blocks = a->tk / a->nseq / 128;
   if (blocks >= 4 && (tiles <= ctas || (int64_t)a->tq * g <= (int64_t)a->nseq * 64)) {
     // the division whose waves of CTAs end first; a CTA's start and end take
-    // it about as long as four blocks of 128 keys
+    // it about as long as four blocks of 128 keys, joining the parts as six
     double best = 0;
     for (int64_t n = 1; n <= 64 && (n == 1 || n * 2 * slots <= blocks); ++n) {
-      const double cost = (double)((tiles * n + ctas - 1) / ctas) * ((double)blocks / n + 4);
+      const double cost = (double)((tiles * n + ctas - 1) / ctas) * ((double)blocks / n + 4) + (n * slots > 1 ? 6 : 0);
       if (n == 1 || cost < best) {
         best = cost;
         pl.splits = (int)n;

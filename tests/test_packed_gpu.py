@@ -109,7 +109,8 @@ def test_bias(dev, spec, causal, dtype):
     check(call(p, causal, True), p, causal)
 
 
-@pytest.mark.parametrize("heads,kv_heads,dim,table_dtype", [(6, 6, 64, torch.float32), (8, 1, 128, torch.bfloat16),
+@pytest.mark.parametrize("heads,kv_heads,dim,table_dtype", [(32, 2, 64, torch.float16), (16, 1, 128, torch.float16), (12, 4, 80, torch.float32),
+                                                            (6, 6, 64, torch.float32), (8, 1, 128, torch.bfloat16),
                                                             (5, 1, 128, torch.float32), (14, 2, 64, torch.float16)])
 def test_bias_heads(dev, heads, kv_heads, dim, table_dtype):
     p = problem(dev, [200, 520], heads=heads, kv_heads=kv_heads, dim=dim, spec=SPEC, table_dtype=table_dtype)
@@ -137,6 +138,88 @@ def test_single_token_with_bias(dev):
 def test_long_sequence(dev):
     p = problem(dev, [2500], heads=4, kv_heads=1, dim=128)
     check(call(p, True, True), p, True)
+
+
+def test_cache_past_32_bit_offsets(dev):
+    """A cache of more than 2^31 values, the sequences at its end; only their
+    rows are ever written."""
+    import mergenet_b200 as mn
+    rows, hk, d = (1 << 21) + 700, 8, 128
+    k = torch.empty(rows, hk, d, device=dev, dtype=torch.bfloat16)
+    v = torch.empty(rows, hk, d, device=dev, dtype=torch.bfloat16)
+    assert k.numel() > 1 << 31
+    p = problem(dev, [3, 1], [300, 400], heads=16, kv_heads=hk, dim=d)
+    k[-700:], v[-700:] = p["k"], p["v"]
+    cu_k = torch.tensor([0, rows - 700, rows - 400, rows], dtype=torch.int32, device=dev)
+    cu_q = torch.tensor([0, 0, 3, 4], dtype=torch.int32, device=dev)
+    want = call(p, True, True)
+    leaves = [t.detach().requires_grad_(True) for t in (p["q"], k, v)]
+    out = mn.packed_attention(*leaves, cu_q, cu_k, causal=True)
+    check({"out": out.detach()}, p, True)
+    gq, gk, gv = torch.autograd.grad(out, leaves, p["dout"])
+    assert torch.equal(gq, want["grad_q"])
+    assert torch.equal(gk[-700:], want["grad_k"]) and torch.equal(gv[-700:], want["grad_v"])
+    assert not gk[:4096].any() and not gk[-4796:-700].any() and not gv[-4796:-700].any()
+
+
+def test_two_streams_at_once(dev):
+    """The same call on two streams at the same time: nothing is shared."""
+    p = [problem(dev, [1] * 4, [9000, 50, 4000, 700], heads=8, kv_heads=2, dim=128, seed=s) for s in (1, 2)]
+    t = [problem(dev, [300, 129], spec=SPEC, seed=s) for s in (3, 4)]
+    want = [call(x, True, False) for x in p], [call(x, True, True) for x in t]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []], [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[0][i].append(call(p[i], True, False))
+                got[1][i].append(call(t[i], True, True))
+    torch.cuda.synchronize()
+    for kind in range(2):
+        for i in range(2):
+            for g in got[kind][i]:
+                for n in g:
+                    assert torch.equal(g[n], want[kind][i][n]), n
+
+
+def test_split_calls_in_captured_graphs(dev):
+    """Two graphs of a call that divides its keys, replayed in turn: each has
+    its own workspace."""
+    import mergenet_b200 as mn
+    p = [problem(dev, [1, 1], [20000, 3000], heads=8, kv_heads=2, dim=128, seed=s) for s in (1, 2)]
+    want = [call(x, True, False)["out"] for x in p]
+    cu_q, cu_k = offsets([1, 1], dev), offsets([20000, 3000], dev)
+    graphs = []
+    for x in p:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mn.packed_attention(x["q"], x["k"], x["v"], cu_q, cu_k, causal=True)
+        graphs.append((graph, out))
+    for order in ((0, 1), (1, 0)):
+        for i in order:
+            graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(graphs[i][1], want[i])
+
+
+def test_leaf_used_twice(dev):
+    """k and v the same tensor: its gradient is the sum of both."""
+    import mergenet_b200 as mn
+    p = problem(dev, [140, 30], heads=4, kv_heads=2, dtype=torch.float16)
+    p["v"] = p["k"]
+    kv = p["k"].detach().requires_grad_(True)
+    q = p["q"].detach().requires_grad_(True)
+    out = mn.packed_attention(q, kv, kv, offsets(p["nq"], dev), causal=True)
+    gq, gkv = torch.autograd.grad(out, [q, kv], p["dout"])
+    val, tol = O.packed_attention(p["q"], p["k"], p["v"], p["nq"], p["nk"], causal=True, dout=p["dout"])
+    total = val["grad_k"] + val["grad_v"]
+    # both gradients are within their bounds, and their sum is rounded once more
+    bound = tol["grad_k"] + tol["grad_v"]
+    assert bool(((gkv.double() - total).abs() <= bound + 2.0 ** -11 * (total.abs() + bound)).all())
+    assert bool(((gq.double() - val["grad_q"]).abs() <= tol["grad_q"]).all())
 
 
 def test_many_sequences(dev):

@@ -94,6 +94,10 @@ def test_bias_refusals():
         _call(bias_table=_half(32, 4), buckets=mn.RelativeBuckets(32, 8192))
     with pytest.raises(ValueError, match="does not fit"):
         _call(bias_table=_half(96, 4), buckets=mn.RelativeBuckets(96, 128))
+    with pytest.raises(ValueError, match="does not fit"):
+        _call(q=_half(6, 34, 64), k=_half(6, 2, 64), v=_half(6, 2, 64), bias_table=_half(32, 34), buckets=b)
+    with pytest.raises(ValueError, match="2\\^30"):
+        mn.relative_position_bias(_half(32, 3), 2, 2, b, query_start=1 << 30)
     with pytest.raises(ValueError, match="negative"):
         mn.relative_position_bias(_half(32, 3), -1, 2, b)
 
