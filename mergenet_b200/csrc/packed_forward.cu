@@ -294,8 +294,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     for (int j = first_of(i); j < end_of(i) && ok; j += kStep, ++c) {
       const int buf = c % NS;
       const uint32_t t_s = tmem + (uint32_t)(i * NS + buf) * kKeys + lane_sel;
-      ok = wait(bars + F::bS + i * NS + buf, (c / NS) & 1, p.err);
-      if (!ok) break;
+      if (!(ok = wait(bars + F::bS + i * NS + buf, (c / NS) & 1, p.err))) break;
       // S(j) is there: K(j) has been read, and V of the block whose P V came before S(j)
       if (wq == 0 && lane == 0) {
         const int jp = j - NS * kStep;
@@ -304,10 +303,10 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
       }
       tc::fence_after_sync();
       const int k0 = j * kKeys;
-      const int nch = (min(kKeys, s.nk - k0) + 31) >> 5;              // chunks of 32 columns that S and P hold
-      const bool fast = nch == kKeys / 32 && kmin >= k0 + kKeys;      // the warp's rows see the whole block
+      const int nch = (min(kKeys, s.nk - k0) + 31) >> 5;          // chunks of 32 columns that S and P hold
+      const bool fast = nch == kKeys / 32 && kmin >= k0 + kKeys;  // the warp's rows see the whole block
+      float f = sl2, add = 0.f;                                   // x enters the softmax as f x + add
       float x[kKeys], mx = -INFINITY;
-      float f = sl2, add = 0.f;  // x enters the softmax as f x + add
       if (__builtin_expect(fast, 1)) {
         if (live) {
           tc::tmem_ld32_nowait(t_s, x);
@@ -327,7 +326,6 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
           if (u < wch) tc::tmem_ld32_nowait(t_s + u * 32, x + u * 32);
         tc::tmem_ld_wait<kKeys>(x);
       }
-      float corr = 1.f;
       if (live) {
         if (BIAS) {
           const int lo = k0 - pmax, hi = k0 + kKeys - 1 - pmin;  // distances of the warp's rows
@@ -349,15 +347,14 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
         }
         if (kKeys == 64 || BIAS || !fast) mx = max32(x + 32, max32(x, mx));
         if constexpr (kKeys == 128) mx = max32(x + 96, max32(x + 64, mx));
-        mx = mx * f + add;
-        const float m_new = fmaxf(m_run, mx);
-        const float m_use = (m_run == -INFINITY || m_new - m_run > kRescaleLog2) ? m_new : m_run;
-        corr = (m_run == -INFINITY || m_use == m_run) ? 1.f : ex2(m_run - m_use);
-        m_run = m_use;
-        // rescale the running output rows, at rest once P V of the block before has completed
-        if (__builtin_expect(c > 0 && __any_sync(MN_FULL_MASK, corr != 1.f), 0)) {
+        const float m_new = fmaxf(m_run, mx * f + add);
+        const bool up = m_new - m_run > kRescaleLog2;  // the first keys of a row included
+        if (__builtin_expect(c > 0 && __any_sync(MN_FULL_MASK, up), 0)) {
+          // rescale the running output rows, at rest once P V of the block before has completed
           if (!(ok = pv_done(c - 1))) break;
           tc::fence_after_sync();
+          const float corr = up ? ex2(m_run - m_new) : 1.f;
+          l_run *= corr;
           float o[32];
 #pragma unroll
           for (int u = 0; u < DT / 32; ++u) {
@@ -367,6 +364,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
             tc::tmem_st32(t_o + u * 32, o);
           }
         }
+        if (up) m_run = m_new;
       }
       const float nm1 = add - (m_run == -INFINITY ? 0.f : m_run);
       const float2 nm = make_float2(nm1, nm1), f2 = make_float2(f, f);
@@ -374,16 +372,18 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
 #pragma unroll
       for (int part = 0; part < F::kParts; ++part) {
         if (live) {
-          uint32_t pk[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float2 y = ffma2(make_float2(x[part * 64 + 2 * e], x[part * 64 + 2 * e + 1]), f2, nm);
-            const float2 q = make_float2(ex2(y.x), ex2(y.y));
-            sum2[e & 1] = fadd2(sum2[e & 1], q);
-            pk[e] = pack2<ET>(q.x, q.y);
+          for (int u = part * 2; u < part * 2 + 2; ++u) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 y = ffma2(make_float2(x[u * 32 + 2 * e], x[u * 32 + 2 * e + 1]), f2, nm);
+              const float2 q = make_float2(ex2(y.x), ex2(y.y));
+              sum2[e & 1] = fadd2(sum2[e & 1], q);
+              pk[e] = pack2<ET>(q.x, q.y);
+            }
+            tc::tmem_st16_nowait(t_s + u * 16, pk);
           }
-          tc::tmem_st16_nowait(t_s + part * 32, pk);
-          tc::tmem_st16_nowait(t_s + part * 32 + 16, pk + 16);
           tc::tmem_wait_st();
         }
         tc::fence_before_sync();
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
         if (lane == 0) tma::arrive(bars + F::bP + (i * NS + buf) * F::kParts + part);
       }
       const float2 ss = fadd2(sum2[0], sum2[1]);
-      l_run = l_run * corr + (ss.x + ss.y);
+      l_run += ss.x + ss.y;
     }
     if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
     if (ok && c > 0) {

@@ -152,13 +152,10 @@ def test_cache_past_32_bit_offsets(dev):
     k[-700:], v[-700:] = p["k"], p["v"]
     cu_k = torch.tensor([0, rows - 700, rows - 400, rows], dtype=torch.int32, device=dev)
     cu_q = torch.tensor([0, 0, 3, 4], dtype=torch.int32, device=dev)
-    want = call(p, True, True)
     leaves = [t.detach().requires_grad_(True) for t in (p["q"], k, v)]
     out = mn.packed_attention(*leaves, cu_q, cu_k, causal=True)
-    check({"out": out.detach()}, p, True)
     gq, gk, gv = torch.autograd.grad(out, leaves, p["dout"])
-    assert torch.equal(gq, want["grad_q"])
-    assert torch.equal(gk[-700:], want["grad_k"]) and torch.equal(gv[-700:], want["grad_v"])
+    check({"out": out.detach(), "grad_q": gq, "grad_k": gk[-700:], "grad_v": gv[-700:]}, p, True)
     assert not gk[:4096].any() and not gk[-4796:-700].any() and not gv[-4796:-700].any()
 
 
