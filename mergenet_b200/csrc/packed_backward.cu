@@ -28,6 +28,7 @@ struct BwdParams {
   mn_packed_args a;
   int group, ntok;
   int span, reach;   // bias: distances held, offset of distance 0
+  int ranked;        // key tiles in descending order of the queries that see them
   float* delta;      // [kv_heads][tq * group]
   float* part;       // [kv_heads][slots][buckets * group] sums of ds by bucket
   int* err;
@@ -501,7 +502,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), C::kCols);
   if (warp == 1) {
-    put_found(misc + 1, seq_of_slot<true>(a, 128, slot_id));
+    put_found(misc + 1, p.ranked ? ranked_slot<true>(a, 128, slot_id) : seq_of_slot<true>(a, 128, slot_id));
   }
   if (warp == 2 && lane == 0) {
     for (int i = 0; i < C::kNumBars; ++i)
@@ -784,6 +785,7 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
   p.group = a->heads / a->kv_heads;
   p.ntok = z.ntok;
   p.span = p.reach = 0;
+  p.ranked = a->nseq > 1 && a->nseq <= kRanked && (z.k_slots - 1) * a->kv_heads > sm_count();  // more than a wave
   if (BIAS) {
     const int last = bo.n ? bo.at[bo.n - 1] : 1;
     p.reach = last;

@@ -83,6 +83,7 @@ struct FwdParams {
   int span, reach;          // bias: distances held, offset of distance 0
   int two_sided;
   int splits;               // grid.y
+  int ranked;               // tiles in descending order of their keys
   float* part_o;            // [part][kv_heads][tq * group][head_dim]
   float* part_lse;          // [part][kv_heads][tq * group]
   int* err;
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), F::kCols);
   if (warp == 1) {
-    put_found(misc + 1, seq_of_slot<false>(a, tile_tokens, slot_id));
+    put_found(misc + 1, SPLIT && p.ranked ? ranked_slot<false>(a, tile_tokens, slot_id) : seq_of_slot<false>(a, tile_tokens, slot_id));
     if (blockIdx.x == 0 && blockIdx.y == 0 && p.err &&
         bad_lengths(a.cu_q, a.cu_k, a.len_k, a.nseq, a.tq, a.tk, lane, 32))
       atomicOr(p.err, MN_STATUS_BAD_LENGTHS);
@@ -515,11 +516,11 @@ int check(const mn_packed_args* a, Borders* bo, bool backward) {
 
 // How the call is divided: 0 parts means whole rows.
 struct Plan {
-  int ntok, parts, splits;
+  int ntok, parts, splits, ranked;
 };
 static Plan plan_of(const mn_packed_args* a) {
   const int g = a->heads / a->kv_heads, slots = a->head_dim <= 64 ? 1 : 2;
-  Plan pl{128 / g, 0, 1};
+  Plan pl{128 / g, 0, 1, 0};
   // Tiles that have rows, at most; a call that leaves the card part empty, or
   // whose tiles are mostly empty rows, and whose sequences are long on average
   // is divided over the keys.
@@ -538,6 +539,7 @@ static Plan plan_of(const mn_packed_args* a) {
       }
     }
     if (pl.splits * slots > 1) pl.parts = pl.splits * slots;
+    pl.ranked = a->nseq > 1 && a->nseq <= kRanked && tiles * pl.splits > ctas;  // more than a wave
   }
   return pl;
 }
@@ -559,6 +561,7 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   p.group = a->heads / a->kv_heads;
   p.ntok = pl.ntok;
   p.splits = pl.splits;
+  p.ranked = pl.ranked;
   p.span = p.reach = p.two_sided = 0;
   if (BIAS) {
     const int last = bo.n ? bo.at[bo.n - 1] : 1;
