@@ -380,9 +380,15 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
             const int gg = i / a.buckets;
             const int2 range = bs.range[i - gg * a.buckets];
             const int o = first[gg], t1 = min(range.y - o, CW - 1 + 31 / G);
-            float sum = 0.f;
-            for (int t = max(range.x - o, 0); t <= t1; ++t) sum += diag[gg * dist + t];
-            my_hist[i] += sum;
+            const float* at = diag + gg * dist;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};  // four chains: a load's way is longer than an addition's
+            int t = max(range.x - o, 0);
+            for (; t + 3 <= t1; t += 4) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) sum[q] += at[t + q];
+            }
+            for (; t <= t1; ++t) sum[0] += at[t];
+            my_hist[i] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           }
           __syncwarp();
         } else if (mine) {
