@@ -31,8 +31,8 @@
 //
 // Measured: 16,384 causal tokens, 16 heads of 128 on 4 key heads, bf16: 0.97
 // to 1.04 ms, 1,060-1,140 TFLOP/s; 128 images of 393-785 tokens, 6 heads of 64,
-// fp16: 0.19 ms; 64 tokens against caches of up to 8,192, 32 heads on 8 of 128:
-// 0.235 ms, 5.4 TB/s.
+// fp16: 0.19 ms; 64 tokens against caches of 700 to 8,192, 32 heads on 8 of 128:
+// 0.227 ms, 5.6 TB/s of the cache in use.
 //
 // With few rows and many keys (SPLIT) the keys are divided over grid.y, and
 // within a CTA of two tile slots the blocks alternate between the slots; the
@@ -81,7 +81,6 @@ struct FwdParams {
   mn_packed_args a;
   int group, ntok;          // heads to a key head, tokens to a tile
   int span, reach;          // bias: distances held, offset of distance 0
-  int two_sided;
   int splits;               // grid.y
   int ranked;               // tiles in descending order of their keys
   float* part_o;            // [part][kv_heads][tq * group][head_dim]
@@ -562,10 +561,9 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   p.ntok = pl.ntok;
   p.splits = pl.splits;
   p.ranked = pl.ranked;
-  p.span = p.reach = p.two_sided = 0;
+  p.span = p.reach = 0;
   if (BIAS) {
     const int last = bo.n ? bo.at[bo.n - 1] : 1;
-    p.two_sided = bo.two_sided;
     p.reach = last;
     p.span = (bo.two_sided ? 2 : 1) * last + 1;
   }

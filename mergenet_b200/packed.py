@@ -190,9 +190,9 @@ def _forward(q, k, v, cu_q, cu_k, len_k, causal, scale, table, buckets, want_lse
     dev = q.device
     q, k, v = _ready(q), _ready(k), _ready(v)
     tq, h, d = q.shape
-    out = torch.empty((tq, h, d), device=dev, dtype=q.dtype)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     hk = k.shape[1]
-    lse = torch.empty((hk, tq, h // hk), device=dev, dtype=torch.float32) if want_lse else None
+    lse = q.new_empty((hk, tq, h // hk), dtype=torch.float32) if want_lse else None
     if tq:
         table = None if table is None else table.contiguous()
         lib = L.lib()
@@ -218,10 +218,8 @@ def _attention_grads(ctx, dout):
     q, k, v, table, cu_q, cu_k, len_k, out, lse = ctx.saved_tensors
     causal, scale, buckets = ctx.call
     dev = q.device
-    dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
-    dv = torch.empty(v.shape, device=dev, dtype=v.dtype)
-    dbias = None if table is None else torch.empty(table.shape, device=dev, dtype=table.dtype)
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+    dbias = None if table is None else torch.empty_like(table, memory_format=torch.contiguous_format)
     if q.numel() == 0:
         for t in (dk, dv, dbias):
             if t is not None:
