@@ -472,19 +472,25 @@ struct Dkv {
   static constexpr int W = NB / 32, CW = 32, kThreads = 32 * (4 * W + 2), kPerSM = NB == 64 ? 2 : 1;
   static constexpr int HV = DT / 64;
   static constexpr uint32_t kTile = HV * kHalfBytes, kQHalf = NB * 128, kQ = HV * kQHalf;
-  static constexpr int NS = DT == 64 && NB == 128 ? 2 : 1;  // S^T buffers in tensor memory
-  static constexpr int QS = NB == 64 ? 3 : NS + 1;  // stages of Q, dout, lse and delta
-  static constexpr uint32_t oK = 0, oV = kTile, oRing = 2 * kTile, oRows = oRing + QS * 2 * kQ;  // rows: [QS][2][NB] floats
-  static constexpr uint32_t oBars = oRows + QS * NB * 8;
-  static constexpr int bKV = 0, bF = 1, bE = bF + QS, bS = bE + QS, bP = bS + NS, bDP = bP + NS, bDS = bDP + 1, bDone = bDS + 1,
-                       bDrain = bDone + 1, kNumBars = bDrain + 1;
+  // Stages of Q and of dout (with lse and delta).  S(i + 1) is issued as soon
+  // as S(i) has been read, so its Q has to be there a tile early: three stages,
+  // but for the bias tables' room at 128 channels.
+  static constexpr int QS = DT == 128 && BIAS ? 2 : 3, OS = 2;
+  // 128 channels then fill shared memory to the last KB: no room for aligning
+  // its start, which the kernel checks instead.
+  static constexpr uint32_t kSlack = DT == 128 && !BIAS ? 0 : 1024;
+  static constexpr uint32_t oK = 0, oV = kTile, oRing = 2 * kTile, oDO = oRing + QS * kQ, oRows = oDO + OS * kQ;  // [OS][2][NB] floats
+  static constexpr uint32_t oBars = oRows + OS * NB * 8;
+  // barriers: K and V landed; Q, dout (and its rows) landed; tile i % 3 done; S ready, read; dP ready; p and ds ready
+  static constexpr int bKV = 0, bF = 1, bO = bF + QS, bE = bO + OS, bS = bE + 3, bSR = bS + 1, bDP = bSR + 1, bDS = bDP + 1,
+                       bDone = bDS + 1, bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
   static constexpr uint32_t oCol = oMisc + 32;  // [NB] (token, head * buckets) of a column
   static constexpr uint32_t oTab = oCol + NB * 8;
   static constexpr uint32_t bytes(int buckets, int group, int span) {
-    return oTab + (BIAS ? bias_bytes(buckets, group, span) : 0) + 1024;
+    return (BIAS ? oTab + bias_bytes(buckets, group, span) : oCol) + kSlack;
   }
-  static constexpr uint32_t cS = 0, cDP = NS * NB, cDV = cDP + NB, cDK = cDV + DT, kCols = NB == 64 ? 256 : 512;
+  static constexpr uint32_t cS = 0, cDP = NB, cDV = cDP + NB, cDK = cDV + DT, kCols = NB == 64 ? 256 : 512;
   static_assert(cDK + DT <= kCols, "tensor memory");
 };
 
@@ -494,8 +500,12 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
                const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const __grid_constant__ BwdParams p, const __grid_constant__ Borders bo) {
   using C = Dkv<DT, NB, BIAS>;
-  constexpr int HV = C::HV, NS = C::NS, QS = C::QS, W = C::W, CW = C::CW;
+  constexpr int HV = C::HV, QS = C::QS, OS = C::OS, W = C::W, CW = C::CW;
   extern __shared__ __align__(16) uint8_t smem_raw[];
+  if (C::kSlack == 0 && (tc::smem_u32(smem_raw) & 1023)) {
+    if (threadIdx.x == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
+    return;
+  }
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(base + C::oMisc);
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
   }
   if (warp == 2 && lane == 0) {
     for (int i = 0; i < C::kNumBars; ++i)
-      tc::mbar_init(bars + i, i >= C::bF && i < C::bE ? 2 : (i >= C::bP && i < C::bDP) || i == C::bDS ? 4 * W : 1);
+      tc::mbar_init(bars + i, i >= C::bO && i < C::bE ? 2 : i == C::bSR || i == C::bDS ? 4 * W : 1);
     tc::fence_mbar_init();
   }
   if (warp == 3 && lane == 0) {
@@ -554,18 +564,28 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
           load_3d(tc::smem_u32(base + C::oV + h * kHalfBytes), &tm_v, h * 64, hk, s.k0 + k0, bars + C::bKV);
         }
       }
-      int done = 0;
+      int q_done = 0, done = 0;
       const int64_t rows = (int64_t)a.tq * G;
       for (int i = 0; i < n && ok; ++i) {
-        const int st = i % QS, t0 = (i0 + i) * p.ntok;
-        if (i >= QS && !(ok = wait(bars + C::bE + st, (i / QS - 1) & 1, p.err))) break;
-        uint8_t* q = base + C::oRing + st * 2 * C::kQ;
+        const int st = i % OS, t0 = (i0 + i) * p.ntok;
+        const uint32_t bytes = (uint32_t)(HV * 128 * G * p.ntok);
+        // tile i - 2 done: its dout stage is free, and with three stages of Q (whose
+        // last tile's end was waited for a turn ago) Q need not wait for it
+        auto before = [&] { return i < 2 || wait(bars + C::bE + (i - 2) % 3, ((i - 2) / 3) & 1, p.err); };
+        if (QS == 2 && !(ok = before())) break;
         if (lane == 0) {
-          tma::expect_tx(bars + C::bF + st, 2u * HV * 128u * (uint32_t)(G * p.ntok));
-          for (int h = 0; h < HV; ++h) {
-            tma::load_4d(tc::smem_u32(q + h * C::kQHalf), &tm_q, h * 64, 0, hk, s.q0 + t0, bars + C::bF + st);
-            tma::load_4d(tc::smem_u32(q + C::kQ + h * C::kQHalf), &tm_do, h * 64, 0, hk, s.q0 + t0, bars + C::bF + st);
-          }
+          tma::expect_tx(bars + C::bF + i % QS, bytes);
+          for (int h = 0; h < HV; ++h)
+            tma::load_4d(tc::smem_u32(base + C::oRing + (i % QS) * C::kQ + h * C::kQHalf), &tm_q, h * 64, 0, hk, s.q0 + t0,
+                         bars + C::bF + i % QS);
+        }
+        q_done = i + 1;
+        if (QS == 3 && !(ok = before())) break;
+        if (lane == 0) {
+          tma::expect_tx(bars + C::bO + st, bytes);
+          for (int h = 0; h < HV; ++h)
+            tma::load_4d(tc::smem_u32(base + C::oDO + st * C::kQ + h * C::kQHalf), &tm_do, h * 64, 0, hk, s.q0 + t0,
+                         bars + C::bO + st);
         }
         // -lse (with the bias where it is the same for the whole tile) and
         // -delta of the rows; rows of no query give p = 0
@@ -586,24 +606,27 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
           x[NB + r] = d;
         }
         __syncwarp();
-        if (lane == 0) tma::arrive(bars + C::bF + st);
+        if (lane == 0) tma::arrive(bars + C::bO + st);
         done = i + 1;
       }
       if (lane == 0) {
         if (!ok && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
         // every copy issued has landed before the CTA may release its shared memory
         wait(bars + C::bKV, 0, nullptr);
-        for (int i = max(0, done - QS); i < done; ++i) wait(bars + C::bF + i % QS, (i / QS) & 1, nullptr);
+        for (int i = max(0, q_done - QS); i < q_done; ++i) wait(bars + C::bF + i % QS, (i / QS) & 1, nullptr);
+        for (int i = max(0, done - OS); i < done; ++i) wait(bars + C::bO + i % OS, (i / OS) & 1, nullptr);
       }
     }
     __syncwarp();
   } else if (warp == 4 * W) {
     // ----------------------------------------------------------------- MMAs
-    // While the compute warps turn S(i) into p the tensor core finishes
-    // dK += ds(i - 1) Q and dP(i); while they form ds(i), dV += p(i) dout and
-    // the next S.
+    // p(i) and ds(i) both go over dP(i), whose values the compute warps have in
+    // registers by then, so S's columns are free from the moment S(i) has been
+    // read: S(i + 1) is computed under the exponentials of tile i, and
+    // dV += p(i) dout, dK += ds(i) Q and dP(i + 1) under those of tile i + 1.
     constexpr uint32_t idesc_s = tc::idesc_f16(ab_bf16, 0, 128, NB), idesc_g = tc::idesc_f16(ab_bf16, 1, 128, DT);
-    auto stage = [&](int i) { return base + C::oRing + (i % QS) * 2 * C::kQ; };
+    auto q_at = [&](int i) { return base + C::oRing + (i % QS) * C::kQ; };
+    auto do_at = [&](int i) { return base + C::oDO + (i % OS) * C::kQ; };
     auto scores = [&](uint32_t d, const uint8_t* x, const uint8_t* y, uint64_t* bar) {
       if (elect_one()) {
         tc::fence_after_sync();
@@ -620,11 +643,15 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
     auto issue_s = [&](int i) -> bool {
       if (!wait(bars + C::bF + i % QS, (i / QS) & 1, p.err)) return false;
       const int valid = min(p.ntok, s.nq - (i0 + i) * p.ntok) * G;
-      if (valid < NB) {  // rows of no query are an operand of dK and dV
-        zero_rows(stage(i), valid, NB, HV, C::kQHalf);
-        zero_rows(stage(i) + C::kQ, valid, NB, HV, C::kQHalf);
-      }
-      scores(tmem + C::cS + (i % NS) * NB, base + C::oK, stage(i), bars + C::bS + i % NS);
+      if (valid < NB) zero_rows(q_at(i), valid, NB, HV, C::kQHalf);  // rows of no query are an operand of dK ...
+      scores(tmem + C::cS, base + C::oK, q_at(i), bars + C::bS);
+      return true;
+    };
+    auto issue_dp = [&](int i) -> bool {
+      if (!wait(bars + C::bO + i % OS, (i / OS) & 1, p.err)) return false;
+      const int valid = min(p.ntok, s.nq - (i0 + i) * p.ntok) * G;
+      if (valid < NB) zero_rows(do_at(i), valid, NB, HV, C::kQHalf);  // ... and of dV
+      scores(tmem + C::cDP, base + C::oV, do_at(i), bars + C::bDP);
       return true;
     };
     auto grads = [&](uint32_t d, uint32_t left, const uint8_t* x, bool more) {  // D += left x
@@ -635,26 +662,19 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
     };
     if (n > 0) {
       ok = wait(bars + C::bKV, 0, p.err);
-      for (int i = 0; i < NS && i < n && ok; ++i) ok = issue_s(i);
-      if (ok) scores(tmem + C::cDP, base + C::oV, stage(0) + C::kQ, bars + C::bDP);
+      ok = ok && issue_s(0) && issue_dp(0);
       for (int i = 0; i < n && ok; ++i) {
-        if (!(ok = wait(bars + C::bP + i % NS, (i / NS) & 1, p.err))) break;
-        if (elect_one()) {
-          tc::fence_after_sync();
-          grads(tmem + C::cDV, tmem + C::cS + (i % NS) * NB, stage(i) + C::kQ, i > 0);
-        }
-        __syncwarp();
-        // S(i + NS) overwrites p(i), which the product before it in order has read
-        if (i + NS < n && !(ok = issue_s(i + NS))) break;
+        if (i + 1 < n && !(ok = wait(bars + C::bSR, i & 1, p.err) && issue_s(i + 1))) break;
         if (!(ok = wait(bars + C::bDS, i & 1, p.err))) break;
         if (elect_one()) {
           tc::fence_after_sync();
-          grads(tmem + C::cDK, tmem + C::cDP, stage(i), i > 0);
-          tc::mma_commit(bars + C::bE + i % QS);
+          grads(tmem + C::cDV, tmem + C::cDP, do_at(i), i > 0);
+          grads(tmem + C::cDK, tmem + C::cDP + CW / 2, q_at(i), i > 0);
+          tc::mma_commit(bars + C::bE + i % 3);
           if (i == n - 1) tc::mma_commit(bars + C::bDone);
         }
         __syncwarp();
-        if (i + 1 < n) scores(tmem + C::cDP, base + C::oV, stage(i + 1) + C::kQ, bars + C::bDP);
+        if (i + 1 < n) ok = issue_dp(i + 1);
       }
       if (!ok && lane == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
       if (elect_one()) {
@@ -670,18 +690,21 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
     const int key = k0 + r;
     const float sl2 = a.scale * kLog2e;
     for (int i = 0; i < n && ok; ++i) {
-      const int st = i % QS, t0 = (i0 + i) * p.ntok;
-      const uint32_t t_s = tmem + C::cS + (i % NS) * NB + w * CW + lane_sel, t_dp = tmem + C::cDP + w * CW + lane_sel;
+      const int st = i % OS, t0 = (i0 + i) * p.ntok;
+      const uint32_t t_s = tmem + C::cS + w * CW + lane_sel, t_dp = tmem + C::cDP + w * CW + lane_sel;
       const float* nl = reinterpret_cast<const float*>(base + C::oRows) + st * 2 * NB + w * CW;
       // columns from here on see this key; the warp's last key sees the latest start
       const int c0 = a.causal ? (key - shift - t0) * G - w * CW : 0;
       const bool masked = a.causal && (k0 + ((warp & 3) * 32 + 31) - shift - t0) * G > w * CW;
-      if (!(ok = wait(bars + C::bF + st, (i / QS) & 1, p.err))) break;  // lse and delta are there
-      if (!(ok = wait(bars + C::bS + i % NS, (i / NS) & 1, p.err))) break;
+      if (!(ok = wait(bars + C::bO + st, (i / OS) & 1, p.err))) break;  // lse and delta are there
+      if (!(ok = wait(bars + C::bS, i & 1, p.err))) break;
       tc::fence_after_sync();
       float x[CW];
       tc::tmem_ld32_nowait(t_s, x);
       tc::tmem_ld_wait<CW>(x);
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tma::arrive(bars + C::bSR);
       if (BIAS && kind_of(t0) == 3) {
         const int at = key - t0 - shift + p.reach;
 #pragma unroll
@@ -706,11 +729,6 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
       }
 #pragma unroll
       for (int e = 0; e < CW; ++e) x[e] = ex2(x[e]);  // hidden keys and columns of no query: exactly 0
-      put32<ET>(t_s, x);
-      tc::tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tma::arrive(bars + C::bP + i % NS);
       if (!(ok = wait(bars + C::bDP, i & 1, p.err))) break;
       tc::fence_after_sync();
       float d[CW];
@@ -723,7 +741,9 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
         const float2 y1 = fmul2(make_float2(x[4 * e + 2], x[4 * e + 3]), fadd2(make_float2(d[4 * e + 2], d[4 * e + 3]), make_float2(nd.z, nd.w)));
         d[4 * e] = y0.x; d[4 * e + 1] = y0.y; d[4 * e + 2] = y1.x; d[4 * e + 3] = y1.y;
       }
-      put32<ET>(t_dp, d);
+      // p over the first half of this thread's columns, ds over the second
+      put32<ET>(t_dp, x);
+      put32<ET>(t_dp + CW / 2, d);
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
