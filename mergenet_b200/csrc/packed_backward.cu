@@ -73,7 +73,7 @@ __device__ __forceinline__ void fill_bias(const BwdParams& p, const Borders& bo,
   for (int i = threadIdx.x; i < p.span; i += threads) s.idx[i] = (uint8_t)bucket_of(bo, i - p.reach);
   for (int i = threadIdx.x; i < p.group * p.a.buckets; i += threads) {
     const int g = i / p.a.buckets, u = i % p.a.buckets;
-    s.tab[i] = load_any(p.a.bias_table, p.a.bias_dtype, (int64_t)u * p.a.heads + hk * p.group + g) * kLog2e;
+    s.tab[i] = table_value(p.a, u, hk * p.group + g);
   }
   for (int u = threadIdx.x; u < p.a.buckets; u += threads) s.range[u] = bucket_range(bo, u);
 }
@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
     const float delta = dl[r] + dl[128 + r];
     if (mine && w == 0) p.delta[hk * rows + row] = delta;
     const float nlse = mine ? -a.lse[hk * rows + row] : -INFINITY;
+    const bool big = __any_sync(MN_FULL_MASK, is_big(nlse));  // scores rounded before lse is taken off, as in the forward
     const float sl2 = a.scale * kLog2e;
     const float* tab = BIAS ? bs.tab + (mine ? g : 0) * a.buckets : nullptr;
     // bias: the warp's sums by (head, bucket), its block's by (head, distance), and each head's first distance
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
       tc::tmem_ld_wait<CW>(x);
       const bool masked = kmin < k0 + CW;
       int kind = 0;  // bias: 1 all below the reach, 2 all above, 3 mixed
-      float add = nlse;
+      float add = big ? 0.f : nlse;
       if (BIAS) {
         kind = k0 + CW - 1 - pmin <= -p.reach ? 1 : k0 - pmax >= p.span - 1 - p.reach ? 2 : 3;
         if (kind == 1) add += tab[bs.idx[0]];
@@ -345,6 +346,10 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
           x[2 * e] = y.x;
           x[2 * e + 1] = y.y;
         }
+      }
+      if (__builtin_expect(big, 0)) {
+#pragma unroll
+        for (int e = 0; e < CW; ++e) x[e] += nlse;
       }
       if (__builtin_expect(masked, 0)) {  // hidden keys get exactly 0
 #pragma unroll
@@ -527,6 +532,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(base + C::oMisc);
+  volatile uint8_t* big = base + C::oMisc + 28;  // [OS] a row's lse is big: scores rounded before it is taken off
   int2* col = reinterpret_cast<int2*>(base + C::oCol);
   const mn_packed_args& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
@@ -611,17 +617,22 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
         const int valid = min(p.ntok, s.nq - t0) * G;
         const int64_t first = hk * rows + (int64_t)(s.q0 + t0) * G;
         const int kind = BIAS ? kind_of(t0) : 0;
+        float l[NB / 32];
+        bool any_big = false;
 #pragma unroll
         for (int e = 0; e < NB / 32; ++e) {
           const int r = e * 32 + lane;
-          float l = -INFINITY, d = 0.f;
-          if (r < valid) {
-            l = -a.lse[first + r];
-            d = -p.delta[first + r];
-            if (BIAS && kind != 3) l += bs.tab[col[r].y + bs.idx[kind == 1 ? 0 : p.span - 1]];
-          }
-          x[r] = l;
-          x[NB + r] = d;
+          l[e] = r < valid ? -a.lse[first + r] : -INFINITY;
+          any_big |= is_big(l[e]);
+          x[NB + r] = r < valid ? -p.delta[first + r] : 0.f;
+        }
+        any_big = __any_sync(MN_FULL_MASK, any_big);
+        if (lane == 0) big[st] = any_big;
+#pragma unroll
+        for (int e = 0; e < NB / 32; ++e) {
+          const int r = e * 32 + lane;
+          if (BIAS && kind != 3 && !any_big && r < valid) l[e] += bs.tab[col[r].y + bs.idx[kind == 1 ? 0 : p.span - 1]];
+          x[r] = l[e];
         }
         __syncwarp();
         if (lane == 0) tma::arrive(bars + C::bO + st);
@@ -723,7 +734,18 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tma::arrive(bars + C::bSR);
-      if (BIAS && kind_of(t0) == 3) {
+      const bool apart = big[st] != 0;
+      if (__builtin_expect(apart, 0)) {
+#pragma unroll
+        for (int e = 0; e < CW; ++e) {
+          float b = 0.f;
+          if (BIAS) {
+            const int2 c = col[w * CW + e];
+            b = bs.tab[c.y + bs.idx[min(max(key - t0 - shift + p.reach - c.x, 0), p.span - 1)]];
+          }
+          x[e] = __fmaf_rn(x[e], sl2, b) + nl[e];
+        }
+      } else if (BIAS && kind_of(t0) == 3) {
         const int at = key - t0 - shift + p.reach;
 #pragma unroll
         for (int e = 0; e < CW; ++e) {

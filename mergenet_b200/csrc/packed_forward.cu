@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
   if (BIAS)
     for (int i = tid; i < G * p.span; i += F::kThreads) {
       const int g = i / p.span, r = i % p.span - p.reach;
-      lut[i] = load_any(a.bias_table, a.bias_dtype, (int64_t)bucket_of(bo, r) * a.heads + hk * G + g) * kLog2e;
+      lut[i] = table_value(a, bucket_of(bo, r), hk * G + g);
     }
   tc::fence_before_sync();
   __syncthreads();
@@ -347,21 +347,30 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
         }
         if (kKeys == 64 || BIAS || !fast) mx = max32(x + 32, max32(x, mx));
         if constexpr (kKeys == 128) mx = max32(x + 96, max32(x + 64, mx));
-        const float m_new = fmaxf(m_run, mx * f + add);
+        const float m_new = fmaxf(m_run, fmaf(mx, f, add));
         const bool up = m_new - m_run > kRescaleLog2;  // the first keys of a row included
-        if (__builtin_expect(c > 0 && __any_sync(MN_FULL_MASK, up), 0)) {
+        const bool big = mine && is_big(m_new);
+        if (__builtin_expect(__any_sync(MN_FULL_MASK, (c > 0 && up) || big), 0)) {
           // rescale the running output rows, at rest once P V of the block before has completed
-          if (!(ok = pv_done(c - 1))) break;
-          tc::fence_after_sync();
-          const float corr = up ? ex2(m_run - m_new) : 1.f;
-          l_run *= corr;
-          float o[32];
+          if (c > 0 && __any_sync(MN_FULL_MASK, up)) {
+            if (!(ok = pv_done(c - 1))) break;
+            tc::fence_after_sync();
+            const float corr = up ? ex2(m_run - m_new) : 1.f;
+            l_run *= corr;
+            float o[32];
 #pragma unroll
-          for (int u = 0; u < DT / 32; ++u) {
-            tc::tmem_ld32(t_o + u * 32, o);
+            for (int u = 0; u < DT / 32; ++u) {
+              tc::tmem_ld32(t_o + u * 32, o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= corr;
-            tc::tmem_st32(t_o + u * 32, o);
+              for (int e = 0; e < 32; ++e) o[e] *= corr;
+              tc::tmem_st32(t_o + u * 32, o);
+            }
+          }
+          if (__any_sync(MN_FULL_MASK, big)) {
+#pragma unroll
+            for (int e = 0; e < kKeys; ++e) x[e] = fmaf(x[e], f, add);
+            f = 1.f;
+            add = 0.f;
           }
         }
         if (up) m_run = m_new;

@@ -32,6 +32,20 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// From 2^16 on (a step of fp32 is then 2^-7) a score is rounded on its own
+// before the row's maximum is taken off it.  One multiply-add for both, with
+// the maximum rounded and the score not, leaves an exponent of up to half a
+// step: 2^16 and more at scores of 10^8, past fp16's range.
+constexpr float kBig = 65536.f;
+__device__ __forceinline__ bool is_big(float x) { return fabsf(x) > kBig && fabsf(x) < INFINITY; }
+// An entry of the bias table in log2 units, held to +-2^17 but for the
+// infinities: a mask's value hides a key as well from there as from -10^9, and
+// the scores beside it, and their row's logarithm, keep steps of 2^-7.
+__device__ __forceinline__ float table_value(const mn_packed_args& a, int bucket, int head) {
+  const float v = load_any(a.bias_table, a.bias_dtype, (int64_t)bucket * a.heads + head);
+  const float y = v * kLog2e;
+  return fabsf(y) > 131072.f && fabsf(v) < INFINITY ? copysignf(131072.f, v) : y;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));

@@ -272,7 +272,10 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
 
     ``bias_table`` [num_buckets, H] (fp32, fp16 or bf16) with ``buckets``
     (RelativeBuckets) adds table[bucket(key position - query position), head].
-    Its gradient is summed in fp32 and rounded once to the table's type.
+    Values beyond +-2^17 ln 2 (90,852) count as that much, a mask's -10^9 or
+    lowest value among them; -inf hides its keys outright, and a query that
+    sees no others comes out as 0.  The table's gradient is summed in fp32 and
+    rounded once to its type.
 
     Scores, softmax statistics and sums are fp32; probabilities and their
     gradients are rounded to the input type before each tensor-core product.

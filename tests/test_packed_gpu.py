@@ -243,6 +243,80 @@ def test_large_scores(dev, amp):
     check(call(p, True, True), p, True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [2.0 ** -3, 1.0, 64.0])
+def test_scores_past_the_integers_of_fp32(dev, scale, dtype):
+    """Scores of 10^7 to 10^10 that fp32 no longer resolves to 1: rows whose
+    best key leads by more than the scores' error take that key alone.  The
+    others stay finite."""
+    p = problem(dev, [300, 1, 150], dtype=dtype, heads=4, kv_heads=2)
+    p["q"], p["k"] = p["q"] * 4000, p["k"] * 4000
+    got = call(p, True, True, scale=scale)
+    for n, x in got.items():
+        if n in ("out", "grad_v"):  # dq and dk have factors of 4000 x scale, past fp16's range
+            assert torch.isfinite(x.float()).all(), n
+    sure = 0
+    r0 = 0
+    for n in p["nq"]:
+        rows = slice(r0, r0 + n)
+        for h in range(4):
+            q, k = p["q"][rows, h].double(), p["k"][rows, h // 2].double()
+            off = (64 + 8) * O.F32 * 2 * scale * (q.abs() @ k.abs().t()).amax(-1)
+            x = (scale * (q @ k.t())).masked_fill(~torch.ones(n, n, dtype=torch.bool, device=dev).tril(), -float("inf"))
+            top = x.topk(min(2, n), dim=-1)
+            lead = top.values[:, 0] - top.values[:, 1] if n > 1 else torch.full((n,), float("inf"), device=dev)
+            clear = lead > 2 * off + 200  # e^-200 is 0 in fp32
+            assert torch.equal(got["out"][rows, h][clear], p["v"][rows, h // 2][top.indices[:, 0]][clear])
+            sure += int(clear.sum())
+        r0 += n
+    assert sure > 900  # of 1,804 rows
+
+
+HIDDEN = [-1e4, -65504.0, -1e9, -1e30, torch.finfo(torch.float32).min, -float("inf")]
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.bfloat16, 64), (torch.float16, 128)])
+@pytest.mark.parametrize("hidden", HIDDEN)
+def test_a_table_that_hides_distances(dev, hidden, dtype, dim):
+    """The outermost buckets at a mask's value: keys that far away have no
+    weight, whichever value it is.  The oracle hides them by -200, whose
+    e^-200 lies below every bound, so that the bounds stay those of the rest."""
+    p = problem(dev, [700, 1, 129], [700, 640, 129], dtype=dtype, dim=dim, spec=SPEC, table_dtype=torch.float32)
+    table = p["table"].clone()
+    for bucket in (15, 31):
+        p["table"][bucket] = -200.0
+        table[bucket] = hidden
+    for causal in (False, True):
+        got = call(dict(p, table=table), causal, True)
+        check(got, p, causal)
+        assert not got["grad_table"][[15, 31]].any()
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("hidden", HIDDEN)
+def test_rows_that_a_table_hides_whole(dev, hidden, dtype, dim):
+    """Queries ahead of all keys, whose buckets are all hidden.  A finite value
+    is the same for all of them and leaves the softmax of the scores (fp32
+    keeps a little of them beside a large value); -inf leaves nothing."""
+    p = problem(dev, [200], [50], dtype=dtype, dim=dim, spec=SPEC, table_dtype=torch.float32)
+    p["table"][16:] = 0.0
+    table = p["table"].clone()
+    table[16:] = hidden
+    ahead = 200 - 50  # rows of positions below 0
+    got = call(dict(p, table=table), False, True)
+    for n, x in got.items():
+        assert torch.isfinite(x.float()).all(), n
+    if hidden == -float("inf"):
+        assert not got["out"][:ahead].any() and not got["grad_q"][:ahead].any()
+        assert not got["grad_table"][16:].any()
+    else:  # weights of the keys within a factor: each output a mean of the values
+        val, tol = O.packed_attention(p["q"], p["k"], p["v"], p["nq"], p["nk"], table=p["table"], spec=p["spec"])
+        # beside 2^17 the sum of a score and the hidden value is off by 2^-7 at
+        # most, in log2 units, and so is the row's logarithm
+        slack = 4 * 2.0 ** -7 * p["v"].double().abs().amax()
+        assert ((got["out"].double() - val["out"]).abs()[:ahead] <= tol["out"][:ahead] + slack).all()
+
+
 def test_growing_maxima(dev):
     """Scores that grow along the keys by far more than one rescale step."""
     p = problem(dev, [600], heads=2, kv_heads=2, dtype=torch.float16)
