@@ -34,7 +34,8 @@
 //
 // Measured (8,192 causal tokens, 16 heads of 128 on 8, bf16): dq 0.36-0.39 ms,
 // dk and dv 0.48 ms; 32 images of 197-785 tokens, 6 heads of 64, fp16, with a
-// bias of 32 buckets: 108 and 94 us.
+// bias of 32 buckets: 94 and 83 us (without it both together 130; with a look-up
+// through the buckets, one chain of shuffles and a lane a bucket 108 and 94).
 #include <algorithm>
 
 #include "packed_tc.cuh"
@@ -52,30 +53,41 @@ struct BwdParams {
   int* err;
 };
 
-// Bias tables of a CTA: value of each (head, bucket) in log2 units, first and
-// last relative position of each bucket, bucket of each distance held.
+// Bias tables of a CTA: the bucket of each distance held, and the values of
+// each head in log2 units.  Up to 64 channels (FLAT) a value per distance, with
+// `pad` more on both sides, so that a warp whose block touches the distances
+// held reads a value per score and needs no clamp; at 128 channels there is
+// room for a value per bucket only.  The compute warps fill them while the first
+// tiles are on their way.
 struct BiasSmem {
-  float* tab;    // [group][buckets]
-  int2* range;   // [buckets]
+  float* val;    // [group][len]
   uint8_t* idx;  // [span]
+  int len;
 };
-__host__ __device__ constexpr uint32_t bias_bytes(int buckets, int group, int span) {
-  return (buckets * group * 4 + 15) / 16 * 16 + buckets * 8 + span;
+template <bool FLAT>
+__host__ __device__ constexpr int bias_len(int buckets, int group, int span, int pad) {
+  // a head's values begin 32 / group banks after the last one's: the lanes of a position read different banks
+  return FLAT ? span + 2 * pad + ((32 / group - span - 2 * pad) & 31) : buckets;
 }
-__device__ __forceinline__ BiasSmem bias_at(uint8_t* at, int buckets, int group) {
+template <bool FLAT>
+__host__ __device__ constexpr uint32_t bias_bytes(int buckets, int group, int span, int pad) {
+  return bias_len<FLAT>(buckets, group, span, pad) * group * 4 + (span + 15) / 16 * 16;
+}
+template <bool FLAT>
+__device__ __forceinline__ BiasSmem bias_at(uint8_t* at, int buckets, int group, int span, int pad) {
   BiasSmem s;
-  s.tab = reinterpret_cast<float*>(at);
-  s.range = reinterpret_cast<int2*>(at + (buckets * group * 4 + 15) / 16 * 16);
-  s.idx = reinterpret_cast<uint8_t*>(s.range + buckets);
+  s.val = reinterpret_cast<float*>(at);
+  s.len = bias_len<FLAT>(buckets, group, span, pad);
+  s.idx = at + s.len * group * 4;
   return s;
 }
-__device__ __forceinline__ void fill_bias(const BwdParams& p, const Borders& bo, int hk, const BiasSmem& s, int threads) {
-  for (int i = threadIdx.x; i < p.span; i += threads) s.idx[i] = (uint8_t)bucket_of(bo, i - p.reach);
-  for (int i = threadIdx.x; i < p.group * p.a.buckets; i += threads) {
-    const int g = i / p.a.buckets, u = i % p.a.buckets;
-    s.tab[i] = table_value(p.a, u, hk * p.group + g);
-  }
-  for (int u = threadIdx.x; u < p.a.buckets; u += threads) s.range[u] = bucket_range(bo, u);
+template <bool FLAT, int THREADS>  // by the compute threads, the first ones of the CTA
+__device__ __forceinline__ void fill_bias(const BwdParams& p, const Borders& bo, int hk, const BiasSmem& s, int pad) {
+  for (int i = threadIdx.x; i < p.span; i += THREADS) s.idx[i] = (uint8_t)bucket_of(bo, i - p.reach);
+  if (FLAT) asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+  for (int g = 0; g < p.group; ++g)
+    for (int i = threadIdx.x; i < s.len; i += THREADS)
+      s.val[g * s.len + i] = table_value(p.a, FLAT ? s.idx[min(max(i - pad, 0), p.span - 1)] : i, hk * p.group + g);
 }
 
 template <typename ET>
@@ -104,12 +116,17 @@ struct Dq {
                        bDone = bDS + 1, bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
   static constexpr uint32_t oDelta = oMisc + 32;             // [2][128] partial deltas
-  // bias: per warp the sums by (head, bucket) and by (head, distance of a block); the bias tables
+  // bias: per warp the sums by (head, bucket) and by (chain of keys, head, distance of a block); the bias tables
+  static constexpr bool kFlat = DT == 64;
+  static constexpr int kChains = DT == 64 ? 4 : 2, kChain = CW / kChains, kPad = 64;
+  static_assert(!kFlat || kPad >= CW + 32, "distances of a warp's block past the ones held");
   static constexpr uint32_t oHist = oDelta + 2 * 128 * 4;
-  static constexpr int diags(int group) { return CW + 32 / group + 1; }  // distances of a warp's rows to CW keys
-  static constexpr uint32_t warp_floats(int buckets, int group) { return buckets * group + group * diags(group) + group; }
+  static constexpr int diags(int group) { return kChain + 32 / group + 1; }  // distances of a warp's rows to a chain's keys
+  static constexpr uint32_t warp_floats(int buckets, int group) {  // a multiple of 4
+    return (buckets * group + kChains * group * diags(group) + group + 3) / 4 * 4;
+  }
   static constexpr uint32_t bytes(int buckets, int group, int span) {
-    return oHist + (BIAS ? 4 * W * warp_floats(buckets, group) * 4 + bias_bytes(buckets, group, span) : 0) + 1024;
+    return oHist + (BIAS ? 4 * W * warp_floats(buckets, group) * 4 + bias_bytes<kFlat>(buckets, group, span, kPad) : 0) + 1024;
   }
   static constexpr uint32_t cS = 0, cDP = 2 * NB, cDQ = 3 * NB, kCols = NB == 64 ? 256 : 512;
   static_assert(cDQ + DT <= kCols, "tensor memory");
@@ -132,7 +149,7 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
   float* hist = reinterpret_cast<float*>(base + C::oHist);
   const int per_warp = BIAS ? C::warp_floats(a.buckets, G) : 0;
   BiasSmem bs;
-  if (BIAS) bs = bias_at(base + C::oHist + 4 * W * per_warp * 4, a.buckets, G);
+  if (BIAS) bs = bias_at<C::kFlat>(base + C::oHist + 4 * W * per_warp * 4, a.buckets, G, p.span, C::kPad);
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), C::kCols);
   if (warp == 1) {
@@ -147,10 +164,6 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
     tma::prefetch_map(&tm_do);
     tma::prefetch_map(&tm_k);
     tma::prefetch_map(&tm_v);
-  }
-  if (BIAS) {
-    fill_bias(p, bo, hk, bs, C::kThreads);
-    for (int i = tid; i < 4 * W * per_warp; i += C::kThreads) hist[i] = 0.f;
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -267,6 +280,11 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
     __syncwarp();
   } else {
     // -------------------------------------------------------------- compute
+    if (BIAS) {
+      fill_bias<C::kFlat, 128 * W>(p, bo, hk, bs, C::kPad);
+      for (int i = tid; i < 4 * W * per_warp; i += 128 * W) hist[i] = 0.f;
+      asm volatile("bar.sync 1, %0;" ::"n"(128 * W) : "memory");
+    }
     const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // part of the columns, row
     const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
     const int my = t0 + r / G, g = r % G;
@@ -307,12 +325,13 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
     const float nlse = mine ? -a.lse[hk * rows + row] : -INFINITY;
     const bool big = __any_sync(MN_FULL_MASK, is_big(nlse));  // scores rounded before lse is taken off, as in the forward
     const float sl2 = a.scale * kLog2e;
-    const float* tab = BIAS ? bs.tab + (mine ? g : 0) * a.buckets : nullptr;
-    // bias: the warp's sums by (head, bucket), its block's by (head, distance), and each head's first distance
+    const float* val = BIAS ? bs.val + (mine ? g : 0) * bs.len : nullptr;
+    const float val_lo = BIAS ? val[C::kFlat ? 0 : bs.idx[0]] : 0.f, val_hi = BIAS ? val[C::kFlat ? bs.len - 1 : bs.idx[p.span - 1]] : 0.f;
+    // bias: the warp's sums by (head, bucket), its block's by (chain, head, distance), and each head's first distance
     float* my_hist = hist + warp * per_warp;
     float* diag = my_hist + a.buckets * G;
     const int dist = BIAS ? C::diags(G) : 0, above = (31 - lane) / G;  // lanes of the same head above this one
-    int* first = reinterpret_cast<int*>(diag + G * dist);
+    int* first = reinterpret_cast<int*>(diag + C::kChains * G * dist);
     float far_lo = 0.f, far_hi = 0.f;
     for (int j = 0; j < n && ok; ++j) {
       const int k0 = j * NB + w * CW;  // this thread's first key
@@ -330,14 +349,16 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
       float add = big ? 0.f : nlse;
       if (BIAS) {
         kind = k0 + CW - 1 - pmin <= -p.reach ? 1 : k0 - pmax >= p.span - 1 - p.reach ? 2 : 3;
-        if (kind == 1) add += tab[bs.idx[0]];
-        if (kind == 2) add += tab[bs.idx[p.span - 1]];
+        if (kind == 1) add += val_lo;
+        if (kind == 2) add += val_hi;
       }
-      const int at = k0 - pos + p.reach;
       if (BIAS && kind == 3) {
+        const int at = k0 - (mine ? pos : pmin) + p.reach;
+        const float* flat = val + at + C::kPad;
 #pragma unroll
         for (int e = 0; e < CW; ++e)
-          if (e / 32 < chunks) x[e] = fmaf(x[e], sl2, tab[bs.idx[min(max(at + e, 0), p.span - 1)]] + add);
+          if (e / 32 < chunks)
+            x[e] = fmaf(x[e], sl2, (C::kFlat ? flat[e] : val[bs.idx[min(max(at + e, 0), p.span - 1)]]) + add);
       } else {
         const float2 f2 = make_float2(sl2, sl2), a2 = make_float2(add, add);
 #pragma unroll
@@ -388,32 +409,58 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
           // distance's sum moves up G lanes a key: a shuffle and an addition
           // a key for the whole warp, and the uppermost lane of each head has
           // the sum of the next distance (the lower lanes hold the last ones).
-          float acc = 0.f;
+          // The keys are cut into chains, whose shuffles run side by side.
+          constexpr int NC = C::kChains, L = C::kChain;
+          float acc[NC];
 #pragma unroll
-          for (int e = 0; e < CW; ++e) {
-            const float below = __shfl_up_sync(MN_FULL_MASK, acc, G);
-            acc = (lane < G ? 0.f : below) + (mine && e / 32 < chunks ? x[e] : 0.f);
-            if (lane >= 32 - G) diag[g * dist + e] = acc;
-          }
-          diag[g * dist + CW - 1 + above] = acc;
+          for (int e = 0; e < L; ++e)
+#pragma unroll
+            for (int q = 0; q < NC; ++q) {
+              const float own = mine && (q * L + e) / 32 < chunks ? x[q * L + e] : 0.f;
+              const float below = e ? __shfl_up_sync(MN_FULL_MASK, acc[q], G) : 0.f;
+              acc[q] = (lane < G ? 0.f : below) + own;
+              if (lane >= 32 - G) diag[(q * G + g) * dist + e] = acc[q];
+            }
+#pragma unroll
+          for (int q = 0; q < NC; ++q) diag[(q * G + g) * dist + L - 1 + above] = acc[q];
           if (above == 0) first[g] = k0 - pos;
           __syncwarp();
-          // a bucket's distances are contiguous: a lane a (head, bucket)
-          for (int i = lane; i < a.buckets * G; i += 32) {
-            const int gg = i / a.buckets;
-            const int2 range = bs.range[i - gg * a.buckets];
-            const int o = first[gg], t1 = min(range.y - o, CW - 1 + 31 / G);
-            const float* at = diag + gg * dist;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};  // four chains: a load's way is longer than an addition's
-            int t = max(range.x - o, 0);
-            for (; t + 3 <= t1; t += 4) {
+          // Sums by bucket over the (head, distance) pairs in order, two a lane and turn:
+          // a bucket's distances are contiguous, so each (head, bucket) is one
+          // run of pairs, and the lane where it ends adds its sum.
+          const int held = CW + 31 / G, all = G * held;  // a head's distances: CW keys, 31 / G + 1 rows
+          for (int i0 = 0; i0 < all; i0 += 64) {
+            float v[2];
+            int to[2];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) sum[q] += at[t + q];
+            for (int h = 0; h < 2; ++h) {
+              const int i = i0 + 2 * lane + h, gg = i / held, t = i - gg * held;
+              v[h] = 0.f;
+              to[h] = -1;
+              if (i < all) {
+#pragma unroll
+                for (int q = 0; q < NC; ++q)
+                  if (t >= q * L && t < q * L + L + 31 / G) v[h] += diag[(q * G + gg) * dist + t - q * L];
+                to[h] = gg * a.buckets + bs.idx[min(max(first[gg] + t + p.reach, 0), p.span - 1)];
+              }
             }
-            for (; t <= t1; ++t) sum[0] += at[t];
-            my_hist[i] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const int before = __shfl_up_sync(MN_FULL_MASK, to[1], 1), after = __shfl_down_sync(MN_FULL_MASK, to[0], 1);
+            // a run goes on through a lane whose two pairs are of it
+            const bool on = lane > 0 && to[0] == to[1] && before == to[0];
+            const unsigned starts = ~__ballot_sync(MN_FULL_MASK, on);
+            const int start = 31 - __clz(starts & (0xffffffffu >> (31 - lane)));  // the lane where the run at this lane's end began
+            float run = v[1] + (to[0] == to[1] ? v[0] : 0.f);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const float t = __shfl_up_sync(MN_FULL_MASK, run, o);
+              if (lane - o >= start) run += t;
+            }
+            const float left = __shfl_up_sync(MN_FULL_MASK, run, 1);
+            if (to[0] != to[1]) my_hist[to[0]] += v[0] + (lane > 0 && before == to[0] ? left : 0.f);
+            __syncwarp();
+            if (to[1] >= 0 && (lane == 31 || after != to[1])) my_hist[to[1]] += run;
+            __syncwarp();
           }
-          __syncwarp();
         } else if (mine) {
           float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
@@ -447,7 +494,7 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
     }
     if (BIAS) {
       __syncwarp();
-      diag[lane] = far_lo;
+      diag[lane] = far_lo;  // at least 64 floats: chains x (chain + 1) of them
       diag[32 + lane] = far_hi;
       __syncwarp();
       if (lane < min(G, 32)) {  // the head of this lane: its rows are G lanes apart
@@ -508,10 +555,14 @@ struct Dkv {
   static constexpr int bKV = 0, bF = 1, bO = bF + QS, bE = bO + OS, bS = bE + 3, bSR = bS + 1, bDP = bSR + 1, bDS = bDP + 1,
                        bDone = bDS + 1, bDrain = bDone + 1, kNumBars = bDrain + 1;
   static constexpr uint32_t oMisc = oBars + ((kNumBars * 8 + 15) / 16) * 16;
-  static constexpr uint32_t oCol = oMisc + 32;  // [NB] (token, head * buckets) of a column
+  static constexpr bool kFlat = DT == 64;
+  static constexpr int pad(int group) { return 128 + NB / group + 2; }  // distances of a tile pair past the ones held
+  // of a column, [NB] each: its token, and the place of its head's first value; FLAT: that place less the token instead
+  // of the token
+  static constexpr uint32_t oCol = oMisc + 32;
   static constexpr uint32_t oTab = oCol + NB * 8;
   static constexpr uint32_t bytes(int buckets, int group, int span) {
-    return (BIAS ? oTab + bias_bytes(buckets, group, span) : oCol) + kSlack;
+    return (BIAS ? oTab + bias_bytes<kFlat>(buckets, group, span, pad(group)) : oCol) + kSlack;
   }
   static constexpr uint32_t cS = 0, cDP = NB, cDV = cDP + NB, cDK = cDV + DT, kCols = NB == 64 ? 256 : 512;
   static_assert(cDK + DT <= kCols, "tensor memory");
@@ -533,12 +584,12 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(base + C::oMisc);
   volatile uint8_t* big = base + C::oMisc + 28;  // [OS] a row's lse is big: scores rounded before it is taken off
-  int2* col = reinterpret_cast<int2*>(base + C::oCol);
+  int *col = reinterpret_cast<int*>(base + C::oCol), *col_val = col + NB;
   const mn_packed_args& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
   const int hk = blockIdx.x % a.kv_heads, slot_id = blockIdx.x / a.kv_heads;
   BiasSmem bs;
-  if (BIAS) bs = bias_at(base + C::oTab, a.buckets, G);
+  if (BIAS) bs = bias_at<C::kFlat>(base + C::oTab, a.buckets, G, p.span, C::pad(G));
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), C::kCols);
   if (warp == 1) {
@@ -554,10 +605,6 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
     tma::prefetch_map(&tm_do);
     tma::prefetch_map(&tm_k);
     tma::prefetch_map(&tm_v);
-  }
-  if (BIAS) {
-    fill_bias(p, bo, hk, bs, C::kThreads);
-    if (tid < NB) col[tid] = make_int2(tid / G, (tid % G) * a.buckets);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -611,12 +658,17 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
             tma::load_4d(tc::smem_u32(base + C::oDO + st * C::kQ + h * C::kQHalf), &tm_do, h * 64, 0, hk, s.q0 + t0,
                          bars + C::bO + st);
         }
+        if (BIAS && i == 0) {  // the bias tables are there
+          __syncwarp();
+          asm volatile("bar.sync 2, %0;" ::"n"(128 * W + 32) : "memory");
+        }
         // -lse (with the bias where it is the same for the whole tile) and
         // -delta of the rows; rows of no query give p = 0
         float* x = reinterpret_cast<float*>(base + C::oRows) + st * 2 * NB;
         const int valid = min(p.ntok, s.nq - t0) * G;
         const int64_t first = hk * rows + (int64_t)(s.q0 + t0) * G;
         const int kind = BIAS ? kind_of(t0) : 0;
+        const int lo = !BIAS || C::kFlat ? 0 : bs.idx[0], hi = !BIAS ? 0 : C::kFlat ? bs.len - 1 : bs.idx[p.span - 1];
         float l[NB / 32];
         bool any_big = false;
 #pragma unroll
@@ -631,7 +683,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
 #pragma unroll
         for (int e = 0; e < NB / 32; ++e) {
           const int r = e * 32 + lane;
-          if (BIAS && kind != 3 && !any_big && r < valid) l[e] += bs.tab[col[r].y + bs.idx[kind == 1 ? 0 : p.span - 1]];
+          if (BIAS && kind != 3 && !any_big && r < valid) l[e] += bs.val[col_val[r] + (kind == 1 ? lo : hi)];
           x[r] = l[e];
         }
         __syncwarp();
@@ -714,6 +766,14 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
     __syncwarp();
   } else {
     // -------------------------------------------------------------- compute
+    if (BIAS && n > 0) {
+      fill_bias<C::kFlat, 128 * W>(p, bo, hk, bs, C::pad(G));
+      if (tid < NB) {
+        col_val[tid] = tid % G * bs.len;
+        col[tid] = C::kFlat ? col_val[tid] - tid / G : tid / G;
+      }
+      asm volatile("bar.sync 2, %0;" ::"n"(128 * W + 32) : "memory");  // with the load warp
+    }
     const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // part of the columns, key row
     const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
     const int key = k0 + r;
@@ -735,22 +795,30 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
       __syncwarp();
       if (lane == 0) tma::arrive(bars + C::bSR);
       const bool apart = big[st] != 0;
+      const int at = key - t0 - shift + p.reach;  // place of token 0's distance among those held
+      const float* flat = bs.val + at + C::pad(G);
+      auto bias = [&](int c, int cv) {  // of a column, in a tile pair that touches the distances held
+        return C::kFlat ? flat[c] : bs.val[cv + bs.idx[min(max(at - c, 0), p.span - 1)]];
+      };
+      auto bias_any = [&](int c, int cv) {  // in any tile pair
+        return C::kFlat ? bs.val[cv + min(max(at + C::pad(G) + c - cv, 0), bs.len - 1)] : bias(c, cv);
+      };
       if (__builtin_expect(apart, 0)) {
 #pragma unroll
         for (int e = 0; e < CW; ++e) {
-          float b = 0.f;
-          if (BIAS) {
-            const int2 c = col[w * CW + e];
-            b = bs.tab[c.y + bs.idx[min(max(key - t0 - shift + p.reach - c.x, 0), p.span - 1)]];
-          }
+          const float b = BIAS ? bias_any(col[w * CW + e], col_val[w * CW + e]) : 0.f;
           x[e] = __fmaf_rn(x[e], sl2, b) + nl[e];
         }
       } else if (BIAS && kind_of(t0) == 3) {
-        const int at = key - t0 - shift + p.reach;
 #pragma unroll
-        for (int e = 0; e < CW; ++e) {
-          const int2 c = col[w * CW + e];
-          x[e] = fmaf(x[e], sl2, nl[e] + bs.tab[c.y + bs.idx[min(max(at - c.x, 0), p.span - 1)]]);
+        for (int e = 0; e < CW / 4; ++e) {
+          const float4 l = reinterpret_cast<const float4*>(nl)[e];
+          const int4 c = reinterpret_cast<const int4*>(col + w * CW)[e];
+          const int4 cv = C::kFlat ? c : reinterpret_cast<const int4*>(col_val + w * CW)[e];
+          x[4 * e] = fmaf(x[4 * e], sl2, l.x + bias(c.x, cv.x));
+          x[4 * e + 1] = fmaf(x[4 * e + 1], sl2, l.y + bias(c.y, cv.y));
+          x[4 * e + 2] = fmaf(x[4 * e + 2], sl2, l.z + bias(c.z, cv.z));
+          x[4 * e + 3] = fmaf(x[4 * e + 3], sl2, l.w + bias(c.w, cv.w));
         }
       } else {
         const float2 f2 = make_float2(sl2, sl2);

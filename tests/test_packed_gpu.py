@@ -557,3 +557,12 @@ def test_both_together_in_a_training_step(dev):
     # each gradient is rounded to fp32, and their sum again
     assert bool(((table.grad.double() - total).abs() <= tol["grad_table"] + more_tol + 3 * O.F32 * total.abs()).all())
     assert all(t.grad is not None and torch.isfinite(t.grad).all() for t in (q, k, v))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,spec", [(16, 1, 128, (48, 255, True)), (16, 1, 64, (48, 255, True)), (1, 1, 64, (48, 4000, True)),
+                                                     (2, 2, 128, (48, 8191, False)), (9, 3, 64, (40, 300, False)), (14, 2, 96, (6, 5, True))])
+def test_largest_bias_tables(dev, heads, kv_heads, dim, spec):
+    """Tables that take all the room there is for them, and groups that do not
+    divide a warp."""
+    p = problem(dev, [330, 1, 140], [330, 400, 61], heads=heads, kv_heads=kv_heads, dim=dim, spec=spec, table_dtype=torch.float32)
+    check(call(p, False, True), p, False)
