@@ -71,7 +71,11 @@ struct Fwd {
                        bPV = bP + NQ * NS * kParts, bDrain = bPV + NQ * NS, kNumBars = bDrain + 1;
   static constexpr uint32_t kMisc = kBars + ((kNumBars * 8 + 15) / 16) * 16;  // TMEM base, sequence
   static constexpr uint32_t kLut = kMisc + 32;
-  static constexpr uint32_t bytes(uint32_t lut_floats) { return kLut + lut_floats * 4 + 1024; }
+  // Bias: a value per distance and head.  Up to 64 channels with a margin on
+  // both sides, so that a warp whose block touches the distances held needs no
+  // clamp (NOCLAMP); at 128 channels there is no room for it.
+  static constexpr int margin(int group) { return DT == 64 ? KB + 32 / group + 1 : 0; }
+  static constexpr uint32_t bytes(int group, int span) { return kLut + (BIAS ? group * (span + 2 * margin(group)) * 4 : 0) + 1024; }
   // TMEM columns: the slots' S buffers, then their O
   static constexpr uint32_t kCols = DT == 64 ? 256 : 512, cO = NQ * NS * KB;
   static_assert(cO + NQ * DT <= kCols, "tensor memory");
@@ -105,6 +109,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
   const int hk = blockIdx.x % a.kv_heads, slot_id = blockIdx.x / a.kv_heads;
   const int tile_tokens = SPLIT ? p.ntok : NQ * p.ntok;  // SPLIT: both slots work on one tile
   const int G = p.group;
+  const int margin = BIAS ? F::margin(G) : 0, row_len = p.span + 2 * margin;
 
   if (warp == 0) tc::tmem_alloc(const_cast<uint32_t*>(misc), F::kCols);
   if (warp == 1) {
@@ -124,8 +129,8 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     tma::prefetch_map(&tm_v);
   }
   if (BIAS)
-    for (int i = tid; i < G * p.span; i += F::kThreads) {
-      const int g = i / p.span, r = i % p.span - p.reach;
+    for (int i = tid; i < G * row_len; i += F::kThreads) {
+      const int g = i / row_len, r = i % row_len - margin - p.reach;
       lut[i] = table_value(a, bucket_of(bo, r), hk * G + g);
     }
   tc::fence_before_sync();
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
     const int kmin = __reduce_min_sync(MN_FULL_MASK, klim), kmax = __reduce_max_sync(MN_FULL_MASK, mine ? klim : 0);
     const int pmin = __reduce_min_sync(MN_FULL_MASK, mine ? pos : 0x7fffffff);
     const int pmax = __reduce_max_sync(MN_FULL_MASK, mine ? pos : -0x7fffffff);
-    const float* row_lut = lut + (BIAS ? (mine ? g : 0) * p.span : 0);
+    const float* row_lut = lut + (BIAS ? (mine ? g : 0) * row_len : 0);
     float m_run = -INFINITY, l_run = 0.f;
     int c = 0;
     const int total = first_of(i) < end_of(i) ? (end_of(i) - first_of(i) + kStep - 1) / kStep : 0;
@@ -332,11 +337,11 @@ __global__ void __launch_bounds__(Fwd<DT, BIAS>::kThreads, DT == 64 ? 2 : 1)
           if (hi <= -p.reach) {
             add = row_lut[0];
           } else if (lo >= p.span - 1 - p.reach) {
-            add = row_lut[p.span - 1];
+            add = row_lut[row_len - 1];
           } else {
-            const int at = k0 - pos + p.reach;
+            const int at = k0 - (mine ? pos : pmin) + p.reach + margin;
 #pragma unroll
-            for (int e = 0; e < kKeys; ++e) x[e] = fmaf(x[e], sl2, row_lut[min(max(at + e, 0), p.span - 1)]);
+            for (int e = 0; e < kKeys; ++e) x[e] = fmaf(x[e], sl2, row_lut[DT == 64 ? at + e : min(max(at + e, 0), p.span - 1)]);
             f = 1.f;
           }
         }
@@ -580,7 +585,7 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   p.part_lse = p.part_o + (size_t)pl.parts * a->tq * a->heads * a->head_dim;
   p.err = err;
   if ((int64_t)a->tq * a->heads > 0x7fffffff) return false;
-  const size_t smem = F::bytes(p.span * p.group);
+  const size_t smem = F::bytes(p.group, p.span);
   auto kern = forward_kernel<ET, DT, BIAS, SPLIT>;
   if (!ensure_smem(kern, smem) || !launch_regs(kern, F::kLaunchRegs)) return false;
   const int64_t slots = tile_slots(a->tq, a->nseq, SPLIT ? pl.ntok : F::NQ * pl.ntok) * a->kv_heads;
