@@ -13,7 +13,7 @@ struct Borders {
   int n;
   int two_sided;
   int side;  // buckets to a side
-  int at[kMaxBorders];
+  int at[(kMaxBorders + 7) / 8 * 8];  // behind the last one: beyond every distance
 };
 
 // Bucket of r = key position - query position: the number of borders at or
@@ -21,7 +21,9 @@ struct Borders {
 __device__ __forceinline__ int bucket_of(const Borders& b, int r) {
   const int n = b.two_sided ? abs(r) : max(-r, 0);
   int u = 0;
-  for (int i = 0; i < b.n; ++i) u += b.at[i] <= n ? 1 : 0;
+  for (int i = 0; i < b.n; i += 8)  // eight reads on their way at a time
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u += b.at[i + e] <= n ? 1 : 0;
   return u + (b.two_sided && r > 0 ? b.side : 0);
 }
 
@@ -47,6 +49,7 @@ inline bool make_borders(Borders* b, int buckets, int two_sided, int num_borders
     if (at[i] < 1 || (i > 0 && at[i] < at[i - 1])) return false;
     b->at[i] = at[i];
   }
+  for (int i = num_borders; i < (kMaxBorders + 7) / 8 * 8; ++i) b->at[i] = 0x7fffffff;
   return true;
 }
 
