@@ -29,7 +29,7 @@
 // the products of 64 columns became the bound (16,384 causal tokens, 16 heads
 // of 128: 1.13 ms against 0.97-1.04 ms).
 //
-// Measured: 16,384 causal tokens, 16 heads of 128 on 4 key heads, bf16: 0.97
+// Measured: 16,384 causal tokens, 16 heads of 128 on 4 key heads, bf16: 0.95
 // to 1.04 ms, 1,060-1,140 TFLOP/s; 128 images of 393-785 tokens, 6 heads of 64,
 // fp16: 0.19 ms; 64 tokens against caches of 700 to 8,192, 32 heads on 8 of 128:
 // 0.227 ms, 5.6 TB/s of the cache in use.
@@ -73,7 +73,8 @@ struct Fwd {
   static constexpr uint32_t kLut = kMisc + 32;
   // Bias: a value per distance and head.  Up to 64 channels with a margin on
   // both sides, so that a warp whose block touches the distances held needs no
-  // clamp (NOCLAMP); at 128 channels there is no room for it.
+  // clamp (forward over 32 images with a bias of 32 buckets: 60 -> 56 us); at 128
+  // channels there is no room for it.
   static constexpr int margin(int group) { return DT == 64 ? KB + 32 / group + 1 : 0; }
   static constexpr uint32_t bytes(int group, int span) { return kLut + (BIAS ? group * (span + 2 * margin(group)) * 4 : 0) + 1024; }
   // TMEM columns: the slots' S buffers, then their O

@@ -1,5 +1,5 @@
 // Tensor-core plumbing shared by the packed attention's forward and backward:
-// tensor maps of packed rows, tile lookup, the two exponentials.
+// tensor maps of packed rows, tile lookup, bias values, waits.
 #pragma once
 
 #include <type_traits>
