@@ -344,8 +344,8 @@ int mn_attention(int batch, int nq, int nk, int heads, int head_dim, int dtype,
  * lse [kv_heads, tq, heads / kv_heads] fp32: log2 of each row's sum of
  * exponentials (+inf where no key is seen); NULL when no backward follows.
  * status: MN_STATUS_BAD_LENGTHS for offsets that decrease or leave the tensors
- * and lengths that leave their slots (no access follows them out), and
- * MN_STATUS_TC_TIMEOUT. */
+ * and lengths that leave their slots (no access follows them out; calls that
+ * share the word are not affected by this bit), and MN_STATUS_TC_TIMEOUT. */
 typedef struct mn_packed_args {
   const void *q, *k, *v;
   const int32_t *cu_q, *cu_k, *len_k;

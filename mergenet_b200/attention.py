@@ -23,7 +23,10 @@ def _status(dev):
 
 def attention_status(device=None, reset=False):
     """Error bits recorded by attention kernels on ``device`` (sticky until
-    reset; reading synchronises)."""
+    reset; reading synchronises).  MN_STATUS_TC_TIMEOUT: a bounded wait gave
+    up, results are not to be used, and later calls give up early until the
+    reset.  MN_STATUS_BAD_LENGTHS: a ``packed_attention`` call had offsets or
+    lengths out of range; it concerns that call's results alone."""
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     st = _status(dev)
     val = int(st.item())

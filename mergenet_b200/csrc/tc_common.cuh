@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "mergenet_b200.h"
+
 namespace mn {
 namespace tc {
 
@@ -29,8 +31,9 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 
 // Wait for the phase with the given parity to complete.  Bounded in time:
 // gives up (returns false) after `limit_ns`, or early once another CTA has
-// recorded an error in *err, so a stuck wait costs each CTA at most the
-// bound and the grid drains quickly.
+// recorded a timeout in *err, so a stuck wait costs each CTA at most the
+// bound and the grid drains quickly.  The word's other bits are conditions of
+// the data of some call, and no reason to leave a wait.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const int* err = nullptr,
                                           uint64_t limit_ns = 100000000ull) {
   const uint32_t addr = smem_u32(bar);
@@ -49,7 +52,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const 
       const uint64_t now = globaltimer_ns();
       if (i == 0) t0 = now;
       else if (now - t0 > limit_ns) return false;
-      if (err && *reinterpret_cast<const volatile int*>(err) != 0) return false;
+      if (err && (*reinterpret_cast<const volatile int*>(err) & MN_STATUS_TC_TIMEOUT)) return false;
     }
   }
 }

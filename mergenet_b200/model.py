@@ -403,15 +403,19 @@ class MergeNetSmall(nn.Module):
         """Raise if the last forward's routing (or the routing call whose
         status word is given) flagged a data condition, or an attention
         kernel's bounded wait gave up (reads the device status words, which
-        synchronises)."""
+        synchronises).  Offsets of a ``packed_attention`` call that were out
+        of range are recorded in the same word; the model makes no such call,
+        so they are not its error."""
+        from . import _lib as L
         from .attention import attention_status
         from .routing import check_status
         status = route_status if route_status is not None else getattr(self, "_route_status", None)
         if status is not None:
             check_status(status)
-            st = attention_status(status.device)
+            st = attention_status(status.device) & ~L.MN_STATUS_BAD_LENGTHS
             if st:
-                raise RuntimeError(f"attention kernel status {st:#x} (a bounded tensor-core wait gave up)")
+                what = "a bounded tensor-core wait gave up" if st & L.MN_STATUS_TC_TIMEOUT else "unknown condition"
+                raise RuntimeError(f"attention kernel status {st:#x} ({what})")
 
 
 class ForwardGraph:

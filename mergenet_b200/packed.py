@@ -286,7 +286,8 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
 
     Offsets are read on the device and not checked on the host: those that
     decrease or pass the tensors' ends leave the results undefined, touch no
-    other memory, and set MN_STATUS_BAD_LENGTHS in attention_status()."""
+    other memory, and set MN_STATUS_BAD_LENGTHS in attention_status(), where it
+    stays until reset.  Other calls are not affected."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"q, k and v must be [rows, heads, head_dim], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     tq, h, d = q.shape
