@@ -370,7 +370,9 @@ int mn_packed_attention(const mn_packed_args* args, void* workspace,
 
 /* Gradients of mn_packed_attention: reads its out and lse and dout, writes
  * dq, dk, dv (rows of no sequence and unused key rows get 0) and, with a
- * bias_table, dbias.  Every sum has a fixed order.  tq is at least 1 (without
+ * bias_table, dbias.  Every sum has a fixed order.  In fp16 the probabilities
+ * and score gradients are held times powers of two that keep them in its
+ * range whatever the upstream gradients' size.  tq is at least 1 (without
  * a query every gradient is 0). */
 size_t mn_packed_attention_backward_workspace_bytes(const mn_packed_args* args);
 int mn_packed_attention_backward(const mn_packed_args* args, void* workspace,

@@ -50,8 +50,84 @@ struct BwdParams {
   int ranked;        // key tiles in descending order of the queries that see them
   float* delta;      // [kv_heads][tq * group]
   float* part;       // [kv_heads][slots][buckets * group] sums of ds by bucket
+  unsigned* norms;   // fp16: [nseq][kv_heads][2] bits of the a bound of the largest squared norm of a row of dout, of v
   int* err;
 };
+
+// p and ds of fp16 inputs.  As they stand they would leave its range: ds
+// passes 65,504 under the upstream gradients of a large loss scale and has
+// steps of 2^-24 under small ones, and a weight below 2^-14 loses bits (one of
+// 16,384 equal keys).  So dv takes 2^14 p, and dq and dk take 2^s ds, with one
+// s for all rows of a sequence and key head, from |ds| <= |dp - delta| <=
+// 2 max|dout| max|v| (delta = dout . out, out a mean of the v); the powers are
+// taken off the fp32 sums.  bf16 has the range of fp32.
+constexpr int kPowerP = 14;
+template <typename ET>
+constexpr bool kPowers = std::is_same<ET, __half>::value;
+__device__ __forceinline__ int power_of(const unsigned* norms) {  // s: 2 max|dout| max|v| 2^s <= 2^15, by the bounds of both
+  const unsigned x = norms[0], y = norms[1];
+  if (x == 0 || y == 0) return 0;
+  const int e = (int)(x >> 23) + (int)(y >> 23) - 252;  // (max|dout| max|v|)^2 < 2^e
+  return min(max(14 - ((e + 1) >> 1), -40), 40);
+}
+__device__ __forceinline__ float pow2(int n) { return __int_as_float((127 + n) << 23); }
+
+// The norms: a block takes 256 rows of (token, head of the group) of dout, or
+// 256 keys of v, of one sequence and key head; a maximum depends on no order.
+// A vector's eight channels of the largest sum stand for all of its eights:
+// a bound within two bits, and no shuffles (15 us with them).
+// Rows of no sequence and unused keys are not looked at, and rows with an
+// infinity or a NaN do not count (their results show it in any case).
+// 32 images of 197-785 tokens, 6 heads of 64: 10 us (24 MB from a cold cache),
+// and the training step with a bias 231 -> 246 us.
+__host__ __device__ constexpr int norm_tokens(int group) { return 256 / group; }
+constexpr int kNormKeys = 256;
+__global__ void __launch_bounds__(256) norms_kernel(const __grid_constant__ BwdParams p, int q_slots) {
+  __shared__ uint32_t found_at[8];
+  __shared__ float most[8];
+  const mn_packed_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
+  const int hk = blockIdx.x % a.kv_heads, slot = blockIdx.x / a.kv_heads;
+  const bool keys = slot >= q_slots;
+  if (warp == 0)
+    put_found(found_at, keys ? seq_of_slot<true>(a, kNormKeys, slot - q_slots) : seq_of_slot<false>(a, norm_tokens(G), slot));
+  __syncthreads();
+  const Found f = get_found(found_at);
+  if (f.seq >= a.nseq || f.local < 0) return;
+  const int t0 = f.local * (keys ? kNormKeys : norm_tokens(G));
+  const int n = keys ? min(kNormKeys, f.s.nk - t0) : min(norm_tokens(G), f.s.nq - t0) * G;  // vectors of the block
+  const int width = a.head_dim / 8;
+  int lanes = 1;  // a vector's lanes, eight channels each
+  while (lanes < width) lanes *= 2;
+  const int sub = lane % lanes, step = 8 * (32 / lanes);  // vectors of the block at a time
+  float m = 0.f;
+  for (int i0 = warp * (32 / lanes) + lane / lanes; i0 < n; i0 += 8 * step) {
+    uint4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * step;
+      const __half* row = keys ? static_cast<const __half*>(a.v) + (int64_t)(f.s.k0 + t0 + i) * a.v_st + hk * a.v_sh
+                               : static_cast<const __half*>(a.dout) + (int64_t)(f.s.q0 + t0 + i / G) * a.do_st + (hk * G + i % G) * a.do_sh;
+      v[u] = i < n && sub < width ? *reinterpret_cast<const uint4*>(row + sub * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const __half* e = reinterpret_cast<const __half*>(&v[u]);
+      float x = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) x = fmaf(to_f32(e[c]), to_f32(e[c]), x);
+      if (x < INFINITY) m = fmaxf(m, x);
+    }
+  }
+  m *= width;  // at least the largest of the vectors' sums
+  m = warp_max(m);
+  if (lane == 0) most[warp] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) m = fmaxf(m, most[w]);
+    if (m > 0.f) atomicMax(p.norms + ((int64_t)f.seq * a.kv_heads + hk) * 2 + (keys ? 1 : 0), __float_as_uint(m));
+  }
+}
 
 // Bias tables of a CTA: the bucket of each distance held, and the values of
 // each head in log2 units.  Up to 64 channels (FLAT) a value per distance, with
@@ -295,6 +371,9 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
     const int pmin = __reduce_min_sync(MN_FULL_MASK, mine ? pos : 0x7fffffff);
     const int pmax = __reduce_max_sync(MN_FULL_MASK, mine ? pos : -0x7fffffff);
     const int64_t row = (int64_t)(s.q0 + my) * G + g, rows = (int64_t)a.tq * G;
+    int power = 0;  // fp16: p enters as 2^power p, so that ds comes out as 2^power ds
+    if (kPowers<ET>) power = n > 0 ? power_of(p.norms + ((int64_t)found.seq * a.kv_heads + hk) * 2) : 0;
+    const float lift = (float)power, off = pow2(-power);
     // delta = dout . out, the channels in 8s in turn to the row's threads
     float* dl = reinterpret_cast<float*>(base + C::oDelta);
     {
@@ -346,7 +425,7 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
       tc::tmem_ld_wait<CW>(x);
       const bool masked = kmin < k0 + CW;
       int kind = 0;  // bias: 1 all below the reach, 2 all above, 3 mixed
-      float add = big ? 0.f : nlse;
+      float add = big ? 0.f : kPowers<ET> ? nlse + lift : nlse;
       if (BIAS) {
         kind = k0 + CW - 1 - pmin <= -p.reach ? 1 : k0 - pmax >= p.span - 1 - p.reach ? 2 : 3;
         if (kind == 1) add += val_lo;
@@ -370,7 +449,7 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
       }
       if (__builtin_expect(big, 0)) {
 #pragma unroll
-        for (int e = 0; e < CW; ++e) x[e] += nlse;
+        for (int e = 0; e < CW; ++e) x[e] = kPowers<ET> ? (x[e] + nlse) + lift : x[e] + nlse;
       }
       if (__builtin_expect(masked, 0)) {  // hidden keys get exactly 0
 #pragma unroll
@@ -488,7 +567,7 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
         }
-        if (mine) store32<ET>(dst, c0, a.head_dim, o, a.scale);
+        if (mine) store32<ET>(dst, c0, a.head_dim, o, kPowers<ET> ? a.scale * off : a.scale);
         __syncwarp();
       }
     }
@@ -513,7 +592,7 @@ __global__ void __launch_bounds__(Dq<DT, NB, BIAS>::kThreads, Dq<DT, NB, BIAS>::
         const int at = i % G * a.buckets + i / G;
         float acc = 0.f;
         for (int ww = 0; ww < 4 * W; ++ww) acc += hist[ww * per_warp + at];
-        p.part[(hk * slots + slot_id) * per + i] = acc;
+        p.part[(hk * slots + slot_id) * per + i] = kPowers<ET> ? acc * off : acc;
       }
     }
   }
@@ -559,7 +638,7 @@ struct Dkv {
   static constexpr int pad(int group) { return 128 + NB / group + 2; }  // distances of a tile pair past the ones held
   // of a column, [NB] each: its token, and the place of its head's first value; FLAT: that place less the token instead
   // of the token
-  static constexpr uint32_t oCol = oMisc + 32;
+  static constexpr uint32_t oCol = oMisc + 48;
   static constexpr uint32_t oTab = oCol + NB * 8;
   static constexpr uint32_t bytes(int buckets, int group, int span) {
     return (BIAS ? oTab + bias_bytes<kFlat>(buckets, group, span, pad(group)) : oCol) + kSlack;
@@ -583,7 +662,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(base + C::oMisc);
-  volatile uint8_t* big = base + C::oMisc + 28;  // [OS] a row's lse is big: scores rounded before it is taken off
+  volatile uint8_t* big = base + C::oMisc + 32;  // [OS] a row's lse is big: scores rounded before it is taken off
   int *col = reinterpret_cast<int*>(base + C::oCol), *col_val = col + NB;
   const mn_packed_args& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
@@ -623,6 +702,10 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
   auto kind_of = [&](int t0) {
     return k0 + 127 - (t0 + shift) <= -p.reach ? 1 : k0 - (t0 + p.ntok - 1 + shift) >= p.span - 1 - p.reach ? 2 : 3;
   };
+  // fp16: 2^kPowerP p, and with dp and delta times 2^(power - kPowerP) 2^power ds
+  int power = 0;
+  if (kPowers<ET>) power = n > 0 ? power_of(p.norms + ((int64_t)found.seq * a.kv_heads + hk) * 2) : 0;
+  const float lift = kPowers<ET> ? (float)kPowerP : 0.f, dp_by = kPowers<ET> ? pow2(power - kPowerP) : 1.f;
   bool ok = true;
 
   if (warp == 4 * W + 1) {
@@ -676,7 +759,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
           const int r = e * 32 + lane;
           l[e] = r < valid ? -a.lse[first + r] : -INFINITY;
           any_big |= is_big(l[e]);
-          x[NB + r] = r < valid ? -p.delta[first + r] : 0.f;
+          x[NB + r] = r < valid ? -p.delta[first + r] * dp_by : 0.f;
         }
         any_big = __any_sync(MN_FULL_MASK, any_big);
         if (lane == 0) big[st] = any_big;
@@ -684,6 +767,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
         for (int e = 0; e < NB / 32; ++e) {
           const int r = e * 32 + lane;
           if (BIAS && kind != 3 && !any_big && r < valid) l[e] += bs.val[col_val[r] + (kind == 1 ? lo : hi)];
+          if (kPowers<ET> && !any_big) l[e] += lift;
           x[r] = l[e];
         }
         __syncwarp();
@@ -808,6 +892,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
         for (int e = 0; e < CW; ++e) {
           const float b = BIAS ? bias_any(col[w * CW + e], col_val[w * CW + e]) : 0.f;
           x[e] = __fmaf_rn(x[e], sl2, b) + nl[e];
+          if (kPowers<ET>) x[e] += lift;
         }
       } else if (BIAS && kind_of(t0) == 3) {
 #pragma unroll
@@ -845,8 +930,10 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
 #pragma unroll
       for (int e = 0; e < CW / 4; ++e) {
         const float4 nd = reinterpret_cast<const float4*>(nl + NB)[e];
-        const float2 y0 = fmul2(make_float2(x[4 * e], x[4 * e + 1]), fadd2(make_float2(d[4 * e], d[4 * e + 1]), make_float2(nd.x, nd.y)));
-        const float2 y1 = fmul2(make_float2(x[4 * e + 2], x[4 * e + 3]), fadd2(make_float2(d[4 * e + 2], d[4 * e + 3]), make_float2(nd.z, nd.w)));
+        const float2 d0 = make_float2(d[4 * e], d[4 * e + 1]), d1 = make_float2(d[4 * e + 2], d[4 * e + 3]);
+        const float2 n0 = make_float2(nd.x, nd.y), n1 = make_float2(nd.z, nd.w), by = make_float2(dp_by, dp_by);
+        const float2 y0 = fmul2(make_float2(x[4 * e], x[4 * e + 1]), kPowers<ET> ? ffma2(d0, by, n0) : fadd2(d0, n0));
+        const float2 y1 = fmul2(make_float2(x[4 * e + 2], x[4 * e + 3]), kPowers<ET> ? ffma2(d1, by, n1) : fadd2(d1, n1));
         d[4 * e] = y0.x; d[4 * e + 1] = y0.y; d[4 * e + 2] = y1.x; d[4 * e + 3] = y1.y;
       }
       // p over the first half of this thread's columns, ds over the second
@@ -876,7 +963,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
         }
         if (mine)
           store32<ET>(static_cast<ET*>(is_v ? a.dv : a.dk) + ((int64_t)(s.k0 + key) * a.kv_heads + hk) * a.head_dim, c0, a.head_dim,
-                      o, is_v ? 1.f : a.scale);
+                      o, is_v ? pow2(kPowers<ET> ? -kPowerP : 0) : kPowers<ET> ? a.scale * pow2(-power) : a.scale);
         __syncwarp();
       }
     }
@@ -893,7 +980,7 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
 struct BwdSizes {
   int ntok, ntok_k;  // tokens to a tile of the query side, to a block of the key side
   int64_t q_slots, k_slots;
-  size_t delta_bytes, bytes;
+  size_t delta_bytes, norm_bytes, bytes;
 };
 // Up to 64 channels: blocks of 64 columns and two CTAs to an SM, so that one's
 // start and end run under the other's products; not where a token's heads
@@ -907,7 +994,8 @@ static BwdSizes sizes_of(const mn_packed_args* a) {
   z.q_slots = tile_slots(a->tq, a->nseq, z.ntok);
   z.k_slots = tile_slots(a->tk, a->nseq, 128);
   z.delta_bytes = ((size_t)a->tq * a->heads * 4 + 255) / 256 * 256;
-  z.bytes = z.delta_bytes + (a->bias_table ? (size_t)z.q_slots * a->heads * a->buckets * 4 : 0);
+  z.norm_bytes = a->dtype == MN_F16 ? ((size_t)a->nseq * a->kv_heads * 8 + 255) / 256 * 256 : 0;
+  z.bytes = z.delta_bytes + z.norm_bytes + (a->bias_table ? (size_t)z.q_slots * a->heads * a->buckets * 4 : 0);
   return z;
 }
 
@@ -926,7 +1014,8 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
     p.span = (bo.two_sided ? 2 : 1) * last + 1;
   }
   p.delta = static_cast<float*>(ws);
-  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + z.delta_bytes);
+  p.norms = reinterpret_cast<unsigned*>(static_cast<char*>(ws) + z.delta_bytes);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + z.delta_bytes + z.norm_bytes);
   p.err = err;
   CUtensorMap mq, mdo, mk, mv, nq, ndo, nk, nv;  // m: the query-side kernel's, n: the key-side kernel's
   const void *k = a->tk ? a->k : a->q, *v = a->tk ? a->v : a->q;
@@ -945,6 +1034,12 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
   auto kkv = dkv_kernel<ET, DT, NB, BIAS>;
   const size_t sq = Dq<DT, NB, BIAS>::bytes(a->buckets, p.group, p.span), skv = Dkv<DT, NB, BIAS>::bytes(a->buckets, p.group, p.span);
   if (!ensure_smem(kq, sq) || !ensure_smem(kkv, skv)) return false;
+  if constexpr (kPowers<ET>) {
+    const int64_t qs = tile_slots(a->tq, a->nseq, norm_tokens(p.group)), ks = tile_slots(a->tk, a->nseq, kNormKeys);
+    if ((qs + ks) * a->kv_heads > 0x7fffffff) return false;
+    if (cudaMemsetAsync(p.norms, 0, z.norm_bytes, st) != cudaSuccess) return false;
+    norms_kernel<<<(unsigned)((qs + ks) * a->kv_heads), 256, 0, st>>>(p, (int)qs);
+  }
   kq<<<(unsigned)(z.q_slots * a->kv_heads), Dq<DT, NB, BIAS>::kThreads, sq, st>>>(mq, mdo, mk, mv, p, bo);
   BwdParams pk = p;
   pk.ntok = z.ntok_k;

@@ -120,6 +120,7 @@ inline int64_t tile_slots(int rows, int n, int m) { return (int64_t)rows / m + n
 struct Found {
   Seq s;
   int local;  // the slot's place among the sequence's own
+  int seq;    // its number (nseq: the rows behind the last one)
 };
 template <bool KEYS>
 __device__ __forceinline__ Found seq_of_slot(const mn_packed_args& a, int m, int slot) {
@@ -152,6 +153,7 @@ __device__ __forceinline__ Found seq_of_slot(const mn_packed_args& a, int m, int
   f.s.slot = __shfl_sync(MN_FULL_MASK, f.s.slot, src);
   f.s.nk = __shfl_sync(MN_FULL_MASK, f.s.nk, src);
   f.local = slot - __shfl_sync(MN_FULL_MASK, first, src);
+  f.seq = __shfl_sync(MN_FULL_MASK, b, src);
   return f;
 }
 // The same with the tiles in descending order of their work, so that the last
@@ -199,6 +201,7 @@ __device__ __forceinline__ Found ranked_slot(const mn_packed_args& a, int m, int
   Found f;
   f.s.q0 = f.s.nq = f.s.k0 = f.s.nk = f.s.slot = 0;
   f.local = -1;
+  f.seq = n;
   if (slot >= total(0)) return f;
   int most = 0;
 #pragma unroll
@@ -231,7 +234,7 @@ __device__ __forceinline__ Found ranked_slot(const mn_packed_args& a, int m, int
     }
     at -= c;
   }
-  b = __shfl_sync(MN_FULL_MASK, b, src);
+  f.seq = b = __shfl_sync(MN_FULL_MASK, b, src);
   f.local = __shfl_sync(MN_FULL_MASK, f.local, src);
   const int end = min(b + 1, n);
   f.s.q0 = min(max(a.cu_q[b], 0), a.tq);
@@ -245,11 +248,13 @@ __device__ __forceinline__ Found ranked_slot(const mn_packed_args& a, int m, int
 __device__ __forceinline__ void put_found(volatile uint32_t* at, const Found& f) {
   if ((threadIdx.x & 31) == 0) {
     at[0] = f.s.q0; at[1] = f.s.nq; at[2] = f.s.k0; at[3] = f.s.nk; at[4] = f.s.slot; at[5] = f.local;
+    at[6] = f.seq;
   }
 }
 __device__ __forceinline__ Found get_found(const volatile uint32_t* at) {
   Found f;
   f.s.q0 = at[0]; f.s.nq = at[1]; f.s.k0 = at[2]; f.s.nk = at[3]; f.s.slot = at[4]; f.local = at[5];
+  f.seq = at[6];
   return f;
 }
 

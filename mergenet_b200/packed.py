@@ -278,7 +278,9 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
     rounded once to its type.
 
     Scores, softmax statistics and sums are fp32; probabilities and their
-    gradients are rounded to the input type before each tensor-core product.
+    gradients are rounded to the input type before each tensor-core product
+    (in fp16 times a power of two that keeps them in its range, one for each
+    sequence and key head).
     All sums have a fixed order, so equal calls give equal bits.  What lies in
     rows of no sequence, in unused cache rows and in other sequences never
     reaches a result, infinities and NaN included; within a sequence a NaN

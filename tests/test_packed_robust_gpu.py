@@ -61,3 +61,108 @@ def test_a_call_with_bad_offsets_leaves_later_calls_alone(dev, bad):
             for name in b:
                 assert torch.equal(a[name], b[name]), name
     assert mn.attention.attention_status(dev, reset=True) == L.MN_STATUS_BAD_LENGTHS
+
+
+# ------------------------------------------- gradients in the range of fp16
+def _scaled(p, **factors):
+    for name, f in factors.items():
+        p[name] = (p[name].float() * f).to(p[name].dtype)
+    return p
+
+
+@pytest.mark.parametrize("spec", [None, SPEC])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (4, 2, 128), (8, 1, 64)])
+def test_score_gradients_past_the_range_of_fp16(dev, heads, kv_heads, dim, spec):
+    """Upstream gradients of a large loss scale: dq, dk and dv fit fp16, while
+    p (dp - delta) reaches 2 x 10^5 and more."""
+    p = problem(dev, [300, 1, 150], heads=heads, kv_heads=kv_heads, dim=dim, dtype=torch.float16, spec=spec, table_dtype=torch.float32)
+    _scaled(p, q=1 / 16, k=1 / 16, v=16, dout=4096)
+    check(call(p, True, True), p, True)
+
+
+def _relative(x, want):
+    return float((x.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 2, 128), (2, 1, 32)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("name,factors", [("grad_q", dict(k=64, q=1 / 64)), ("grad_k", dict(q=64, k=1 / 64))])
+def test_small_upstream_gradients_in_fp16(dev, name, factors, causal, heads, kv_heads, dim):
+    """Upstream gradients of 2^-12 over 1,500 keys: p (dp - delta) is about
+    2^-20, where fp16 has steps of 2^-24; the gradients that it gives (about
+    2^-12, the keys or queries being large) are good to fp16's own step.
+
+    A term is rounded once (2^-11 at most, 2^-11 / sqrt(3) in the mean square)
+    and so is the result; both together come to 2^-11 of the norm.  The bound
+    is four times that.  Terms rounded in steps of 2^-24 would be off by
+    2^-26 or more each, 2^-6 of the norm."""
+    p = _scaled(problem(dev, [1500], heads=heads, kv_heads=kv_heads, dim=dim, dtype=torch.float16), dout=2.0 ** -12, **factors)
+    got = call(p, causal, True)
+    val, _ = O.packed_attention(p["q"], p["k"], p["v"], p["nq"], p["nk"], causal=causal, dout=p["dout"])
+    assert _relative(got[name], val[name]) < 2.0 ** -9
+    assert _relative(got["grad_v"], val["grad_v"]) < 2.0 ** -9 + 2.0 ** -25 * val["grad_v"].numel() ** 0.5 / float(val["grad_v"].norm())
+
+
+def test_values_of_little_weight_in_fp16(dev):
+    """A key whose weight is 2^-21 for every query, under upstream gradients of
+    2^10: its dv is within the normal range of fp16.  Each of the weights is
+    rounded by 2^-11 relative, is off by 2 E through the scores (66 products:
+    72 x 2^-24 x 2 x 7.5 x 2) and 2^-16 through the exponential, and the result
+    is rounded once more."""
+    n = 64
+    p = problem(dev, [n], [2], heads=2, kv_heads=2, dtype=torch.float16)
+    p["q"] = (1 + 0.02 * p["q"].float()).half()
+    p["k"] = torch.full_like(p["k"], 0.9375)
+    p["k"][1] *= -1
+    _scaled(p, dout=1024)
+    got = call(p, False, True)["grad_v"]
+    val, _ = O.packed_attention(p["q"], p["k"], p["v"], [n], [2], dout=p["dout"])
+    weight = torch.softmax(torch.einsum("ihd,jhd->hij", p["q"].double(), p["k"].double()) / 8, -1)
+    assert float(weight[..., 1].max()) < 2.0 ** -18 and float(weight[..., 1].min()) > 2.0 ** -25
+    mag = torch.einsum("hij,ihd->jhd", weight, p["dout"].double().abs())
+    assert ((got.double() - val["grad_v"]).abs() <= (2.0 ** -11 + 72 * 2.0 ** -24 * 30 + 2.0 ** -16) * mag
+            + 2.0 ** -11 * val["grad_v"].abs() + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_the_range_of_other_rows_reaches_nothing(dev, dim):
+    """Large finite values in another sequence, in unused cache rows and behind
+    the last sequence change no bit of a sequence's gradients."""
+    nq, nk, slots = [70, 50, 131], [70, 60, 131], [100, 128, 256]
+    p = problem(dev, nq, nk, slots, dim=dim, dtype=torch.float16, spec=SPEC, extra=40)
+    lens = torch.tensor(nk, dtype=torch.int32, device=dev)
+    clean = call(p, False, True, lengths=lens)
+    for n in ("q", "dout"):
+        p[n][70:120] *= 2.0 ** 12
+        p[n][251:] = 60000.0
+    p["k"][100:228] = 1.5
+    for n in ("k", "v"):
+        p[n][70:100] = 60000.0
+        p[n][100:228] = p[n][100:228].abs() + 512
+        p[n][228 + 131:] = -60000.0
+    got = call(p, False, True, lengths=lens)
+    rows = torch.cat([torch.arange(70), torch.arange(120, 251)]).to(dev)
+    keys = torch.cat([torch.arange(70), torch.arange(228, 359)]).to(dev)
+    for n in ("out", "grad_q"):
+        assert torch.equal(got[n][rows], clean[n][rows]), n
+    for n in ("grad_k", "grad_v"):
+        assert torch.equal(got[n][keys], clean[n][keys]), n
+
+
+def test_gradients_of_zero_and_of_one_value_in_fp16(dev):
+    """Ranges without a value to go by: no upstream gradient, no values, the
+    smallest and the largest ones that fp16 has."""
+    p = problem(dev, [140, 30], heads=4, kv_heads=2, dtype=torch.float16)
+    for n in ("dout", "v"):
+        got = call(dict(p, **{n: torch.zeros_like(p[n])}), True, True)
+        assert not got["grad_q"].any() and not got["grad_k"].any()
+        assert (n == "v") == bool(got["grad_v"].any())
+    for dout, v in ((2.0 ** -24, 2.0 ** -24), (65504.0, 2.0 ** -24), (2.0 ** -24, 65504.0)):
+        one = dict(p, dout=torch.sign(p["dout"]) * dout, v=torch.sign(p["v"]) * v)
+        got = call(one, False, True)
+        val, tol = O.packed_attention(one["q"], one["k"], one["v"], one["nq"], one["nk"], dout=one["dout"])
+        for n, x in got.items():  # a key that many queries weigh highest may have a dv past fp16's range
+            fits = val[n].abs() + tol[n] < 65504
+            assert ((x.double() - val[n]).abs() <= tol[n])[fits].all(), n
+            assert (torch.isinf(x) | ((x.double() - val[n]).abs() <= tol[n]))[~fits].all(), n
+            assert float(fits.double().mean()) > 0.99
