@@ -6,7 +6,8 @@ of the relative position by distance buckets.
 prompts, or one new token each against a cache) instead of the equal lengths
 of ``cross_attention`` and ``local_attention_packed``.  Heads may be grouped,
 the mask may be causal, and a learned table adds a bias that depends on the
-distance of query and key.  It is differentiable in q, k, v and the table.
+distance of query and key.  It is differentiable once, in reverse mode, in q,
+k, v and the table; forward-mode tangents are refused.
 
 ``relative_position_bias`` writes the same bias out as a tensor, for an
 attention that takes it as a mask.
@@ -19,6 +20,7 @@ import math
 import operator
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -237,6 +239,12 @@ def _attention_grads(ctx, dout):
 _attention_grads_once = once_differentiable(_attention_grads)  # where a graph of the gradients is asked for
 
 
+def _has_tangent(*tensors):
+    """A forward-mode tangent on one of them: the autograd functions have no
+    such derivative and refuse the call, where a plain call would drop it."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _check_offsets(name, t, entries):
     if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D int32 tensor, got {t.dtype} of shape {tuple(t.shape)}")
@@ -331,8 +339,8 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
         raise ValueError("at most 2^30 rows x grouped heads")
     _require(q.device, q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, bias_table)
     causal = bool(causal)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or (bias_table is not None and bias_table.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                     or (bias_table is not None and bias_table.requires_grad))) or _has_tangent(q, k, v, bias_table):
         return _PackedAttention.apply(q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, lengths_k, causal, scale, buckets)
     return _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, causal, scale, bias_table, buckets, False)[0]
 
@@ -410,6 +418,6 @@ def relative_position_bias(table, queries, keys, buckets, query_start=None):
     if table.shape[1] > 65535 or queries > 32 * 65535:
         raise ValueError("at most 65535 heads and 2097120 queries")
     L.require_cuda(table)
-    if torch.is_grad_enabled() and table.requires_grad:
+    if (torch.is_grad_enabled() and table.requires_grad) or _has_tangent(table):
         return _RelativeBias.apply(table, queries, keys, start, buckets)
     return _bias_forward(table, queries, keys, start, buckets)

@@ -166,3 +166,49 @@ def test_gradients_of_zero_and_of_one_value_in_fp16(dev):
             assert ((x.double() - val[n]).abs() <= tol[n])[fits].all(), n
             assert (torch.isinf(x) | ((x.double() - val[n]).abs() <= tol[n]))[~fits].all(), n
             assert float(fits.double().mean()) > 0.99
+
+
+# ------------------------------------------------------ forward-mode tangents
+@pytest.mark.parametrize("which", ["q", "k", "v", "table"])
+def test_forward_mode_tangents_are_refused(dev, which):
+    """Not dropped: the same error with and without a gradient asked for."""
+    import mergenet_b200 as mn
+    from torch.autograd import forward_ad
+    p = problem(dev, [20], spec=SPEC)
+    buckets, cu = mn.RelativeBuckets(*SPEC), offsets([20], dev)
+
+    def run(x):
+        out = mn.packed_attention(x["q"], x["k"], x["v"], cu, bias_table=x["table"], buckets=buckets)
+        return out, mn.relative_position_bias(x["table"], 4, 4, buckets)
+
+    want = run(p)
+    for grad in (False, True):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(p[which].detach().requires_grad_(grad), torch.ones_like(p[which]))
+            with pytest.raises(NotImplementedError, match="jvp"):
+                mn.packed_attention(*(dual if n == which else p[n] for n in ("q", "k", "v")), cu,
+                                    bias_table=dual if which == "table" else p["table"], buckets=buckets)
+            if which == "table":
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    mn.relative_position_bias(dual, 4, 4, buckets)
+    with forward_ad.dual_level():  # no tangent on these
+        for a, b in zip(run(p), want):
+            assert torch.equal(a, b) and not a.requires_grad
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = forward_ad.make_dual(p["q"], torch.ones_like(p["q"]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            mn.packed_attention(dual, p["k"], p["v"], cu)
+
+
+def test_function_transforms_are_refused(dev):
+    """torch.func's wrappers have no memory that a kernel could read."""
+    import mergenet_b200 as mn
+    p = problem(dev, [20])
+    cu = offsets([20], dev)
+    f = lambda q: mn.packed_attention(q, p["k"], p["v"], cu)  # noqa: E731
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(f, (p["q"],), (torch.ones_like(p["q"]),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(f)(p["q"][None])
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda q: f(q).float().sum())(p["q"])
