@@ -339,7 +339,8 @@ int mn_attention(int batch, int nq, int nk, int heads, int head_dim, int dtype,
  * at most 16 query heads to a key head, 48 buckets, and 8192 distances x
  * grouped heads (distances: up to the last border, on each side).  Anything
  * else returns MN_ERR_UNSUPPORTED.  out, dq, dk, dv: contiguous, of the same
- * type.  bias_table
+ * type, 16-byte aligned like the workspaces (an unaligned one returns
+ * MN_ERR_WORKSPACE).  bias_table
  * [buckets, heads] contiguous, of bias_dtype; dbias the same.
  * lse [kv_heads, tq, heads / kv_heads] fp32: log2 of each row's sum of
  * exponentials (+inf where no key is seen); NULL when no backward follows.

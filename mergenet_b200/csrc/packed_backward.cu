@@ -1079,7 +1079,7 @@ extern "C" int mn_packed_attention_backward(const mn_packed_args* a, void* works
   if (rc != MN_OK) return rc;
   if (a->tq == 0) return MN_ERR_ARG;  // no query: the gradients are 0, nothing to launch
   const pk::BwdSizes z = pk::sizes_of(a);
-  if (!workspace || workspace_bytes < z.bytes) return MN_ERR_WORKSPACE;
+  if (!workspace || !pk::aligned({workspace}) || workspace_bytes < z.bytes) return MN_ERR_WORKSPACE;
   cudaGetLastError();
   auto st = static_cast<cudaStream_t>(stream);
   bool done;

@@ -518,6 +518,7 @@ int check(const mn_packed_args* a, Borders* bo, bool backward) {
       !rows_ok(a->v, a->v_st, a->v_sh, a->tk, a->kv_heads) ||
       (backward && !rows_ok(a->dout, a->do_st, a->do_sh, a->tq, a->heads)))
     return MN_ERR_UNSUPPORTED;
+  if (!aligned({a->out}) || (backward && !aligned({a->dq, a->dk, a->dv}))) return MN_ERR_UNSUPPORTED;
   bo->n = 0;
   if (a->bias_table) {
     if (a->bias_dtype < 0 || a->bias_dtype > 2 || (backward && !a->dbias)) return MN_ERR_ARG;
@@ -624,7 +625,7 @@ extern "C" int mn_packed_attention(const mn_packed_args* a, void* workspace, siz
   if (rc != MN_OK) return rc;
   if (a->tq == 0) return MN_OK;
   const pk::Plan pl = pk::plan_of(a);
-  if (pl.parts && (!workspace || workspace_bytes < pk::part_bytes(a, pl))) return MN_ERR_WORKSPACE;
+  if (pl.parts && (!workspace || !pk::aligned({workspace}) || workspace_bytes < pk::part_bytes(a, pl))) return MN_ERR_WORKSPACE;
   cudaGetLastError();
   auto st = static_cast<cudaStream_t>(stream);
   bool done;

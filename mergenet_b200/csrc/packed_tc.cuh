@@ -2,6 +2,7 @@
 // tensor maps of packed rows, tile lookup, bias values, waits.
 #pragma once
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "packed.cuh"
@@ -317,6 +318,13 @@ inline bool map_k(CUtensorMap* map, bool bf16, const void* p, int64_t st, int64_
   const cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
   const cuuint32_t box[3] = {64, 1, (cuuint32_t)n};
   return tma::encode(map, bf16, 3, p, dims, strides, box, true, true);
+}
+// Tensors and workspaces are read and written 16 bytes at a time (NULL is
+// looked at where it matters).
+inline bool aligned(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  return true;
 }
 // what a tensor map needs of a [rows, heads, d] tensor
 inline bool rows_ok(const void* p, int64_t st, int64_t sh, int rows, int heads) {

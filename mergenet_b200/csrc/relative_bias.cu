@@ -159,7 +159,7 @@ extern "C" int mn_relative_bias_backward(int heads, int queries, int keys, int q
   if (queries == 0 || keys == 0) return MN_ERR_ARG;
   if (!dbias) return MN_ERR_ARG;
   if (heads > 65535 || rb::chunks_of(queries) > 65535) return MN_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < mn_relative_bias_backward_workspace_bytes(heads, queries, keys, buckets))
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < mn_relative_bias_backward_workspace_bytes(heads, queries, keys, buckets))
     return MN_ERR_WORKSPACE;
   cudaGetLastError();
   float* part = static_cast<float*>(workspace);

@@ -1,5 +1,6 @@
 """Uses of the packed attention and the relative position bias at the edge of
 what they accept, without a GPU."""
+import ctypes
 import types
 
 import pytest
@@ -26,3 +27,51 @@ def test_a_models_status_names_the_timeout(monkeypatch, more):
         _check_status(monkeypatch, L.MN_STATUS_TC_TIMEOUT | more)
     with pytest.raises(RuntimeError, match="unknown"):
         _check_status(monkeypatch, 1 << 20 | more)
+
+
+def _c_args(backward=False, **kw):
+    """Arguments of a call that divides its keys, on addresses that are never read."""
+    from mergenet_b200 import _lib as L
+    a = L.PackedArgs()
+    for i, n in enumerate(("q", "k", "v", "cu_q", "cu_k", "out", "lse") + (("dout", "dq", "dk", "dv") if backward else ())):
+        setattr(a, n, 1 << 20 | i << 12)
+    a.nseq, a.tq, a.tk, a.heads, a.kv_heads, a.head_dim, a.dtype, a.scale = 1, 1, 20000, 4, 2, 128, L.MN_F16, 1.0
+    a.q_st = a.do_st = 512
+    a.k_st = a.v_st = 256
+    a.q_sh = a.k_sh = a.v_sh = a.do_sh = 128
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "out"])
+def test_c_entry_refuses_unaligned_tensors(name):
+    """Rows are read and written 16 bytes at a time: nothing is launched on an
+    address that is not a multiple (the size of the workspace is 0 for calls
+    that are refused)."""
+    from mergenet_b200 import _lib as L
+    size = L.lib().mn_packed_attention_workspace_bytes
+    assert size(ctypes.byref(_c_args())) > 0
+    for off in (2, 4, 8):
+        a = _c_args(**{name: (1 << 20) + off})
+        assert size(ctypes.byref(a)) == 0
+        assert L.lib().mn_packed_attention(ctypes.byref(a), 1 << 21, 1 << 40, None, None) == L.MN_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "out", "dout", "dq", "dk", "dv"])
+def test_c_entry_refuses_unaligned_gradients(name):
+    from mergenet_b200 import _lib as L
+    size = L.lib().mn_packed_attention_backward_workspace_bytes
+    assert size(ctypes.byref(_c_args(True))) > 0
+    a = _c_args(True, **{name: (1 << 20) + 8})
+    assert size(ctypes.byref(a)) == 0
+    assert L.lib().mn_packed_attention_backward(ctypes.byref(a), 1 << 21, 1 << 40, None, None) == L.MN_ERR_UNSUPPORTED
+
+
+def test_c_entry_refuses_an_unaligned_workspace():
+    from mergenet_b200 import _lib as L
+    lib = L.lib()
+    assert lib.mn_packed_attention(ctypes.byref(_c_args()), (1 << 21) + 8, 1 << 40, None, None) == L.MN_ERR_WORKSPACE
+    assert lib.mn_packed_attention_backward(ctypes.byref(_c_args(True)), (1 << 21) + 8, 1 << 40, None, None) == L.MN_ERR_WORKSPACE
+    at = ctypes.addressof((ctypes.c_int32 * 1)(1))
+    assert lib.mn_relative_bias_backward(1, 4, 4, 0, 2, 0, 1, at, 0, 1 << 20, 1 << 20, (1 << 21) + 2, 1 << 40, None) == L.MN_ERR_WORKSPACE
