@@ -625,9 +625,6 @@ struct Dkv {
   // as S(i) has been read, so its Q has to be there a tile early: three stages,
   // but for the bias tables' room at 128 channels.
   static constexpr int QS = DT == 128 && BIAS ? 2 : 3, OS = 2;
-  // 128 channels then fill shared memory to the last KB: no room for aligning
-  // its start, which the kernel checks instead.
-  static constexpr uint32_t kSlack = DT == 128 && !BIAS ? 0 : 1024;
   static constexpr uint32_t oK = 0, oV = kTile, oRing = 2 * kTile, oDO = oRing + QS * kQ, oRows = oDO + OS * kQ;  // [OS][2][NB] floats
   static constexpr uint32_t oBars = oRows + OS * NB * 8;
   // barriers: K and V landed; Q, dout (and its rows) landed; tile i % 3 done; S ready, read; dP ready; p and ds ready
@@ -641,7 +638,7 @@ struct Dkv {
   static constexpr uint32_t oCol = oMisc + 48;
   static constexpr uint32_t oTab = oCol + NB * 8;
   static constexpr uint32_t bytes(int buckets, int group, int span) {
-    return (BIAS ? oTab + bias_bytes<kFlat>(buckets, group, span, pad(group)) : oCol) + kSlack;
+    return (BIAS ? oTab + bias_bytes<kFlat>(buckets, group, span, pad(group)) : oCol);
   }
   static constexpr uint32_t cS = 0, cDP = NB, cDV = cDP + NB, cDK = cDV + DT, kCols = NB == 64 ? 256 : 512;
   static_assert(cDK + DT <= kCols, "tensor memory");
@@ -654,12 +651,10 @@ __global__ void __launch_bounds__(Dkv<DT, NB, BIAS>::kThreads, Dkv<DT, NB, BIAS>
                const __grid_constant__ BwdParams p, const __grid_constant__ Borders bo) {
   using C = Dkv<DT, NB, BIAS>;
   constexpr int HV = C::HV, QS = C::QS, OS = C::OS, W = C::W, CW = C::CW;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  if (C::kSlack == 0 && (tc::smem_u32(smem_raw) & 1023)) {
-    if (threadIdx.x == 0 && p.err) atomicOr(p.err, MN_STATUS_TC_TIMEOUT);
-    return;
-  }
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // Swizzled tiles begin on 1,024 bytes.  The declaration asks for it: at 128
+  // channels the tiles fill shared memory to the last KB, without room to align
+  // the start by hand.
+  extern __shared__ __align__(1024) uint8_t base[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::oBars);
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(base + C::oMisc);
   volatile uint8_t* big = base + C::oMisc + 32;  // [OS] a row's lse is big: scores rounded before it is taken off
