@@ -337,7 +337,9 @@ int mn_attention(int batch, int nq, int nk, int heads, int head_dim, int dtype,
  * head_dim a multiple of 8 up to 128; at most 128 query heads to a key head;
  * pointers 16-byte aligned and strides positive multiples of 8.  With a bias
  * at most 16 query heads to a key head, 48 buckets, and 8192 distances x
- * grouped heads (distances: up to the last border, on each side).  Anything
+ * grouped heads (distances: up to the last border, on each side).  Fewer than
+ * 2^30 rows x grouped heads on either side, 2^31 query rows x heads, and 2^31
+ * (tiles of 128 rows + sequences) x key heads.  Anything
  * else returns MN_ERR_UNSUPPORTED.  out, dq, dk, dv: contiguous, of the same
  * type, 16-byte aligned like the workspaces (an unaligned one returns
  * MN_ERR_WORKSPACE).  bias_table

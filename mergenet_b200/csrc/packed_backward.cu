@@ -82,15 +82,15 @@ __device__ __forceinline__ float pow2(int n) { return __int_as_float((127 + n) <
 // and the training step with a bias 231 -> 246 us.
 __host__ __device__ constexpr int norm_tokens(int group) { return 256 / group; }
 constexpr int kNormKeys = 256;
-__global__ void __launch_bounds__(256) norms_kernel(const __grid_constant__ BwdParams p, int q_slots) {
+__global__ void __launch_bounds__(256) norms_kernel(const __grid_constant__ BwdParams p) {
   __shared__ uint32_t found_at[8];
   __shared__ float most[8];
   const mn_packed_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
   const int hk = blockIdx.x % a.kv_heads, slot = blockIdx.x / a.kv_heads;
-  const bool keys = slot >= q_slots;
+  const bool keys = blockIdx.y != 0;
   if (warp == 0)
-    put_found(found_at, keys ? seq_of_slot<true>(a, kNormKeys, slot - q_slots) : seq_of_slot<false>(a, norm_tokens(G), slot));
+    put_found(found_at, keys ? seq_of_slot<true>(a, kNormKeys, slot) : seq_of_slot<false>(a, norm_tokens(G), slot));
   __syncthreads();
   const Found f = get_found(found_at);
   if (f.seq >= a.nseq || f.local < 0) return;
@@ -1024,16 +1024,14 @@ static bool launch_bwd(const mn_packed_args* a, const Borders& bo, const BwdSize
       !map_k(&nk, bf16, k, a->k_st, a->k_sh, tk, a->kv_heads, a->head_dim, 128) ||
       !map_k(&nv, bf16, v, a->v_st, a->v_sh, tk, a->kv_heads, a->head_dim, 128))
     return false;
-  if (z.q_slots * a->kv_heads > 0x7fffffff || z.k_slots * a->kv_heads > 0x7fffffff) return false;
   auto kq = dq_kernel<ET, DT, NB, BIAS>;
   auto kkv = dkv_kernel<ET, DT, NB, BIAS>;
   const size_t sq = Dq<DT, NB, BIAS>::bytes(a->buckets, p.group, p.span), skv = Dkv<DT, NB, BIAS>::bytes(a->buckets, p.group, p.span);
   if (!ensure_smem(kq, sq) || !ensure_smem(kkv, skv)) return false;
   if constexpr (kPowers<ET>) {
     const int64_t qs = tile_slots(a->tq, a->nseq, norm_tokens(p.group)), ks = tile_slots(a->tk, a->nseq, kNormKeys);
-    if ((qs + ks) * a->kv_heads > 0x7fffffff) return false;
     if (cudaMemsetAsync(p.norms, 0, z.norm_bytes, st) != cudaSuccess) return false;
-    norms_kernel<<<(unsigned)((qs + ks) * a->kv_heads), 256, 0, st>>>(p, (int)qs);
+    norms_kernel<<<dim3((unsigned)(std::max(qs, ks) * a->kv_heads), 2), 256, 0, st>>>(p);
   }
   kq<<<(unsigned)(z.q_slots * a->kv_heads), Dq<DT, NB, BIAS>::kThreads, sq, st>>>(mq, mdo, mk, mv, p, bo);
   BwdParams pk = p;

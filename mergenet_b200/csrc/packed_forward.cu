@@ -514,6 +514,10 @@ int check(const mn_packed_args* a, Borders* bo, bool backward) {
   const int g = a->heads / a->kv_heads;
   if (a->head_dim > 128 || a->head_dim % 8 || g > 128 || a->kv_heads > 65535) return MN_ERR_UNSUPPORTED;
   if ((int64_t)a->tq * g >= (1 << 30) || (int64_t)a->tk * g >= (1 << 30)) return MN_ERR_UNSUPPORTED;
+  // grids of a block a row and head, and of the tiles of either side, at most
+  if ((int64_t)a->tq * a->heads > 0x7fffffff) return MN_ERR_UNSUPPORTED;
+  if (std::max(tile_slots(a->tq, a->nseq, 128 / g), tile_slots(a->tk, a->nseq, 128)) * a->kv_heads > 0x7fffffff)
+    return MN_ERR_UNSUPPORTED;
   if (!rows_ok(a->q, a->q_st, a->q_sh, a->tq, a->heads) || !rows_ok(a->k, a->k_st, a->k_sh, a->tk, a->kv_heads) ||
       !rows_ok(a->v, a->v_st, a->v_sh, a->tk, a->kv_heads) ||
       (backward && !rows_ok(a->dout, a->do_st, a->do_sh, a->tq, a->heads)))
@@ -586,12 +590,10 @@ static bool launch(const mn_packed_args* a, const Borders& bo, const Plan& pl, v
   p.part_o = static_cast<float*>(ws);
   p.part_lse = p.part_o + (size_t)pl.parts * a->tq * a->heads * a->head_dim;
   p.err = err;
-  if ((int64_t)a->tq * a->heads > 0x7fffffff) return false;
   const size_t smem = F::bytes(p.group, p.span);
   auto kern = forward_kernel<ET, DT, BIAS, SPLIT>;
   if (!ensure_smem(kern, smem) || !launch_regs(kern, F::kLaunchRegs)) return false;
   const int64_t slots = tile_slots(a->tq, a->nseq, SPLIT ? pl.ntok : F::NQ * pl.ntok) * a->kv_heads;
-  if (slots > 0x7fffffff) return false;
   kern<<<dim3((unsigned)slots, pl.splits), F::kThreads, smem, st>>>(mq, mk, mv, p, bo);
   if (SPLIT) {
     const int64_t rows = (int64_t)a->tq * a->heads;

@@ -265,6 +265,8 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
     any row and head strides) hold the rows of all sequences one behind the
     other; H is a multiple of Hkv and query head h reads key head
     h // (H / Hkv).  D is a multiple of 8 up to 128.  Returns [Tq, H, D].
+    There are fewer than 2^30 rows x grouped heads, 2^31 query rows x heads and
+    2^31 (sequences + tiles of 128 rows) x key heads.
 
     ``cu_seqlens_q`` (int32, on the device, [B + 1], from 0) are the row
     offsets of the sequences' queries, ``cu_seqlens_k`` those of their keys
@@ -337,6 +339,10 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
                              f"{MAX_BIAS_GROUP} grouped heads and {MAX_BIAS_VALUES} distances x grouped heads")
     if max(tq, tk) * group >= 1 << 30:
         raise ValueError("at most 2^30 rows x grouped heads")
+    if tq * h >= 1 << 31:
+        raise ValueError("at most 2^31 query rows x heads")
+    if (entries + max(tq // (128 // group), tk // 128)) * hk >= 1 << 31:
+        raise ValueError(f"{entries - 1} sequences with {hk} key heads: at most 2^31 tiles of 128 rows x heads, one more a sequence")
     _require(q.device, q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, bias_table)
     causal = bool(causal)
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad

@@ -75,3 +75,41 @@ def test_c_entry_refuses_an_unaligned_workspace():
     assert lib.mn_packed_attention_backward(ctypes.byref(_c_args(True)), (1 << 21) + 8, 1 << 40, None, None) == L.MN_ERR_WORKSPACE
     at = ctypes.addressof((ctypes.c_int32 * 1)(1))
     assert lib.mn_relative_bias_backward(1, 4, 4, 0, 2, 0, 1, at, 0, 1 << 20, 1 << 20, (1 << 21) + 2, 1 << 40, None) == L.MN_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("sizes,match", [
+    (dict(tq=1 << 20, tk=1 << 20, heads=4096, kv_heads=4096), "2\\^31 query rows"),
+    (dict(tq=1 << 29, tk=1 << 29, heads=4, kv_heads=4), "2\\^31 query rows"),
+    (dict(tq=1, tk=1, heads=65535, kv_heads=65535, nseq=1 << 15), "2\\^31 tiles"),
+    (dict(tq=1, tk=1 << 29, heads=1024, kv_heads=1024), "2\\^31 tiles"),
+    (dict(tq=1, tk=1 << 30, heads=1, kv_heads=1), "2\\^30 rows"),
+])
+def test_sizes_past_a_launch_are_refused_beforehand(sizes, match):
+    """By name in Python, and before anything is launched in C."""
+    import mergenet_b200 as mn
+    from mergenet_b200 import _lib as L
+    nseq = sizes.get("nseq", 1)
+    meta = [torch.empty(sizes[r], sizes[h], 8, dtype=torch.float16, device="meta")
+            for r, h in (("tq", "heads"), ("tk", "kv_heads"), ("tk", "kv_heads"))]
+    cu = torch.empty(nseq + 1, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match=match):
+        mn.packed_attention(*meta, cu, cu)
+    h, hk = sizes["heads"], sizes["kv_heads"]
+    a = _c_args(True, **sizes, head_dim=8, q_st=8 * h, do_st=8 * h, k_st=8 * hk, v_st=8 * hk, q_sh=8, k_sh=8, v_sh=8, do_sh=8)
+    assert L.lib().mn_packed_attention_backward_workspace_bytes(ctypes.byref(a)) == 0
+    assert L.lib().mn_packed_attention(ctypes.byref(a), 1 << 21, 1 << 40, None, None) == L.MN_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("sizes", [dict(tq=1 << 19, tk=1 << 19, heads=4095, kv_heads=4095), dict(tq=1, tk=1 << 28, heads=8, kv_heads=8),
+                                   dict(tq=1, tk=1, heads=65535, kv_heads=65535, nseq=32000)])
+def test_the_largest_sizes_are_not(sizes):
+    from mergenet_b200 import _lib as L
+    import mergenet_b200 as mn
+    h, hk = sizes["heads"], sizes["kv_heads"]
+    a = _c_args(True, **sizes, head_dim=8, q_st=8 * h, do_st=8 * h, k_st=8 * hk, v_st=8 * hk, q_sh=8, k_sh=8, v_sh=8, do_sh=8)
+    assert L.lib().mn_packed_attention_backward_workspace_bytes(ctypes.byref(a)) > 0
+    meta = [torch.empty(sizes[r], sizes[n], 8, dtype=torch.float16, device="meta")
+            for r, n in (("tq", "heads"), ("tk", "kv_heads"), ("tk", "kv_heads"))]
+    cu = torch.empty(sizes.get("nseq", 1) + 1, dtype=torch.int32, device="meta")
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):  # all that is wrong with it
+        mn.packed_attention(*meta, cu, cu)
