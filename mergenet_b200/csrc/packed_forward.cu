@@ -518,9 +518,9 @@ int check(const mn_packed_args* a, Borders* bo, bool backward) {
   if ((int64_t)a->tq * a->heads > 0x7fffffff) return MN_ERR_UNSUPPORTED;
   if (std::max(tile_slots(a->tq, a->nseq, 128 / g), tile_slots(a->tk, a->nseq, 128)) * a->kv_heads > 0x7fffffff)
     return MN_ERR_UNSUPPORTED;
-  if (!rows_ok(a->q, a->q_st, a->q_sh, a->tq, a->heads) || !rows_ok(a->k, a->k_st, a->k_sh, a->tk, a->kv_heads) ||
-      !rows_ok(a->v, a->v_st, a->v_sh, a->tk, a->kv_heads) ||
-      (backward && !rows_ok(a->dout, a->do_st, a->do_sh, a->tq, a->heads)))
+  if (!rows_ok(a->q, a->q_st, a->q_sh, a->tq, a->heads, g) || !rows_ok(a->k, a->k_st, a->k_sh, a->tk, a->kv_heads, 1) ||
+      !rows_ok(a->v, a->v_st, a->v_sh, a->tk, a->kv_heads, 1) ||
+      (backward && !rows_ok(a->dout, a->do_st, a->do_sh, a->tq, a->heads, g)))
     return MN_ERR_UNSUPPORTED;
   if (!aligned({a->out}) || (backward && !aligned({a->dq, a->dk, a->dv}))) return MN_ERR_UNSUPPORTED;
   bo->n = 0;

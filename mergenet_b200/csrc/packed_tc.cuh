@@ -326,10 +326,13 @@ inline bool aligned(std::initializer_list<const void*> ps) {
     if (reinterpret_cast<uintptr_t>(p) % 16) return false;
   return true;
 }
-// what a tensor map needs of a [rows, heads, d] tensor
-inline bool rows_ok(const void* p, int64_t st, int64_t sh, int rows, int heads) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || (st > 0 && st % 8 == 0)) &&
-         (heads <= 1 || (sh > 0 && sh % 8 == 0)) && st < (int64_t(1) << 38) && sh < (int64_t(1) << 31);
+// what a tensor map of groups of g heads needs of a [rows, heads, d] tensor:
+// strides of whole 16 bytes below 2^40 bytes (no tensor that fits the card has
+// larger ones, but for dimensions of one, whose stride is not looked at)
+inline bool rows_ok(const void* p, int64_t st, int64_t sh, int rows, int heads, int g) {
+  auto fits = [](int64_t stride, int64_t most) { return stride > 0 && stride % 8 == 0 && stride < most; };
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || fits(st, int64_t(1) << 39)) &&
+         (heads <= 1 || fits(sh, (int64_t(1) << 39) / g));
 }
 // The kernel was compiled to launch with at least `regs` registers a thread.
 template <typename F>

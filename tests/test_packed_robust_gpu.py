@@ -212,3 +212,37 @@ def test_function_transforms_are_refused(dev):
         torch.func.vmap(f)(p["q"][None])
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda q: f(q).float().sum())(p["q"])
+
+
+# ----------------------------------------------------------------- layouts
+def test_head_strides_past_32_bits(dev):
+    """Keys, values, queries and their gradient laid out head by head, the
+    heads more than 2^31 values apart; only their rows are ever written."""
+    import mergenet_b200 as mn
+    p = problem(dev, [70, 3], [300, 77], heads=2, kv_heads=2, dim=64)
+    want = call(p, True, True)
+    apart = (1 << 31) + 64
+    memory = torch.empty(apart + (1 << 18), device=dev, dtype=torch.bfloat16)
+    at, wide = 0, {}
+    for n in ("q", "k", "v", "dout"):
+        rows = p[n].shape[0]
+        wide[n] = memory.as_strided((rows, 2, 64), (64, apart, 1), at)
+        wide[n].copy_(p[n])
+        at += rows * 64
+    assert wide["k"].stride(1) > 1 << 31
+    leaves = [wide[n].detach().requires_grad_(True) for n in ("q", "k", "v")]
+    out = mn.packed_attention(*leaves, offsets(p["nq"], dev), offsets(p["nk"], dev), causal=True)
+    got = [out.detach(), *torch.autograd.grad(out, leaves, wide["dout"])]
+    for x, n in zip(got, want):
+        assert torch.equal(x, want[n]), n
+
+
+def test_any_stride_of_a_dimension_of_one(dev):
+    import mergenet_b200 as mn
+    p = problem(dev, [70], heads=1, kv_heads=1)
+    want = call(p, True, True)
+    leaves = [p[n].as_strided(p[n].shape, (64, 1 << 45, 1)).requires_grad_(True) for n in ("q", "k", "v")]
+    out = mn.packed_attention(*leaves, offsets([70], dev), causal=True)
+    got = [out.detach(), *torch.autograd.grad(out, leaves, p["dout"])]
+    for x, n in zip(got, want):
+        assert torch.equal(x, want[n]), n

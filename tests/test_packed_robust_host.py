@@ -113,3 +113,18 @@ def test_the_largest_sizes_are_not(sizes):
     cu = torch.empty(sizes.get("nseq", 1) + 1, dtype=torch.int32, device="meta")
     with pytest.raises(RuntimeError, match="CUDA tensors only"):  # all that is wrong with it
         mn.packed_attention(*meta, cu, cu)
+
+
+@pytest.mark.parametrize("kw", [dict(k_sh=1 << 32, v_sh=1 << 31), dict(q_sh=1 << 35, do_sh=(1 << 31) + 8), dict(q_st=1 << 38),
+                                dict(heads=1, kv_heads=1, q_sh=1 << 45, k_sh=1 << 45), dict(tq=1, q_st=1 << 45)])
+def test_c_entry_takes_any_stride_of_a_tensor(kw):
+    """Strides past 2^31 (a cache laid out head by head), and any stride of a
+    dimension of one."""
+    from mergenet_b200 import _lib as L
+    assert L.lib().mn_packed_attention_backward_workspace_bytes(ctypes.byref(_c_args(True, **dict(dict(tq=2), **kw)))) > 0
+
+
+@pytest.mark.parametrize("kw", [dict(k_sh=1 << 39), dict(q_sh=1 << 38), dict(k_sh=-128), dict(q_st=0), dict(v_sh=4), dict(k_st=1 << 39)])
+def test_c_entry_refuses_strides_that_no_tile_map_has(kw):
+    from mergenet_b200 import _lib as L
+    assert L.lib().mn_packed_attention_backward_workspace_bytes(ctypes.byref(_c_args(True, **dict(dict(tq=2), **kw)))) == 0
