@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 
 int check(const mn_packed_args* a, Borders* bo, bool backward) {
   if (!a || a->nseq < 1 || a->tq < 0 || a->tk < 0 || a->heads < 1 || a->kv_heads < 1) return MN_ERR_ARG;
-  if (a->heads % a->kv_heads || a->head_dim < 1 || !(a->scale > 0.f) || !(a->scale < INFINITY)) return MN_ERR_ARG;
+  if (a->heads % a->kv_heads || a->head_dim < 1 || !(a->scale > 0.f) || !(a->scale <= 0x1p127f)) return MN_ERR_ARG;
   if (!a->cu_q || !a->cu_k || (a->tq > 0 && (!a->q || !a->out)) || (a->tk > 0 && (!a->k || !a->v))) return MN_ERR_ARG;
   if (backward && a->tq > 0 && (!a->dout || !a->lse || !a->dq)) return MN_ERR_ARG;
   if (backward && a->tk > 0 && (!a->dk || !a->dv)) return MN_ERR_ARG;

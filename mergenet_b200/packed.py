@@ -16,7 +16,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 import operator
 
 import torch
@@ -326,8 +325,8 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
     if lengths_k is not None:
         _check_offsets("lengths_k", lengths_k, entries - 1)
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 2.0 ** -149 <= scale <= 2.0 ** 127:  # in fp32, times log2 e
+        raise ValueError(f"scale must be positive and in the range of fp32, got {scale}")
     if (bias_table is None) != (buckets is None):
         raise ValueError("bias_table and buckets go together")
     if bias_table is not None:

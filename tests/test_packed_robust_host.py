@@ -128,3 +128,11 @@ def test_c_entry_takes_any_stride_of_a_tensor(kw):
 def test_c_entry_refuses_strides_that_no_tile_map_has(kw):
     from mergenet_b200 import _lib as L
     assert L.lib().mn_packed_attention_backward_workspace_bytes(ctypes.byref(_c_args(True, **dict(dict(tq=2), **kw)))) == 0
+
+
+@pytest.mark.parametrize("scale", [1e39, 3.5e38, 1e-46, 5e-324, -1.0, float("inf")])
+def test_scales_that_fp32_does_not_have_are_refused(scale):
+    import mergenet_b200 as mn
+    x = torch.zeros(6, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="scale must be positive"):
+        mn.packed_attention(x, x, x, torch.tensor([0, 6], dtype=torch.int32), scale=scale)
