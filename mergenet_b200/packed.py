@@ -87,6 +87,9 @@ class RelativeBuckets:
         self.num_buckets, self.max_distance, self.two_sided = int(num_buckets), int(max_distance), bool(two_sided)
         self.borders, self._c_borders = _borders(self.num_buckets, self.max_distance, self.two_sided)
 
+    def __reduce__(self):  # with a module that is saved or sent to another process
+        return RelativeBuckets, (self.num_buckets, self.max_distance, self.two_sided)
+
     def __repr__(self):
         return f"RelativeBuckets({self.num_buckets}, {self.max_distance}, two_sided={self.two_sided})"
 

@@ -136,3 +136,20 @@ def test_scales_that_fp32_does_not_have_are_refused(scale):
     x = torch.zeros(6, 2, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="scale must be positive"):
         mn.packed_attention(x, x, x, torch.tensor([0, 6], dtype=torch.int32), scale=scale)
+
+
+@pytest.mark.parametrize("spec", [(32, 128, True), (48, 700, False)])
+def test_buckets_are_saved_and_copied(spec):
+    """With a module that holds them, or to another process."""
+    import copy
+    import io
+    import pickle
+    import mergenet_b200 as mn
+    b = mn.RelativeBuckets(*spec)
+    module = torch.nn.Module()
+    module.buckets = b
+    file = io.BytesIO()
+    torch.save(module, file)
+    file.seek(0)
+    for c in (pickle.loads(pickle.dumps(b)), copy.deepcopy(b), copy.copy(b), torch.load(file, weights_only=False).buckets):
+        assert repr(c) == repr(b) and c.borders == b.borders and list(c._c_borders) == list(b.borders)
