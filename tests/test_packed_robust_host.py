@@ -153,3 +153,48 @@ def test_buckets_are_saved_and_copied(spec):
     file.seek(0)
     for c in (pickle.loads(pickle.dumps(b)), copy.deepcopy(b), copy.copy(b), torch.load(file, weights_only=False).buckets):
         assert repr(c) == repr(b) and c.borders == b.borders and list(c._c_borders) == list(b.borders)
+
+
+# ------------------------------------------------- what the GPU tests' bounds catch
+BOUND_SHAPES = [([200, 520], 16, 1, 128, (32, 128, True)), ([200, 520], 6, 6, 64, (32, 128, True)), ([300, 1, 129], 4, 2, 64, (32, 128, False))]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nq,heads,kv_heads,dim,spec", BOUND_SHAPES)
+def test_bounds_reject_results_that_are_off(nq, heads, kv_heads, dim, spec, dtype, causal):
+    """The bounds that add roundings by their squares: a result of another
+    factor, a head or a sum by bucket left out, a table that lost its outermost
+    buckets and a key too few are rejected."""
+    from oracle import packed as O
+    gen = torch.Generator().manual_seed(0)
+    t = {n: torch.randn(sum(nq), h, dim, generator=gen).to(dtype) for n, h in
+         (("q", heads), ("k", kv_heads), ("v", kv_heads), ("dout", heads))}
+    table = torch.randn(spec[0], heads, generator=gen)
+
+    def run(f, nk=nq, dout=t["dout"], table=table):
+        return f(t["q"], t["k"], t["v"], nq, nk, nq, causal=causal, table=table, spec=None if table is None else spec, dout=dout)
+
+    val, tol = run(O.packed_attention_spread)
+    first, _ = run(O.packed_attention)
+    for n in val:
+        assert torch.allclose(val[n], first[n], rtol=1e-12, atol=1e-12), n
+    passes = lambda n, x: bool(((x - val[n]).abs() <= tol[n]).all())  # noqa: E731
+    for n in val:
+        assert passes(n, val[n])
+        assert not passes(n, 0.95 * val[n]) and not passes(n, 1.05 * val[n]), n
+    far = [spec[0] // 2 - 1] + ([] if causal else [spec[0] - 1]) if spec[2] else [spec[0] - 1]
+    for bucket in far:
+        x = val["grad_table"].clone()
+        x[bucket] = 0
+        assert not passes("grad_table", x), bucket
+    less = t["dout"].clone()
+    less[:, heads - 1] = 0  # the last head's share of the gradients
+    part, _ = run(O.packed_attention, dout=less)
+    for n in ("grad_q", "grad_k", "grad_v", "grad_table"):
+        assert not passes(n, part[n]), n
+    plain, plain_tol = run(O.packed_attention_spread, table=None)
+    fewer, _ = run(O.packed_attention, nk=[max(0, x - 1) for x in nq], table=None)
+    if not causal:  # under the causal mask the positions move along
+        for n in plain:
+            assert bool(((fewer[n] - plain[n]).abs() > plain_tol[n]).any()), n
