@@ -58,17 +58,19 @@ struct BwdParams {
 // passes 65,504 under the upstream gradients of a large loss scale and has
 // steps of 2^-24 under small ones, and a weight below 2^-14 loses bits (one of
 // 16,384 equal keys).  So dv takes 2^14 p, and dq and dk take 2^s ds, with one
-// s for all rows of a sequence and key head, from |ds| <= |dp - delta| <=
-// 2 max|dout| max|v| (delta = dout . out, out a mean of the v); the powers are
-// taken off the fp32 sums.  bf16 has the range of fp32.
+// s for all rows of a sequence and key head; the powers are taken off the fp32
+// sums.  delta is the mean of a row's dp by its p, so |ds| <= p (1 - p) times the
+// span of the dp, half of max|dout| max|v|; that product goes to 2^15, which
+// leaves a factor of four for the statistics of very large scores.  A ds below
+// 2^-39 of it loses bits.  bf16 has the range of fp32.
 constexpr int kPowerP = 14;
 template <typename ET>
 constexpr bool kPowers = std::is_same<ET, __half>::value;
-__device__ __forceinline__ int power_of(const unsigned* norms) {  // s: 2 max|dout| max|v| 2^s <= 2^15, by the bounds of both
+__device__ __forceinline__ int power_of(const unsigned* norms) {  // s: max|dout| max|v| 2^s <= 2^15, by the bounds of both
   const unsigned x = norms[0], y = norms[1];
   if (x == 0 || y == 0) return 0;
   const int e = (int)(x >> 23) + (int)(y >> 23) - 252;  // (max|dout| max|v|)^2 < 2^e
-  return min(max(14 - ((e + 1) >> 1), -40), 40);
+  return min(max(15 - ((e + 1) >> 1), -40), 40);
 }
 __device__ __forceinline__ float pow2(int n) { return __int_as_float((127 + n) << 23); }
 

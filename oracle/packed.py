@@ -164,7 +164,14 @@ def packed_attention_spread(q, k, v, nq, nk, slots=None, causal=False, scale=Non
     both as well: 2^-18 for all of it.  A row's sum of b terms rounds b times
     independently: 6 sqrt(b / 3) f.  The tensor cores add 16 terms a step, which
     may cut instead of round (2 f of the sum so far), and keep at least as many
-    bits within the step: n terms are off by (n / 8 + 32) f."""
+    bits within the step: n terms are off by (n / 8 + 32) f.
+
+    Below a floor a term loses all of its bits.  In fp16 a p of the gradients is
+    held as 2^14 p (half a step 2^-25 - 14), and ds as 2^s ds with s from bounds
+    of A = max|dout| and B = max|v| of the sequence and key head: 2^s >= 2^15 /
+    (2^5.5 A B), the bounds being within sqrt(16) of A and of B and the power
+    within 2^1.5, so half a step is 2^(-25 - 15 + 5.5) A B.  An exponential below
+    2^-126 is 0."""
     dt = q.dtype
     u, tiny = HALF_STEP[dt], TINY[dt]
     h, hk, d = q.shape[1], k.shape[1], q.shape[2]
@@ -183,6 +190,8 @@ def packed_attention_spread(q, k, v, nq, nk, slots=None, causal=False, scale=Non
     var = {n: torch.zeros_like(t) for n, t in shapes.items()}    # mean squares of the roundings
     slack = {n: torch.zeros_like(t) for n, t in shapes.items()}  # fp32's errors
     r2 = u * u / 3
+    half = dt == torch.float16
+    floor_p = 2.0 ** -39 if half else 2.0 ** -126
     q0 = k0 = 0
     for a, b, slot in zip(nq, nk, slots):
         if a and b:
@@ -192,6 +201,7 @@ def packed_attention_spread(q, k, v, nq, nk, slots=None, causal=False, scale=Non
             if causal:
                 seen = seen.tril(b - a)
             any_seen = seen.any(-1, keepdim=True)
+            ones = seen.double()
             for j in range(h):
                 Q, K, V = qd[rq, j], kd[rk, j // g], vd[rk, j // g]
                 x = scale * (Q @ K.t())
@@ -217,14 +227,17 @@ def packed_attention_spread(q, k, v, nq, nk, slots=None, causal=False, scale=Non
                     tiny * tiny * DO.square().sum(-1, keepdim=True)
                 raw = ds.abs() * (ep + 4 * F32) + p * (1 + ep) * ((d + 2) * F32 * (DO.abs() @ V.abs().t())
                                                                    + ((2 * ep + (d + 2) * F32) * (DO.abs() * (p @ V.abs())).sum(-1, keepdim=True)))
+                heads = slice(j // g * g, j // g * g + g)
+                most = gd[rq, heads].norm(dim=-1).amax() * V.norm(dim=-1).amax()
+                floor2 = (2.0 ** -34.5 * most) ** 2 if half else (2.0 ** -126 * 2 * most) ** 2
                 val["grad_q"][rq, j] = scale * (ds @ K)
-                var["grad_q"][rq, j] = scale ** 2 * (r2 * (ds.square() @ K.square()) + var_delta * (p @ K).square())
+                var["grad_q"][rq, j] = scale ** 2 * ((r2 * ds.square() + floor2 * ones) @ K.square() + var_delta * (p @ K).square())
                 slack["grad_q"][rq, j] = scale * ((raw + sum_b * ds.abs()) @ K.abs())
                 val["grad_k"][rk, j // g] += scale * (ds.t() @ Q)
-                var["grad_k"][rk, j // g] += scale ** 2 * (r2 * (ds.t().square() @ Q.square()) + (var_delta * p.square()).t() @ Q.square())
+                var["grad_k"][rk, j // g] += scale ** 2 * ((r2 * ds.square() + floor2 * ones + var_delta * p.square()).t() @ Q.square())
                 slack["grad_k"][rk, j // g] += scale * ((raw + sum_n * ds.abs()).t() @ Q.abs())
                 val["grad_v"][rk, j // g] += p.t() @ DO
-                var["grad_v"][rk, j // g] += r2 * (p.t().square() @ DO.square())
+                var["grad_v"][rk, j // g] += (r2 * p.square() + floor_p ** 2 * ones).t() @ DO.square()
                 slack["grad_v"][rk, j // g] += (p * (ep + sum_n)).t() @ DO.abs()
                 if td is not None:
                     hot = at.reshape(-1)
