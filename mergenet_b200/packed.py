@@ -241,10 +241,20 @@ def _attention_grads(ctx, dout):
 _attention_grads_once = once_differentiable(_attention_grads)  # where a graph of the gradients is asked for
 
 
+def _check_sizes(entries, tq, tk, h, hk):
+    group = h // hk
+    if max(tq, tk) * group >= 1 << 30:
+        raise ValueError("at most 2^30 rows x grouped heads")
+    if tq * h >= 1 << 31:
+        raise ValueError("at most 2^31 query rows x heads")
+    if (entries + max(tq // (128 // group), tk // 128)) * hk >= 1 << 31:
+        raise ValueError(f"{entries - 1} sequences with {hk} key heads: at most 2^31 tiles of 128 rows x heads, one more a sequence")
+
+
 def _has_tangent(*tensors):
     """A forward-mode tangent on one of them: the autograd functions have no
     such derivative and refuse the call, where a plain call would drop it."""
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _check_offsets(name, t, entries):
@@ -339,16 +349,13 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, lengths_k=None
                 or (sides * buckets.borders[-1] + 1) * group > MAX_BIAS_VALUES):
             raise ValueError(f"{buckets} with {group} grouped heads does not fit: at most {MAX_BUCKETS} buckets, "
                              f"{MAX_BIAS_GROUP} grouped heads and {MAX_BIAS_VALUES} distances x grouped heads")
-    if max(tq, tk) * group >= 1 << 30:
-        raise ValueError("at most 2^30 rows x grouped heads")
-    if tq * h >= 1 << 31:
-        raise ValueError("at most 2^31 query rows x heads")
-    if (entries + max(tq // (128 // group), tk // 128)) * hk >= 1 << 31:
-        raise ValueError(f"{entries - 1} sequences with {hk} key heads: at most 2^31 tiles of 128 rows x heads, one more a sequence")
+    if (entries + tq + tk) * h >= 1 << 30:  # smaller ones fit in any case
+        _check_sizes(entries, tq, tk, h, hk)
     _require(q.device, q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, bias_table)
     causal = bool(causal)
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                     or (bias_table is not None and bias_table.requires_grad))) or _has_tangent(q, k, v, bias_table):
+                                     or (bias_table is not None and bias_table.requires_grad))) or (
+                                         forward_ad._current_level >= 0 and _has_tangent(q, k, v, bias_table)):
         return _PackedAttention.apply(q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, lengths_k, causal, scale, buckets)
     return _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, lengths_k, causal, scale, bias_table, buckets, False)[0]
 
@@ -426,6 +433,6 @@ def relative_position_bias(table, queries, keys, buckets, query_start=None):
     if table.shape[1] > 65535 or queries > 32 * 65535:
         raise ValueError("at most 65535 heads and 2097120 queries")
     L.require_cuda(table)
-    if (torch.is_grad_enabled() and table.requires_grad) or _has_tangent(table):
+    if (torch.is_grad_enabled() and table.requires_grad) or (forward_ad._current_level >= 0 and _has_tangent(table)):
         return _RelativeBias.apply(table, queries, keys, start, buckets)
     return _bias_forward(table, queries, keys, start, buckets)
