@@ -32,10 +32,16 @@
 // through shared memory measured slower (487 us), as did blocks of 64 columns
 // at 128 channels (893 -> 1,005 us for the step).
 //
-// Measured (8,192 causal tokens, 16 heads of 128 on 8, bf16): dq 0.36-0.39 ms,
-// dk and dv 0.48 ms; 32 images of 197-785 tokens, 6 heads of 64, fp16, with a
-// bias of 32 buckets: 94 and 83 us (without it both together 130; with a look-up
-// through the buckets, one chain of shuffles and a lane a bucket 108 and 94).
+// Measured: 8,192 causal tokens, 16 heads of 128 on 8, bf16: 0.81-0.90 ms for
+// both, the call repeated.  32 images of 197-785 tokens, 6 heads of 64, with a
+// bias of 32 buckets: 97 us for dq and 78 for dk and dv in fp16 (one launch at a
+// time); a bias adds 53 us to the 119 of the whole backward pass in bf16, and 54
+// to the 132 in fp16.  With a look-up through the buckets, one chain of shuffles
+// and a lane a bucket dq and dk with dv took 14 and 11 us more.
+//
+// delta takes out as the forward pass rounded it: its error, that of a mean of
+// rounded values, is not above that of the ds rounded beside it, and an fp32 out
+// would cost the forward pass twice its writes.
 #include <algorithm>
 
 #include "packed_tc.cuh"
@@ -81,7 +87,7 @@ __device__ __forceinline__ float pow2(int n) { return __int_as_float((127 + n) <
 // Rows of no sequence and unused keys are not looked at, and rows with an
 // infinity or a NaN do not count (their results show it in any case).
 // 32 images of 197-785 tokens, 6 heads of 64: 10 us (24 MB from a cold cache),
-// and the training step with a bias 231 -> 246 us.
+// and the training step with a bias 232 -> 236 us.
 __host__ __device__ constexpr int norm_tokens(int group) { return 256 / group; }
 constexpr int kNormKeys = 256;
 __global__ void __launch_bounds__(256) norms_kernel(const __grid_constant__ BwdParams p) {

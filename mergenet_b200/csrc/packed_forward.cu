@@ -27,12 +27,13 @@
 // one S a tile, and the tiles take turns: one's products run under the
 // other's softmax.  Blocks of 128 keys: with two S buffers of 64 keys instead
 // the products of 64 columns became the bound (16,384 causal tokens, 16 heads
-// of 128: 1.13 ms against 0.97-1.04 ms).
+// of 128, the same call repeated: 1.13 ms against 0.99-1.08 ms).
 //
-// Measured: 16,384 causal tokens, 16 heads of 128 on 4 key heads, bf16: 0.95
-// to 1.04 ms, 1,060-1,140 TFLOP/s; 128 images of 393-785 tokens, 6 heads of 64,
-// fp16: 0.19 ms; 64 tokens against caches of 700 to 8,192, 32 heads on 8 of 128:
-// 0.227 ms, 5.6 TB/s of the cache in use.
+// Measured among calls on other inputs: 16,384 causal tokens, 16 heads of 128
+// on 4 key heads, bf16: 1.09-1.11 ms, 990-1,010 TFLOP/s; 128 images of 393-785
+// tokens, 6 heads of 64, fp16: 0.185-0.19 ms; 64 tokens against caches of 700 to
+// 8,192, 32 heads on 8 of 128: 0.24-0.256 ms, 5.0-5.3 TB/s of the cache in use
+// (0.228 ms, 5.6 TB/s, repeated on one input).
 //
 // With few rows and many keys (SPLIT) the keys are divided over grid.y, and
 // within a CTA of two tile slots the blocks alternate between the slots; the

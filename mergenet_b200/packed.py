@@ -2,8 +2,8 @@
 of the relative position by distance buckets.
 
 ``packed_attention`` takes the sequences of a batch laid one behind the other
-(images left with different numbers of tokens after merging, documents,
-prompts, or one new token each against a cache) instead of the equal lengths
+(images of different sizes or numbers of kept tokens, documents, prompts, or one
+new token each against a cache) instead of the equal lengths
 of ``cross_attention`` and ``local_attention_packed``.  Heads may be grouped,
 the mask may be causal, and a learned table adds a bias that depends on the
 distance of query and key.  It is differentiable once, in reverse mode, in q,
