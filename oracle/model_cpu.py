@@ -89,7 +89,9 @@ def route_torch(x, metrics, r_list, geom, tau1=1.0, tau2=30.0):
         valid_row = allowed.any(-1)
         logits = (scores / tau1).masked_fill(~allowed, float("-inf"))
         safe = torch.where(valid_row[..., None], logits, torch.zeros_like(logits))
-        energy = torch.where(valid_row, torch.logsumexp(safe, -1).exp(), torch.zeros_like(valid_row, dtype=torch.float32))
+        # in 64 bits: the fp32 exponential's last bit goes by where the memory lies,
+        # and the soft top-k makes 3e-4 of the masses out of it
+        energy = torch.where(valid_row, torch.logsumexp(safe.double(), -1).exp().float(), torch.zeros_like(valid_row, dtype=torch.float32))
         row_khot = _thre_topk(energy, int(min(r, (t - 1) // 2)), tau2) * valid_row
         khot = torch.softmax(safe, -1) * allowed * row_khot[..., None]
         assign = khot / ((khot.sum(-1, keepdim=True) - 1).clamp_min(0) + 1)
